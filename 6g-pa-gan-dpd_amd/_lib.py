@@ -1,4 +1,5 @@
 """ctypes binding of libdpd_hip.so (the C ABI in include/dpd_hip.h)."""
+import contextlib
 import ctypes
 import os
 import threading
@@ -17,7 +18,7 @@ ERR_SHAPE = 2
 _lib = None
 _lock = threading.Lock()
 
-c_p, c_i, c_l, c_f, c_sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+c_p, c_i, c_l, c_f, c_d, c_sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double, ctypes.c_size_t
 
 # name -> argument types (all return int unless listed in _RESTYPES)
 PROTOTYPES = {
@@ -63,12 +64,24 @@ PROTOTYPES = {
     "dpd_q88_matrix_image_bytes": [],
     "dpd_q88_matrix_prepare": [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p],
     "dpd_q88_matrix_infer": [c_p, c_l, c_l, c_p, c_p, c_p, c_p],
+    "dpd_quantize_rows_int8": [c_p, c_i, c_l, c_l, c_l, c_p, c_l, c_p, c_p],
+    "dpd_int8_matmul_workspace_bytes": [c_l, c_l, c_l],
+    "dpd_int8_matmul": [c_p, c_l, c_p, c_p, c_l, c_p, c_p, c_i, c_l, c_l, c_l, c_p, c_i, c_l, c_p, c_sz, c_p],
+    "dpd_int8_row_bytes": [c_l],
+    "dpd_int8_linear_workspace_bytes": [c_l, c_l, c_l],
+    "dpd_int8_linear": [c_p, c_i, c_l, c_l, c_l, c_p, c_p, c_p, c_i, c_l, c_p, c_l, c_p, c_sz, c_p],
+    "dpd_int8_linear_backward_workspace_bytes": [c_l, c_l, c_l, c_i, c_i, c_i, c_i],
+    "dpd_int8_linear_backward": [c_p, c_i, c_l, c_l, c_l, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_sz, c_p],
+    "dpd_orthogonalize_workspace_bytes": [c_l, c_l, c_l, c_i],
+    "dpd_orthogonalize": [c_p, c_i, c_l, c_l, c_l, c_i, c_p, c_d, c_i, c_p, c_p, c_sz, c_p],
+    "dpd_muon_workspace_bytes": [c_i, c_p, c_p, c_i],
+    "dpd_muon_step": [c_i, c_p, c_p, c_p, c_p, c_p, c_i, c_d, c_d, c_i, c_d, c_i, c_p, c_d, c_i, c_p, c_sz, c_p],
     "dpd_workspace_bytes": [c_l],
     "dpd_set_option": [ctypes.c_char_p, c_i],
     "dpd_last_error": [],
     "dpd_version": [],
 }
-_RESTYPES = {"dpd_workspace_bytes": c_sz, "dpd_impair_workspace_bytes": c_sz, "dpd_q88_matrix_image_bytes": c_sz, "dpd_last_error": ctypes.c_char_p}
+_RESTYPES = {**{k: c_sz for k in PROTOTYPES if k.endswith("_workspace_bytes")}, "dpd_int8_row_bytes": c_l, "dpd_workspace_bytes": c_sz, "dpd_impair_workspace_bytes": c_sz, "dpd_q88_matrix_image_bytes": c_sz, "dpd_last_error": ctypes.c_char_p}
 
 
 def lib():
@@ -126,6 +139,16 @@ def fptr(t, dtype=torch.float32):
 def as_f32(t):
     t = t if t.dtype == torch.float32 else t.float()
     return t if t.is_contiguous() else t.contiguous()
+
+
+# element types of the entry points that take more than fp32 (DPD_F32, DPD_BF16, DPD_F16)
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def device(t):
+    """Context in which t's device is the current one (launches and torch's current stream go by it)."""
+    return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def stream():

@@ -20,6 +20,11 @@ ASAN = os.environ.get("DPD_ASAN", "") not in ("", "0")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-mllvm", "-amdgpu-mfma-vgpr-form=1",
          "-Wno-unused-result", "-I", os.path.join(os.path.dirname(HERE), "include")]
 
+# The tiled products and what belongs to them are compiled without packed fp32 instructions (some of their forms are
+# not reliable next to matrix instructions); the older kernels choose theirs by hand.
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FILE_FLAGS = {"int8_linear.hip": NO_PACKED, "orthogonal.hip": NO_PACKED}
+
 
 def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")))
@@ -47,7 +52,7 @@ def _build(lib_path, objdir, verbose, jobs):
     for src in sources():
         obj = os.path.join(objdir, os.path.basename(src) + ".o")
         objs.append(obj)
-        cmd = [HIPCC] + FLAGS + EXTRA + (["-Xarch_host", "-fsanitize=address", "-g"] if ASAN else []) + ["-c", src, "-o", obj]
+        cmd = [HIPCC] + FLAGS + FILE_FLAGS.get(os.path.basename(src), []) + EXTRA + (["-Xarch_host", "-fsanitize=address", "-g"] if ASAN else []) + ["-c", src, "-o", obj]
         if src.endswith(".cpp"):
             cmd.insert(1, "-x"); cmd.insert(2, "hip")
         if verbose:

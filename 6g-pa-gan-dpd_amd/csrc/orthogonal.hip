@@ -1,0 +1,535 @@
+// Orthogonalised updates: the quintic Newton-Schulz iteration
+//     X <- X / max(|X|_F, eps);   steps times:  A = X X^T,  X <- a X + (b A + c A A) X
+// on the short side of each matrix, and the optimiser step that uses it (momentum, iteration, update of the weights).
+//
+// Matrices of up to 64 x 128 run in one workgroup, in fp32 out of LDS.  Larger ones take three tiled products a step
+// (gemm_nt.h).  Their factors are fp16, scaled by powers of two so that the range is used: after the division by its
+// norm a matrix has entries around 1 / sqrt(r c) and singular values that stay below 4, so X is held times
+// S = 2^floor(log2 sqrt(r c)) (at most 2^14) and A, B = b A + c A A times 2^12.  One fp16 term has a relative rounding of
+// 2^-11, an eighth of that of bf16 inputs; two terms (the split form of gemm_nt.h) hold 22 bits and match an fp32
+// evaluation.  Sums are fp32 in the matrix cores, the norm is a sum of fp64.
+#include <cmath>
+#include <utility>
+#include "gemm_nt.h"
+
+namespace {
+
+constexpr float T_SCALE = 4096.f;
+constexpr int MAX_STEPS = 32, NORM_BLOCKS = 512;
+
+struct Coef {
+    float v[3 * MAX_STEPS];
+};
+
+// ---- what is orthogonalised, and where the result goes ------------------------------------------
+template <class T>
+struct FromTensor {                                   // a matrix of a batch
+    const T *x;
+    int64_t batch;
+    DEV float first(int z, int64_t i) const { return to_f32(x[z * batch + i]); }
+    DEV float again(int z, int64_t i) const { return to_f32(x[z * batch + i]); }
+};
+template <class T>
+struct FromMomentum {                                 // g and the momentum, which the first pass updates
+    const T *g;
+    float *m;
+    float mu;
+    int nesterov;
+    DEV float first(int, int64_t i) const {
+        m[i] = mu * m[i] + to_f32(g[i]);
+        return again(0, i);
+    }
+    DEV float again(int, int64_t i) const { return nesterov ? to_f32(g[i]) + mu * m[i] : m[i]; }
+};
+template <class T>
+struct ToTensor {
+    T *out;
+    int64_t batch;
+    DEV void put(int z, int64_t i, float v) const { out[z * batch + i] = from_f32<T>(v); }
+};
+template <class T>
+struct ToWeights {
+    T *p;
+    float keep, factor;                               // 1 - lr wd, lr sqrt(max(1, rows / cols))
+    DEV void put(int, int64_t i, float v) const { p[i] = from_f32<T>(to_f32(p[i]) * keep - factor * v); }
+};
+
+DEV double block_sum_d(double v, double *red) {       // over the 256 threads of a workgroup, the same value in all
+    v = wave_sum_d(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ---- small matrices --------------------------------------------------------------------------
+constexpr int SMALL_R = 64, SMALL_C = 128, XS = SMALL_C + 1, AS = SMALL_R + 1;
+
+// One workgroup, one matrix: r <= c after the transposition, X [r][c], A and B [r][r] in LDS.  A thread forms 4 x 4
+// blocks of a product (8 LDS reads for 16 FMAs).
+template <class From, class To>
+DEV void small_iterate(const From &from, const To &to, int z, int rows, int cols, const Coef &coef, int steps, double eps, float *lds) {
+    __shared__ double red[4];
+    float *X = lds, *A = X + SMALL_R * XS, *B = A + SMALL_R * AS;
+    const bool wide = rows <= cols;
+    const int r = wide ? rows : cols, c = wide ? cols : rows, n = rows * cols, t = threadIdx.x;
+    const int r4 = (r + 3) >> 2, c4 = (c + 3) >> 2;
+    for (int e = t; e < SMALL_R * XS + 2 * SMALL_R * AS; e += 256) lds[e] = 0.f;
+    __syncthreads();
+    double s = 0.0;
+    for (int e = t; e < n; e += 256) {
+        const int i = e / cols, j = e - i * cols;
+        const float v = from.first(z, e);
+        X[wide ? i * XS + j : j * XS + i] = v;
+        s += (double)v * (double)v;
+    }
+    const double norm = sqrt(block_sum_d(s, red)), inv = 1.0 / (norm > eps ? norm : (norm == norm ? eps : norm));
+    for (int e = t; e < n; e += 256) {
+        const int i = e / cols, j = e - i * cols, at = wide ? i * XS + j : j * XS + i;
+        X[at] = (float)((double)X[at] * inv);
+    }
+    __syncthreads();
+    for (int k = 0; k < steps; ++k) {
+        const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
+        for (int e = t; e < r4 * r4; e += 256) {               // A = X X^T
+            const int i = (e / r4) * 4, j = (e % r4) * 4;
+            float acc[4][4] = {};
+            for (int q = 0; q < c; ++q) {
+                float u[4], v[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) u[d] = X[(i + d) * XS + q], v[d] = X[(j + d) * XS + q];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) acc[d][f] = __builtin_fmaf(u[d], v[f], acc[d][f]);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) A[(i + d) * AS + j + f] = acc[d][f];
+        }
+        __syncthreads();
+        for (int e = t; e < r4 * r4; e += 256) {               // B = b A + c A A
+            const int i = (e / r4) * 4, j = (e % r4) * 4;
+            float acc[4][4] = {};
+            for (int q = 0; q < r; ++q) {
+                float u[4], v[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) u[d] = A[(i + d) * AS + q], v[d] = A[q * AS + j + d];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) acc[d][f] = __builtin_fmaf(u[d], v[f], acc[d][f]);
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) B[(i + d) * AS + j + f] = __builtin_fmaf(cc, acc[d][f], cb * A[(i + d) * AS + j + f]);
+        }
+        __syncthreads();
+        float next[2][4][4];                                   // X <- a X + B X, written once every thread has read X
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = t + h * 256;
+            if (e >= r4 * c4) break;
+            const int i = (e / c4) * 4, j = (e % c4) * 4;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) next[h][d][f] = ca * X[(i + d) * XS + j + f];
+            for (int q = 0; q < r; ++q) {
+                float u[4], v[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) u[d] = B[(i + d) * AS + q], v[d] = X[q * XS + j + d];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) next[h][d][f] = __builtin_fmaf(u[d], v[f], next[h][d][f]);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = t + h * 256;
+            if (e >= r4 * c4) break;
+            const int i = (e / c4) * 4, j = (e % c4) * 4;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int f = 0; f < 4; ++f) X[(i + d) * XS + j + f] = next[h][d][f];
+        }
+        __syncthreads();
+    }
+    for (int e = t; e < n; e += 256) {
+        const int i = e / cols, j = e - i * cols;
+        to.put(z, e, X[wide ? i * XS + j : j * XS + i]);
+    }
+}
+
+constexpr int SMALL_LDS = SMALL_R * XS + 2 * SMALL_R * AS;
+
+template <class T>
+__global__ __launch_bounds__(256) void k_small(FromTensor<T> from, ToTensor<T> to, int rows, int cols, Coef coef, int steps, double eps) {
+    __shared__ float lds[SMALL_LDS];
+    small_iterate(from, to, blockIdx.x, rows, cols, coef, steps, eps, lds);
+}
+
+constexpr int TABLE = 24;              // matrices of one launch: the table travels with the kernel's arguments
+struct SmallTable {
+    void *p[TABLE];
+    const void *g[TABLE];
+    float *m[TABLE];
+    int rows[TABLE], cols[TABLE];
+    float factor[TABLE];
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
+    __shared__ float lds[SMALL_LDS];
+    const int z = blockIdx.x;
+    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z]}, 0, tab.rows[z],
+                  tab.cols[z], coef, steps, eps, lds);
+}
+
+// ---- large matrices ----------------------------------------------------------------------------
+// A factor in the workspace: rows of fp16, or of blocks of 32 leading halves and 32 remainders (SPLIT).
+struct Image {
+    char *base;
+    int64_t ld, batch;                 // bytes
+};
+DEV int64_t img_row(const Image &im, int z, int64_t row) { return z * im.batch + row * im.ld; }
+template <bool SPLIT>
+DEV int64_t img_col(int col) { return SPLIT ? (int64_t)(col >> 5) * 128 + (col & 31) * 2 : (int64_t)col * 2; }
+
+template <bool SPLIT>
+DEV f32x4_t img_load4(const Image &im, int z, int64_t row, int col) {
+    const char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
+    const nt::f16x4 h = *(const nt::f16x4 *)p;
+    f32x4_t v = {(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    if (SPLIT) {
+        const nt::f16x4 l = *(const nt::f16x4 *)(p + 64);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += (float)l[i];
+    }
+    return v;
+}
+template <bool SPLIT>
+DEV void img_store4(const Image &im, int z, int64_t row, int col, f32x4_t v) {
+    char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
+    const nt::f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    *(nt::f16x4 *)p = h;
+    if (SPLIT) *(nt::f16x4 *)(p + 64) = nt::f16x4{(_Float16)(v[0] - (float)h[0]), (_Float16)(v[1] - (float)h[1]), (_Float16)(v[2] - (float)h[2]), (_Float16)(v[3] - (float)h[3])};
+}
+template <bool SPLIT>
+DEV void img_store1(const Image &im, int z, int64_t row, int col, float v) {
+    char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
+    const _Float16 h = (_Float16)v;
+    *(_Float16 *)p = h;
+    if (SPLIT) *(_Float16 *)(p + 64) = (_Float16)(v - (float)h);
+}
+
+// Sum of squares of each matrix (and, for the optimiser, the new momentum): NORM_BLOCKS fp64 partial sums each.
+template <class From>
+__global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__restrict__ part) {
+    __shared__ double red[4];
+    const int z = blockIdx.z;
+    double s = 0.0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const double v = (double)from.first(z, i);
+        s += v * v;
+    }
+    s = block_sum_d(s, red);
+    if (threadIdx.x == 0) part[z * NORM_BLOCKS + blockIdx.x] = s;
+}
+
+// X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.
+template <class From, bool SPLIT>
+__global__ __launch_bounds__(256) void k_prepare(From from, int rows, int cols, const double *__restrict__ part, int blocks, double eps, double scale,
+                                                 Image P, Image Q) {
+    __shared__ double red[4];
+    __shared__ float tile[64][65];
+    const int z = blockIdx.z, t = threadIdx.x;
+    double s = 0.0;
+    for (int i = t; i < blocks; i += 256) s += part[z * NORM_BLOCKS + i];
+    const double norm = sqrt(block_sum_d(s, red)), inv = scale / (norm > eps ? norm : (norm == norm ? eps : norm));
+    const bool wide = rows <= cols;
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;          // of x
+    for (int e = t; e < 4096; e += 256) {
+        const int i = e >> 6, j = e & 63;
+        tile[i][j] = (r0 + i < rows && c0 + j < cols) ? (float)((double)from.again(z, (int64_t)(r0 + i) * cols + c0 + j) * inv) : 0.f;
+    }
+    __syncthreads();
+    const Image &same = wide ? P : Q, &flip = wide ? Q : P;        // the image in x's orientation, and the other one
+    for (int e = t; e < 1024; e += 256) {
+        const int i = e >> 4, j = (e & 15) * 4;
+        const int64_t end_c = SPLIT ? same.ld / 4 : same.ld / 2, end_r = SPLIT ? flip.ld / 4 : flip.ld / 2;
+        if (r0 + i < rows && c0 + j < end_c) img_store4<SPLIT>(same, z, r0 + i, c0 + j, f32x4_t{tile[i][j], tile[i][j + 1], tile[i][j + 2], tile[i][j + 3]});
+        if (c0 + i < cols && r0 + j < end_r) img_store4<SPLIT>(flip, z, c0 + i, r0 + j, f32x4_t{tile[j][i], tile[j + 1][i], tile[j + 2][i], tile[j + 3][i]});
+    }
+}
+
+// zeros behind column `from` of the rows of up to three images (16-bit words; both halves of a block in the split form)
+template <bool SPLIT>
+__global__ __launch_bounds__(256) void k_zero_pads(Image a, int64_t ra, Image b, int64_t rb, Image c, int64_t rc, int from) {
+    const int z = blockIdx.z, pad = (int)((SPLIT ? a.ld / 4 : a.ld / 2) - from);
+    const int64_t total = (ra + rb + rc) * pad;
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
+        int64_t row = e / pad;
+        const int col = from + (int)(e - row * pad);
+        const Image *im = &a;
+        if (row >= ra) row -= ra, im = &b;
+        if (im == &b && row >= rb) row -= rb, im = &c;
+        img_store1<SPLIT>(*im, z, row, col, 0.f);
+    }
+}
+
+template <bool SPLIT>
+struct GramOut {                       // A = X X^T (times T_SCALE)
+    Image A;
+    float scale;
+    int N;
+    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
+        f32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? acc[i] * scale : 0.f;
+        img_store4<SPLIT>(A, z, m, n, v);
+    }
+};
+template <bool SPLIT>
+struct PolyOut {                       // B = b A + c A A (times T_SCALE)
+    Image A, B;
+    float b, c;
+    int N;
+    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
+        const f32x4_t a = img_load4<SPLIT>(A, z, m, n);
+        f32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? __builtin_fmaf(c, acc[i] * (1.f / T_SCALE), b * a[i]) : 0.f;
+        img_store4<SPLIT>(B, z, m, n, v);
+    }
+};
+template <bool SPLIT>
+struct NextOut {                       // X <- a X + B X into P (in place: a tile reads its own entries only) and the other Q
+    Image P, Q;
+    float a;
+    int N;
+    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
+        const f32x4_t x = img_load4<SPLIT>(P, z, m, n);
+        f32x4_t v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? __builtin_fmaf(a, x[i], acc[i] * (1.f / T_SCALE)) : 0.f;
+        img_store4<SPLIT>(P, z, m, n, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) img_store1<SPLIT>(Q, z, n + i, m, v[i]);
+    }
+};
+template <bool SPLIT, class To>
+struct LastOut {                       // the last step: X in the orientation of the result (P, or Q for tall matrices)
+    Image X;
+    float a, scale;                    // scale = 1 / S
+    To to;
+    int N;
+    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
+        const f32x4_t x = img_load4<SPLIT>(X, z, m, n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < N) to.put(z, (int64_t)m * N + n + i, __builtin_fmaf(a, x[i], acc[i] * (1.f / T_SCALE)) * scale);
+    }
+};
+
+struct Plan {
+    int64_t r, c, part, p, q0, q1, a, b, total;
+    int64_t ld_r, ld_c;                // bytes of a row along the short and the long side
+    Plan(int64_t batch, int64_t rows, int64_t cols, bool split) {
+        r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
+        ld_r = split ? nt::pad_to(r, 32) * 4 : nt::pad_to(r, 64) * 2;
+        ld_c = split ? nt::pad_to(c, 32) * 4 : nt::pad_to(c, 64) * 2;
+        int64_t at = 0;
+        auto take = [&](int64_t bytes) {
+            const int64_t here = at;
+            at += nt::pad_to(bytes, 256);
+            return here;
+        };
+        part = take(batch * NORM_BLOCKS * 8);
+        p = take(batch * r * ld_c);
+        q0 = take(batch * c * ld_r);
+        q1 = take(batch * c * ld_r);
+        a = take(batch * r * ld_r);
+        b = take(batch * r * ld_r);
+        total = at;
+    }
+};
+
+bool is_small(int64_t rows, int64_t cols) {
+    const int64_t r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
+    return r <= SMALL_R && c <= SMALL_C;
+}
+
+template <bool SPLIT, class From, class To>
+int large(const From &from, const To &to, int batch, int64_t rows, int64_t cols, int steps, const float *coef, double eps, char *ws, hipStream_t st) {
+    constexpr int KIND = SPLIT ? nt::F16_SPLIT : nt::F16;
+    const Plan pl(batch, rows, cols, SPLIT);
+    const int r = (int)pl.r, c = (int)pl.c;
+    const bool wide = rows <= cols;
+    double *part = (double *)(ws + pl.part);
+    const Image P{ws + pl.p, pl.ld_c, r * pl.ld_c}, A{ws + pl.a, pl.ld_r, r * pl.ld_r}, B{ws + pl.b, pl.ld_r, r * pl.ld_r};
+    Image Q{ws + pl.q0, pl.ld_r, c * pl.ld_r}, Q2{ws + pl.q1, pl.ld_r, c * pl.ld_r};
+    int log_s = 0;
+    while (log_s < 14 && (int64_t)1 << (2 * log_s + 2) <= (int64_t)r * c) ++log_s;
+    const float S = (float)(1 << log_s);
+    const int blocks = grid_for(rows * cols, 256 * 8, NORM_BLOCKS);
+    hipLaunchKernelGGL((k_norm<From>), dim3(blocks, 1, batch), dim3(256), 0, st, from, rows * cols, part);
+    DPD_LAUNCH_CHECK();
+    hipLaunchKernelGGL((k_prepare<From, SPLIT>), dim3((unsigned)((cols + 63) / 64), (unsigned)((rows + 63) / 64), batch), dim3(256), 0, st, from, (int)rows,
+                       (int)cols, part, blocks, eps, (double)S, P, Q);
+    DPD_LAUNCH_CHECK();
+    const int64_t pad = (SPLIT ? pl.ld_r / 4 : pl.ld_r / 2) - r;
+    if (pad) {
+        hipLaunchKernelGGL((k_zero_pads<SPLIT>), dim3(grid_for((2 * r + c) * pad, 256), 1, batch), dim3(256), 0, st, A, (int64_t)r, B, (int64_t)r, Q2, (int64_t)c, r);
+        DPD_LAUNCH_CHECK();
+    }
+    auto product = [&](const Image &x, int M, const Image &y, int N, const auto &epi) {
+        nt::Args g{};
+        g.a = x.base, g.lda = x.ld, g.a_batch = x.batch, g.b = y.base, g.ldb = y.ld, g.b_batch = y.batch, g.M = M, g.N = N;
+        g.steps = g.wrap = (int)(x.ld / nt::STEP), g.tail = nt::STEP;
+        return nt::product<KIND>(g, batch, epi, st);
+    };
+    for (int k = 0; k < steps; ++k) {
+        const float *f = coef + 3 * k;
+        int rc = product(P, r, P, r, GramOut<SPLIT>{A, T_SCALE / (S * S), r});
+        if (!rc) rc = product(A, r, A, r, PolyOut<SPLIT>{A, B, f[1], f[2], r});
+        if (!rc && k + 1 < steps) {
+            rc = product(B, r, Q, c, NextOut<SPLIT>{P, Q2, f[0], c});
+            std::swap(Q, Q2);
+        } else if (!rc) {
+            rc = wide ? product(B, r, Q, c, LastOut<SPLIT, To>{P, f[0], 1.f / S, to, c}) : product(Q, c, B, r, LastOut<SPLIT, To>{Q, f[0], 1.f / S, to, r});
+        }
+        if (rc) return rc;
+    }
+    return DPD_OK;
+}
+
+// The largest singular value that `steps` steps can reach from 1, and the largest |b s^2 + c s^4| on the way, must stay
+// inside the range of the scaled fp16 factors.
+int check_iteration(const char *who, int steps, const float *coef, double eps) {
+    DPD_REQUIRE(steps >= 1 && steps <= MAX_STEPS && coef, DPD_ERR_SHAPE, "%s: %d steps not in 1..%d", who, steps, MAX_STEPS);
+    DPD_REQUIRE(eps > 0.0 && eps < 1e300, DPD_ERR_SHAPE, "%s: eps must be positive and finite", who);
+    double top = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        const double a = coef[3 * k], b = coef[3 * k + 1], c = coef[3 * k + 2];
+        double next = 0.0, poly = 0.0;
+        for (int i = 1; i <= 64; ++i) {
+            const double s = top * i / 64, s2 = s * s, p = b * s2 + c * s2 * s2;
+            next = fmax(next, fabs(s * (a + p)));
+            poly = fmax(poly, fabs(p));
+        }
+        next *= 1.02;
+        DPD_REQUIRE(std::isfinite(a) && std::isfinite(b) && std::isfinite(c) && next <= 3.9 && poly <= 15.0, DPD_ERR_SHAPE, "%s: step %d with coefficients (%g, %g, %g) can take singular values out of range", who,
+                    k, a, b, c);
+        top = fmax(next, 1e-3);
+    }
+    return DPD_OK;
+}
+
+int check_matrix(const char *who, int64_t rows, int64_t cols) {
+    DPD_REQUIRE(rows >= 0 && cols >= 0, DPD_ERR_INVALID_ARG, "%s: negative size", who);
+    DPD_REQUIRE((rows < cols ? cols : rows) * 4 <= nt::MAX_ROW_BYTES - 512, DPD_ERR_SHAPE, "%s: a side of %lld is too long", who,
+                (long long)(rows < cols ? cols : rows));
+    return DPD_OK;
+}
+
+}  // namespace
+
+extern "C" size_t dpd_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int accurate) {
+    if (batch <= 0 || rows <= 0 || cols <= 0 || is_small(rows, cols)) return 256;
+    return (size_t)Plan(batch, rows, cols, accurate != 0).total + 256;
+}
+
+extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *h_coef, double eps,
+                                 int accurate, void *out, void *ws, size_t ws_bytes, void *stream) {
+    DPD_REQUIRE(type == DPD_F32 || type == DPD_BF16 || type == DPD_F16, DPD_ERR_INVALID_ARG, "orthogonalize: element type %d", type);
+    DPD_REQUIRE(batch >= 0 && batch <= INT32_MAX, DPD_ERR_INVALID_ARG, "orthogonalize: batch");
+    if (const int rc = check_matrix("orthogonalize", rows, cols)) return rc;
+    if (const int rc = check_iteration("orthogonalize", steps, h_coef, eps)) return rc;
+    if (batch == 0 || rows == 0 || cols == 0) return DPD_OK;
+    DPD_REQUIRE(x && out, DPD_ERR_INVALID_ARG, "orthogonalize: null pointer");
+    hipStream_t st = as_stream(stream);
+    Coef coef{};
+    for (int i = 0; i < 3 * steps; ++i) coef.v[i] = h_coef[i];
+    if (is_small(rows, cols))
+        return with_type(type, [&](auto t) {
+            using T = decltype(t);
+            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols}, ToTensor<T>{(T *)out, rows * cols},
+                               (int)rows, (int)cols, coef, steps, eps);
+            DPD_LAUNCH_CHECK();
+            return DPD_OK;
+        });
+    DPD_REQUIRE(batch <= 65535, DPD_ERR_SHAPE, "orthogonalize: %lld matrices of this size in one call (at most 65535)", (long long)batch);
+    DPD_REQUIRE(ws && ws_bytes >= dpd_orthogonalize_workspace_bytes(batch, rows, cols, accurate), DPD_ERR_WORKSPACE, "orthogonalize: workspace");
+    char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        const FromTensor<T> from{(const T *)x, rows * cols};
+        const ToTensor<T> to{(T *)out, rows * cols};
+        return accurate ? large<true>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st)
+                        : large<false>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st);
+    });
+}
+
+extern "C" size_t dpd_muon_workspace_bytes(int n, const int64_t *h_rows, const int64_t *h_cols, int accurate) {
+    size_t most = 256;
+    for (int i = 0; i < n; ++i) {
+        const size_t b = dpd_orthogonalize_workspace_bytes(1, h_rows[i], h_cols[i], accurate);
+        most = b > most ? b : most;
+    }
+    return most;
+}
+
+extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, float *const *h_m, const int64_t *h_rows, const int64_t *h_cols, int p_type,
+                             double lr, double momentum, int nesterov, double weight_decay, int steps, const float *h_coef, double eps, int accurate, void *ws,
+                             size_t ws_bytes, void *stream) {
+    DPD_REQUIRE(n >= 0 && (n == 0 || (h_p && h_g && h_m && h_rows && h_cols)), DPD_ERR_INVALID_ARG, "muon_step: null pointer");
+    DPD_REQUIRE(p_type == DPD_F32 || p_type == DPD_BF16 || p_type == DPD_F16, DPD_ERR_INVALID_ARG, "muon_step: element type %d", p_type);
+    if (const int rc = check_iteration("muon_step", steps, h_coef, eps)) return rc;
+    bool any_large = false;
+    for (int i = 0; i < n; ++i) {                  // every matrix is looked at before the first one changes
+        if (const int rc = check_matrix("muon_step", h_rows[i], h_cols[i])) return rc;
+        const bool empty = h_rows[i] == 0 || h_cols[i] == 0;
+        DPD_REQUIRE(empty || (h_p[i] && h_g[i] && h_m[i]), DPD_ERR_INVALID_ARG, "muon_step: null pointer (matrix %d)", i);
+        any_large = any_large || (!empty && !is_small(h_rows[i], h_cols[i]));
+    }
+    DPD_REQUIRE(!any_large || (ws && ws_bytes >= dpd_muon_workspace_bytes(n, h_rows, h_cols, accurate)), DPD_ERR_WORKSPACE, "muon_step: workspace");
+    char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+    hipStream_t st = as_stream(stream);
+    Coef coef{};
+    for (int i = 0; i < 3 * steps; ++i) coef.v[i] = h_coef[i];
+    const float keep = (float)(1.0 - lr * weight_decay), mu = (float)momentum;
+    return with_type(p_type, [&](auto t) {
+        using T = decltype(t);
+        SmallTable tab{};
+        int used = 0;
+        auto flush = [&]() {
+            if (used) hipLaunchKernelGGL((k_small_muon<T>), dim3(used), dim3(256), 0, st, tab, mu, nesterov, keep, coef, steps, eps);
+            used = 0;
+            DPD_LAUNCH_CHECK();
+            return DPD_OK;
+        };
+        for (int i = 0; i < n; ++i) {
+            const int64_t rows = h_rows[i], cols = h_cols[i];
+            if (rows == 0 || cols == 0) continue;
+            const float factor = (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0));
+            if (!is_small(rows, cols)) {
+                const FromMomentum<T> from{(const T *)h_g[i], h_m[i], mu, nesterov};
+                const ToWeights<T> to{(T *)h_p[i], keep, factor};
+                const int rc = accurate ? large<true>(from, to, 1, rows, cols, steps, coef.v, eps, w, st) : large<false>(from, to, 1, rows, cols, steps, coef.v, eps, w, st);
+                if (rc) return rc;
+                continue;
+            }
+            tab.p[used] = h_p[i], tab.g[used] = h_g[i], tab.m[used] = h_m[i], tab.rows[used] = (int)rows, tab.cols[used] = (int)cols, tab.factor[used] = factor;
+            if (++used == TABLE)
+                if (const int rc = flush()) return rc;
+        }
+        return flush();
+    });
+}

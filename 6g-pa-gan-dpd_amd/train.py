@@ -147,6 +147,14 @@ def create_models(config: dict, qat: bool, device):
 def create_optimizers(gen, disc, config: dict):
     o = config["training"]["optimizer"]
     kw = dict(betas=tuple(o.get("betas", [0.0, 0.9])), weight_decay=float(o.get("weight_decay", 1e-5)), fused=True)
+    kind = str(o.get("type", "adam")).lower()
+    if kind == "muon":           # the weight matrices by orthogonalised momentum, the biases by Adam as below
+        from .optim import Muon
+        mk = lambda net, lr: Muon(net.parameters(), lr=float(o.get("lr_matrix", 2e-3)), momentum=float(o.get("momentum", 0.95)),
+                                  weight_decay=kw["weight_decay"], adam=dict(kw, lr=lr))
+        return mk(gen, float(o.get("lr_generator", 1e-4))), mk(disc, float(o.get("lr_discriminator", 1e-4)))
+    if kind != "adam":
+        raise ValueError(f"optimizer type {kind!r} is neither 'adam' nor 'muon'")
     return (torch.optim.Adam(gen.parameters(), lr=float(o.get("lr_generator", 1e-4)), **kw),
             torch.optim.Adam(disc.parameters(), lr=float(o.get("lr_discriminator", 1e-4)), **kw))
 
@@ -206,6 +214,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--seq-len", type=int, default=1029, help="row length L + 5 (L a power of two for the ACPR term)")
     p.add_argument("--rows", type=int, default=4096, help="synthetic training rows per rank")
     p.add_argument("--stage1-epochs", type=int, default=None, help="supervised epochs before the CWGAN-GP epochs")
+    p.add_argument("--optimizer", type=str, default=None, choices=["adam", "muon"],
+                   help="muon: orthogonalised momentum for the weight matrices, Adam for the biases (default: the configuration's, adam)")
     p.add_argument("--augment", type=float, default=0.0, help="per-epoch augmentation strength of the input rows (0 = off)")
     return p
 
@@ -225,6 +235,8 @@ def main(argv=None) -> Dict[str, float]:
         tr["epochs"] = args.epochs
     if args.batch_size:
         tr["batch_size"] = args.batch_size
+    if args.optimizer:
+        tr["optimizer"] = dict(tr["optimizer"], type=args.optimizer)
     if args.stage1_epochs is not None:
         tr["stage1_epochs"] = args.stage1_epochs
     if not torch.cuda.is_available() or not args.device.startswith("cuda"):

@@ -10,6 +10,7 @@ from typing import Callable, Dict, Optional
 import torch
 
 from . import _lib as L
+from .optim import Muon  # noqa: F401
 
 # fused: the whole update of all parameter tensors in one launch (same arithmetic as the reference's default Adam)
 ADAM = dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True)

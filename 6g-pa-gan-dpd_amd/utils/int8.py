@@ -1,0 +1,228 @@
+"""The linear layer in 8 bits, with one scale for each token and each output channel (csrc/int8_linear.hip).
+
+`QuantizedLinear` quantises with fixed power-of-two scales; here the scales follow the data, so that wide layers keep
+7 bits of every row.  `quantize_rows_int8` and `int8_matmul` are the two parts, `int8_linear` / `Int8Linear` train through
+them with the straight-through estimator, `Int8Inference` serves weights that are quantised once.  The reference has no
+counterpart."""
+from typing import Dict, Optional, Tuple
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+TYPES = L.TYPES
+
+
+def _type(t: torch.Tensor, what: str) -> int:
+    try:
+        return TYPES[t.dtype]
+    except KeyError:
+        raise RuntimeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}") from None
+
+
+def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """x as rows [M, K] whose elements lie one behind the other, and the row stride: x itself where its layout allows."""
+    if x.dim() == 0:
+        raise ValueError("expected at least one dimension")
+    k = x.shape[-1]
+    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= k:
+        return x, x.stride(0)
+    return x.contiguous().view(-1, k) if x.numel() else x.new_empty(x.shape[:-1].numel(), k), k
+
+
+def _check_scale(s: torch.Tensor, rows: int, device, what: str) -> torch.Tensor:
+    if s.dtype != torch.float32 or s.numel() != rows or s.device != device:
+        raise ValueError(f"{what} must be {rows} float32 values on {device}, got {tuple(s.shape)} {s.dtype} on {s.device}")
+    return s.contiguous()
+
+
+def _check_bias(b: Optional[torch.Tensor], n: int, device) -> Tuple[Optional[torch.Tensor], int]:
+    if b is None:
+        return None, 0
+    if b.dim() != 1 or b.shape[0] != n or b.device != device:
+        raise ValueError(f"bias must be {n} values on {device}, got {tuple(b.shape)} on {b.device}")
+    return b.contiguous(), _type(b, "bias")
+
+
+def _quantize(x2: torch.Tensor, ldx: int, ldq: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    m, k = x2.shape
+    q = torch.empty(m, ldq, dtype=torch.int8, device=x2.device)
+    s = torch.empty(m, dtype=torch.float32, device=x2.device)
+    L.call("dpd_quantize_rows_int8", L.c_p(x2.data_ptr()), _type(x2, "x"), m, k, ldx, L.c_p(q.data_ptr()), ldq, L.c_p(s.data_ptr()), L.stream())
+    return q, s
+
+
+def _row_bytes(k: int) -> int:
+    return (k + 127) // 128 * 128
+
+
+def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of the rows of x [..., K]: scale = max(max|row|, 2^-100) / 127 in fp32, q = round-half-even(row / scale)
+    as int8.  A row that holds a NaN or an infinity gets the scale NaN and zeros, so every product with it is NaN."""
+    L.need_gpu(x)
+    x = x.detach()
+    x2, ldx = _rows(x)
+    with L.device(x):
+        q, s = _quantize(x2, ldx, x2.shape[1])
+    return q.view(x.shape), s.view(x.shape[:-1])
+
+
+def _matmul(a, lda, sa, b, ldb, sb, bias, bias_type, m, n, k, dtype):
+    out = torch.empty(m, n, dtype=dtype, device=a.device)
+    ws = None
+    nbytes = 0
+    if k % 16 or lda % 16 or ldb % 16 or a.data_ptr() % 16 or b.data_ptr() % 16:
+        nbytes = L.lib().dpd_int8_matmul_workspace_bytes(m, n, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+    L.call("dpd_int8_matmul", L.c_p(a.data_ptr()), lda, L.c_p(sa.data_ptr()), L.c_p(b.data_ptr()), ldb, L.c_p(sb.data_ptr()),
+           L.c_p(bias.data_ptr() if bias is not None else 0), bias_type, m, n, k, L.c_p(out.data_ptr()), TYPES[dtype], n,
+           L.c_p(ws.data_ptr() if ws is not None else 0), nbytes, L.stream())
+    return out
+
+
+def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """a [..., K] int8 with one scale a row, b [N, K] int8 with one scale a row: (a b^T) a_scale b_scale + bias as [..., N].
+    The sum is exact (K <= 131071); scales and bias enter in fp32, and the result is rounded once."""
+    L.need_gpu(a, a_scale, b, b_scale, bias)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise RuntimeError(f"int8_matmul takes int8 matrices, got {a.dtype} and {b.dtype}")
+    if out_dtype not in TYPES:
+        raise RuntimeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1] or a.device != b.device:
+        raise ValueError(f"cannot multiply rows of {tuple(a.shape)} on {a.device} with rows of {tuple(b.shape)} on {b.device}")
+    a2, lda = _rows(a)
+    b2, ldb = _rows(b)
+    m, n, k = a2.shape[0], b2.shape[0], b2.shape[1]
+    sa, sb = _check_scale(a_scale, m, a.device, "a_scale"), _check_scale(b_scale, n, a.device, "b_scale")
+    bc, bt = _check_bias(bias, n, a.device)
+    with L.device(a):
+        return _matmul(a2, lda, sa, b2, ldb, sb, bc, bt, m, n, k, out_dtype).view(*a.shape[:-1], n)
+
+
+class _Int8LinearFn(torch.autograd.Function):
+    """Both factors quantised on the way; the backward reads the 8-bit factors, so x and the weight are not kept."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        x2, ldx = _rows(x)
+        w2, ldw = _rows(weight)
+        (m, k), n = x2.shape, w2.shape[0]
+        ld = _row_bytes(k)
+        with L.device(x):
+            qx, sx = _quantize(x2, ldx, ld)
+            qw, sw = _quantize(w2, ldw, ld)
+            bc, bt = _check_bias(bias, n, x.device)
+            out = _matmul(qx, ld, sx, qw, ld, sw, bc, bt, m, n, ld, x.dtype)      # both images carry zeros behind the rows
+        ctx.save_for_backward(qx, sx, qw, sw)
+        ctx.sizes, ctx.lead, ctx.types = (m, n, k, ld), x.shape[:-1], (x.dtype, weight.dtype, bias.dtype if bias is not None else None)
+        return out.view(*x.shape[:-1], n)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        qx, sx, qw, sw = ctx.saved_tensors
+        m, n, k, ld = ctx.sizes
+        tx, tw, tb = ctx.types
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        need_b = tb is not None and ctx.needs_input_grad[2]
+        dev = qx.device
+        g2, ldg = _rows(gy)
+        gx = torch.empty(m, k, dtype=tx, device=dev) if need_x else None
+        gw = torch.empty(n, k, dtype=tw, device=dev) if need_w else None
+        gb = torch.empty(n, dtype=tb, device=dev) if need_b else None
+        ptr = lambda t: L.c_p(t.data_ptr() if t is not None else 0)
+        t = TYPES[tx]
+        with L.device(qx):
+            nbytes = L.lib().dpd_int8_linear_backward_workspace_bytes(m, n, k, t, need_x, need_w, need_b)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            L.call("dpd_int8_linear_backward", ptr(g2), t, m, n, k, ldg, ptr(qx), ld, ptr(sx), ptr(qw), ld, ptr(sw), ptr(gx), ptr(gw), TYPES[tw],
+                   ptr(gb), TYPES[tb] if need_b else 0, ptr(ws), nbytes, L.stream())
+        return gx.view(*ctx.lead, k) if need_x else None, gw, gb
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q(x) q(weight)^T + bias in the type of x, both factors quantised by rows in this call; differentiable in x, weight
+    and bias with the straight-through estimator (the quantisers count as the identity).  x [..., K], weight [N, K]."""
+    L.need_gpu(x, weight, bias)
+    _type(x, "x")
+    _type(weight, "weight")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.device != weight.device:
+        raise ValueError(f"cannot apply a weight of shape {tuple(weight.shape)} on {weight.device} to {tuple(x.shape)} on {x.device}")
+    _check_bias(bias, weight.shape[0], x.device)
+    return _Int8LinearFn.apply(x, weight, bias)
+
+
+class Int8Linear(nn.Module):
+    """A linear layer trained through its 8-bit form (see `int8_linear`); the weight stays in floating point."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.weight = nn.Parameter(torch.randn(out_features, in_features) * 0.1)
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(out_features))
+        else:
+            self.register_parameter("bias", None)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int8_linear(x, self.weight, self.bias)
+
+    @torch.no_grad()
+    def get_quantized_weights(self) -> Dict[str, torch.Tensor]:
+        """weight int8 [out, in], scale fp32 [out] and the bias: what `Int8Inference` serves."""
+        q, s = quantize_rows_int8(self.weight)
+        out = {"weight": q, "scale": s}
+        if self.bias is not None:
+            out["bias"] = self.bias.detach().clone()
+        return out
+
+
+class Int8Inference:
+    """Serves a linear layer from 8-bit weights: tokens are quantised on the way.  `weights`: "weight" int8 [N, K],
+    "scale" float32 [N] and, optionally, "bias" [N], as `Int8Linear.get_quantized_weights` gives them.  The weights are laid
+    out once, here; they are a copy, and later changes of the tensors that were passed do not show."""
+
+    def __init__(self, weights: Dict[str, torch.Tensor]):
+        w, s, b = weights["weight"], weights["scale"], weights.get("bias")
+        L.need_gpu(w, s, b)
+        if w.dtype != torch.int8 or w.dim() != 2:
+            raise ValueError(f"weight must be an int8 matrix, got {w.dtype} {tuple(w.shape)}")
+        n, k = w.shape
+        if k < 1 or k > 131071:
+            raise ValueError(f"{k} input features; 1 to 131071 keep the 32-bit sum exact")
+        self.out_features, self.in_features, self.device = n, k, w.device
+        self.image = torch.zeros(n, _row_bytes(k), dtype=torch.int8, device=w.device)
+        self.image[:, :k] = w
+        self.scale = _check_scale(s, n, w.device, "scale").clone()
+        bc, self._bias_type = _check_bias(b, n, w.device)
+        self.bias = None if bc is None else bc.detach().clone()
+        self._w = (L.c_p(self.image.data_ptr()), L.c_p(self.scale.data_ptr()), L.c_p(0 if self.bias is None else self.bias.data_ptr()))
+
+    def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [..., K] -> [..., N] in the type of x.  `out` (optional: [..., N], contiguous, the type of x, apart from x in
+        memory) receives the result in place of a new tensor."""
+        k, n = self.in_features, self.out_features
+        t = _type(x, "x")
+        if x.dim() < 1 or x.shape[-1] != k:
+            raise ValueError(f"expected {k} input features, got {tuple(x.shape)}")
+        if x.device != self.device:
+            raise RuntimeError(f"the weights are on {self.device}, the tokens on {x.device}")
+        x2, ldx = _rows(x.detach())
+        m = x2.shape[0]
+        shape = (*x.shape[:-1], n)
+        if out is None:
+            out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        elif tuple(out.shape) != shape or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device or out.requires_grad:
+            raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {shape} on {x.device} without gradient")
+        elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+            raise RuntimeError("out must not share memory with x")
+        with L.device(x):
+            nbytes = L.lib().dpd_int8_linear_workspace_bytes(m, n, k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            qw, sw, b = self._w
+            L.call("dpd_int8_linear", L.c_p(x2.data_ptr()), t, m, k, ldx, qw, sw, b, self._bias_type, n, L.c_p(out.data_ptr()), n,
+                   L.c_p(ws.data_ptr()), nbytes, L.stream())
+        return out

@@ -359,6 +359,64 @@ int dpd_q88_matrix_prepare(const int16_t *w1, const int16_t *b1, const int16_t *
 int dpd_q88_matrix_infer(const int16_t *iq, int64_t B, int64_t S, const void *image, const int16_t *lut,
                          int16_t *out, void *stream);
 
+/* ---------------------------------------------------------------- 8-bit linear layer ---- */
+
+/* Element types of the entry points below; row strides (ld*) count elements.  None of them has a counterpart in the
+ * reference, whose QuantizedLinear (utils/quantization.py:186-256) has fixed power-of-two scales. */
+#define DPD_F32 0
+#define DPD_BF16 1
+#define DPD_F16 2
+
+/* Rows of x [rows, cols] in 8 bits with one scale each: scale[r] = max(max|x[r]|, 2^-100) / 127 (rounded once to fp32),
+ * q = the integer nearest to the exact x / scale, ties to even (|q| <= 127).  A row that holds a NaN or an infinity gets
+ * the scale NaN and zeros.  q [rows, ldq]: the columns cols..ldq-1 are set to zero. */
+int dpd_quantize_rows_int8(const void *x, int type, int64_t rows, int64_t cols, int64_t ldx, int8_t *q, int64_t ldq,
+                           float *scale, void *stream);
+
+/* out[m, n] = ((sum_k a[m, k] b[n, k]) * a_scale[m]) * b_scale[n] + bias[n]: a [M, K], b [N, K] int8, the sum exactly
+ * (int32; K <= 131071, DPD_ERR_SHAPE above), then fp32, rounded once to the type of out; bias may be NULL.  The workspace
+ * is read only where a row of a or b is not 16-byte aligned or K is no multiple of 16 (the rows are copied then). */
+size_t dpd_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dpd_int8_matmul(const int8_t *a, int64_t lda, const float *a_scale, const int8_t *b, int64_t ldb, const float *b_scale,
+                    const void *bias, int bias_type, int64_t M, int64_t N, int64_t K, void *out, int out_type, int64_t ldo,
+                    void *ws, size_t ws_bytes, void *stream);
+
+/* Tokens x [M, K] against a weight image: dpd_quantize_rows_int8 of x and dpd_int8_matmul in one call, out in the type of
+ * x.  qw: [N, dpd_int8_row_bytes(K)] int8, 16-byte aligned, as dpd_quantize_rows_int8 writes it with that ldq. */
+int64_t dpd_int8_row_bytes(int64_t K);
+size_t dpd_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, int64_t ldx, const int8_t *qw, const float *w_scale,
+                    const void *bias, int bias_type, int64_t N, void *out, int64_t ldo, void *ws, size_t ws_bytes, void *stream);
+
+/* Its straight-through gradients (the quantisers count as the identity): gx [M, K] = g (qw w_scale) in the type of g,
+ * gw [N, K] = g^T (qx x_scale), gb [N] = column sums of g; each may be NULL.  Products on the bf16 matrix cores: the
+ * 8-bit factor is exact there, g times a scale is rounded to bf16 once (type bf16), held in two bf16 terms (fp16) or in
+ * three (fp32: the whole value); sums in fp32, in a fixed order. */
+size_t dpd_int8_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, int need_gx, int need_gw, int need_gb);
+int dpd_int8_linear_backward(const void *g, int type, int64_t M, int64_t N, int64_t K, int64_t ldg, const int8_t *qx, int64_t ldqx,
+                             const float *x_scale, const int8_t *qw, int64_t ldqw, const float *w_scale, void *gx, void *gw,
+                             int gw_type, void *gb, int gb_type, void *ws, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------- orthogonalised update - */
+
+/* out = the Newton-Schulz iterate of each matrix x [batch, rows, cols] (contiguous) after `steps` steps:
+ *     X <- X / max(|X|_F, eps);   steps times:  A = X X^T,  X <- a X + (b A + c A A) X
+ * on the transposed matrix where rows > cols.  h_coef: steps triples (a, b, c), host memory.  The iterate's singular
+ * values are at most 1 at the start; coefficients that could take them above 3.9, or b A + c A A above 15, are refused
+ * (DPD_ERR_SHAPE), as are more than 32 steps.  accurate != 0: fp32 accuracy (each factor as two fp16 halves, three
+ * products); accurate == 0: factors rounded to fp16 (2^-11), sums in fp32. */
+size_t dpd_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int accurate);
+int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *h_coef,
+                      double eps, int accurate, void *out, void *ws, size_t ws_bytes, void *stream);
+
+/* One step of the Muon rule on n matrices p[i] [rows[i], cols[i]] (type p_type, as g[i]; momentum m[i] fp32), h_* host
+ * arrays:  m <- mu m + g;  u = g + mu m (nesterov != 0) or m;  p <- p (1 - lr wd) - lr sqrt(max(1, rows / cols)) O(u)
+ * with O the iterate above.  fp32 arithmetic, p rounded once. */
+size_t dpd_muon_workspace_bytes(int n, const int64_t *h_rows, const int64_t *h_cols, int accurate);
+int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, float *const *h_m, const int64_t *h_rows,
+                  const int64_t *h_cols, int p_type, double lr, double momentum, int nesterov, double weight_decay, int steps,
+                  const float *h_coef, double eps, int accurate, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
