@@ -3,23 +3,27 @@
 // orthogonalised update are made of.
 //
 // Every element type is seen as bytes: a K step is 128 bytes of each row (128 int8, 64 bf16 / fp16), two 16-byte
-// fragments per lane and step.  A workgroup of WAVES_M x WAVES_N waves owns a BM x BN tile; two LDS stages hold the
-// 128-byte pieces of its BM + BN rows, filled by direct global -> LDS loads (16 bytes a lane, 8 rows an instruction)
-// while the other stage is multiplied.  One barrier a step: behind it every wave has both finished reading the stage
-// that is filled next and seen the arrival of the stage that is read next.
+// fragments per lane and step.  A workgroup of WAVES_M x WAVES_N waves owns a BM x BN tile.  STAGES pieces of LDS, each
+// for one step of its BM + BN rows, are filled by direct global -> LDS loads (16 bytes a lane, 8 rows an instruction).
+// The loop runs half a step ahead of itself: while the first fragments of a step are multiplied the second ones are
+// read, and while those are multiplied the first ones of the next step.  One barrier a step, between the halves: behind
+// it every wave has read all of this step's stage (which is filled again, STAGES steps ahead) and seen its successor.
 //
-// LDS layout: row r keeps its 16-byte chunk c at position c ^ (r & 7).  The direct load writes lane after lane, so the
-// permutation is applied to the global chunk a lane asks for; a fragment read then touches all banks evenly (8
-// successive lanes read 8 different 16-byte columns).
+// LDS layout: row r keeps its 16-byte chunk c at position c ^ key(r).  The direct load writes lane after lane, so the
+// permutation is applied to the global chunk a lane asks for.  Keys are chosen so that the 16 lanes that read together
+// hit 16 different 16-byte columns of the 256-byte bank row, for the row orders of both operands (measured: no conflicts).
 //
 // Operands of a product in a split form (SPLIT): a row holds blocks of 32 elements, first their leading halves (64
 // bytes), then their remainders (64 bytes).  A step then carries 32 elements, and the three products lead*lead,
 // lead*rest, rest*lead go into one accumulator: fp16 halves of a scaled fp32 value give 22 bits of it.
 //
 // Lane layout of the results: the B rows are the first operand of the instruction, so a lane of a 16 x 16 block holds
-// C[m = lane & 15][n = 4 * (lane >> 4) + 0..3]: four consecutive columns of one row.
+// one row m = lane & 15 and four columns.  The B rows of a pair of blocks are interleaved in fours, so that the pair gives
+// a lane eight successive columns: n = 8 * (lane >> 4) + 0..7 of 32.
 #pragma once
 #include "common.h"
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 namespace nt {
 
@@ -31,6 +35,13 @@ typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 enum Kind { I8, BF16, F16, F16_SPLIT };
+
+struct Yes {
+    static constexpr bool value = true;
+};
+struct No {
+    static constexpr bool value = false;
+};
 
 template <int KIND>
 struct Acc {
@@ -58,33 +69,71 @@ struct Args {
     int M, N;                      // rows of a and of b
     int steps;                     // K steps of the whole product
     int wrap;                      // steps after which the B operand starts again (a has several planes along k); == steps otherwise
-    int tail;                      // valid bytes of the last step of a plane (a multiple of 16; 128 where rows are padded)
+    int tail;                      // valid bytes of the last step (a multiple of 16; 128 where rows are padded or wrap < steps)
     int tiles_m, tiles_n;
-    int lower;                     // C is symmetric: tiles wholly above the diagonal are left out (BM == BN)
+    int lower;                     // C is symmetric: the tiles above the diagonal are left out (BM == BN)
 };
 
 constexpr int STEP = 128;                                   // bytes of a row per step
 
 // Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, and
-// inside a run the tiles go down bands of 8 tile rows, so that the operands of neighbours meet in one L2.
+// inside a run the tiles go down bands of 8 tile rows, so that the operands of neighbours meet in one L2.  `lower`: the
+// tiles on and below the diagonal only (the last 8 columns of a band are a triangle).
 DEV void tile_of(const Args &g, int id, int n_tiles, int *tm, int *tn) {
     const int xcd = id & 7, q = n_tiles >> 3, r = n_tiles & 7;
-    const int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3);
-    const int band = 8 * g.tiles_n, b = t / band, in = t - b * band;
-    const int rows = min(8, g.tiles_m - b * 8);
-    *tn = in / rows;
-    *tm = b * 8 + in - *tn * rows;
+    int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (id >> 3), b = 0;
+    if (!g.lower) {
+        b = t / (8 * g.tiles_n), t -= b * 8 * g.tiles_n;
+        const int rows = min(8, g.tiles_m - b * 8);
+        *tn = t / rows;
+        *tm = b * 8 + t - *tn * rows;
+        return;
+    }
+    for (;; ++b) {
+        const int rows = min(8, g.tiles_m - b * 8), square = rows * 8 * b, size = square + rows * (rows + 1) / 2;
+        if (t >= size) {
+            t -= size;
+            continue;
+        }
+        if (t < square) {
+            *tn = t / rows;
+            *tm = b * 8 + t - *tn * rows;
+            return;
+        }
+        t -= square;
+        int col = 0;
+        while (t >= rows - col) t -= rows - col++;
+        *tn = b * 8 + col;
+        *tm = b * 8 + col + t;
+        return;
+    }
+}
+static inline int tiles_of(const Args &g) { return g.lower ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n; }
+
+// Row of a tile that lane r (0..15) of block j of the B operand stands for: blocks 2q and 2q + 1 share 32 rows.
+DEV int b_row(int j, int r) { return (j >> 1) * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3); }
+DEV int key_a(int row) { return row & 7; }                                              // 16 successive rows
+DEV int key_b(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }           // rows 0..3, 8..11, 16..19, 24..27 (+ 4)
+
+// All but the N newest loads of this wave, and all its LDS reads, have arrived; then all waves of the workgroup.
+template <int N>
+DEV void wait_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));       // vmcnt(N), lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, class Epilogue>
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
 DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     constexpr int WAVES = WAVES_M * WAVES_N, TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
-    constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, STAGE = (BM + BN) * STEP;
-    static_assert(LOADS_A >= 1 && LOADS_B >= 1, "every wave loads whole groups of 8 rows");
-    __shared__ __attribute__((aligned(128))) char smem[2 * STAGE];
+    constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B, STAGE = (BM + BN) * STEP;
+    static_assert(LOADS_A >= 1 && LOADS_B >= 1 && LOADS_A * 8 * WAVES == BM && LOADS_B * 8 * WAVES == BN, "every wave loads whole groups of 8 rows");
+    static_assert(TN % 2 == 0 && (TM % 2 == 0 || KIND != F16_SPLIT) && STAGES >= 2 && (STAGES - 2) * LOADS < 64, "pairs of blocks; the wait counter has 6 bits");
+    static_assert(STAGES * STAGE <= 160 * 1024, "LDS of a compute unit");
+    __shared__ __attribute__((aligned(256))) char smem[STAGES * STAGE];
     int tm, tn;
-    tile_of(g, blockIdx.x, g.tiles_m * g.tiles_n, &tm, &tn);
-    if (g.lower && tn > tm) return;
+    tile_of(g, blockIdx.x, gridDim.x, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
@@ -94,24 +143,31 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     // and arrive as zeros.  The step is the scalar offset, which the bounds check leaves out.
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc((void *)ab, 0, 0x7fffffff, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void *)bb, 0, 0x7fffffff, 0x00020000);
-    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     unsigned va[LOADS_A], vb[LOADS_B];
+    auto chunk_a = [&](int i) { return ((lane & 7) ^ key_a((i * WAVES + wave) * 8 + (lane >> 3))) * 16; };
+    auto chunk_b = [&](int i) { return ((lane & 7) ^ key_b((i * WAVES + wave) * 8 + (lane >> 3))) * 16; };
 #pragma unroll
-    for (int i = 0; i < LOADS_A; ++i) va[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.M - 1 - m0) * (int)g.lda + chunk);
+    for (int i = 0; i < LOADS_A; ++i) va[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.M - 1 - m0) * (int)g.lda + chunk_a(i));
 #pragma unroll
-    for (int i = 0; i < LOADS_B; ++i) vb[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.N - 1 - n0) * (int)g.ldb + chunk);
-
-    auto stage = [&](int s, int buf) {
-        char *base = smem + buf * STAGE;
-        const int w = s % g.wrap;
-        const bool cut = w == g.wrap - 1 && chunk >= g.tail;
-#pragma unroll
-        for (int i = 0; i < LOADS_A; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *)(base + (i * WAVES + wave) * 1024), 16, cut ? 0xfffffff0u : va[i], s * STEP, 0, 0);
-#pragma unroll
-        for (int i = 0; i < LOADS_B; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(base + BM * STEP + (i * WAVES + wave) * 1024), 16, cut ? 0xfffffff0u : vb[i], w * STEP, 0, 0);
+    for (int i = 0; i < LOADS_B; ++i) vb[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.N - 1 - n0) * (int)g.ldb + chunk_b(i));
+    int wrapped = 0;                                       // step of the B operand that is loaded next
+    auto load = [&](int i, int s, int at) {                // 8 rows: part i of LOADS
+        if (i < LOADS_A)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *)(smem + at + (i * WAVES + wave) * 1024), 16, va[i], s * STEP, 0, 0);
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(smem + at + BM * STEP + ((i - LOADS_A) * WAVES + wave) * 1024), 16, vb[i - LOADS_A],
+                                                     wrapped * STEP, 0, 0);
     };
+    const int cut_step = g.tail == STEP ? -1 : g.steps - 1;
+    auto before_loads = [&](int s) {                       // chunks that the last step does not have
+        if (s == cut_step) {
+#pragma unroll
+            for (int i = 0; i < LOADS_A; ++i) va[i] = chunk_a(i) >= g.tail ? 0xfffffff0u : va[i];
+#pragma unroll
+            for (int i = 0; i < LOADS_B; ++i) vb[i] = chunk_b(i) >= g.tail ? 0xfffffff0u : vb[i];
+        }
+    };
+    auto after_loads = [&]() { wrapped = wrapped == g.wrap - 1 ? 0 : wrapped + 1; };
 
     typename Acc<KIND>::type acc[TM][TN];
 #pragma unroll
@@ -119,77 +175,234 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = typename Acc<KIND>::type{0, 0, 0, 0};
 
-    const int frag = (lane & 15) * STEP, c0 = ((lane >> 4) ^ (lane & 7)) * 16, c1 = ((4 + (lane >> 4)) ^ (lane & 7)) * 16;
-    auto compute = [&](int buf) {
-        const char *pa = smem + buf * STAGE + wm * TM * 16 * STEP + frag, *pb = smem + buf * STAGE + (BM + wn * TN * 16) * STEP + frag;
-        i32x4 a0[TM], b0[TN], a1[TM], b1[TN];
+    // fragment c (0 or 1) of block i of A, of block j of B: the keys do not depend on i and j
+    const int r = lane & 15, q = lane >> 4;
+    const char *pa = smem + (wm * TM * 16 + r) * STEP, *pb = smem + (BM + wn * TN * 16) * STEP;
+    const int ka[2] = {(q ^ key_a(r)) * 16, ((4 + q) ^ key_a(r)) * 16};
+    const int kb[2] = {b_row(0, r) * STEP + (q ^ key_b(b_row(0, r))) * 16, b_row(0, r) * STEP + ((4 + q) ^ key_b(b_row(0, r))) * 16};
+    constexpr bool SPLIT = KIND == F16_SPLIT;
+    i32x4 a0[SPLIT ? 2 : TM], b0[TN], a1[SPLIT ? 2 : TM], b1[TN];
+    auto reada = [&](i32x4 *a, int k, int i, int at, int c) { a[k] = *(const i32x4 *)(pa + at + i * 16 * STEP + ka[c]); };
+    auto readb = [&](i32x4 *b, int j, int at, int c) { b[j] = *(const i32x4 *)(pb + at + b_row(j, 0) * STEP + kb[c]); };
+    auto mul = [&](const i32x4 *a, const i32x4 *b, int i) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a0[i] = *(const i32x4 *)(pa + i * 16 * STEP + c0);
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma<KIND>(b[j], a[i], acc[i][j]);
+    };
+    auto mul3 = [&](int i, int j, int count) {             // small terms first; blocks j .. j + count - 1 in turn
 #pragma unroll
-        for (int j = 0; j < TN; ++j) b0[j] = *(const i32x4 *)(pb + j * 16 * STEP + c0);
+        for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b1[k], a0[i & 1], acc[i][k]);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a1[i] = *(const i32x4 *)(pa + i * 16 * STEP + c1);
+        for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b0[k], a1[i & 1], acc[i][k]);
 #pragma unroll
-        for (int j = 0; j < TN; ++j) b1[j] = *(const i32x4 *)(pb + j * 16 * STEP + c1);
+        for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b0[k], a0[i & 1], acc[i][k]);
+    };
+    // The order of the instructions is the order written here: in front of the products of block row i the reads of the
+    // fragments that the next half needs (early, so that the last of them has arrived by then) and the loads.
+    constexpr int READ_ROWS = TM > 2 ? TM - 2 : 1, READS = (TM + TN + READ_ROWS - 1) / READ_ROWS, LOADS_ROW = (LOADS + TM - 1) / TM;
+    auto read_part = [&](i32x4 *a, i32x4 *b, int i, int at, int c) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int k = i * READS; k < (i + 1) * READS; ++k) {
+            if (k < TM) reada(a, k, k, at, c);
+            else if (k < TM + TN) readb(b, k - TM, at, c);
+        }
+    };
+    auto next = [](int at) { return at == (STAGES - 1) * STAGE ? 0 : at + STAGE; };
+
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                if constexpr (KIND == F16_SPLIT) {
-                    acc[i][j] = mfma<KIND>(b1[j], a0[i], acc[i][j]);
-                    acc[i][j] = mfma<KIND>(b0[j], a1[i], acc[i][j]);
-                    acc[i][j] = mfma<KIND>(b0[j], a0[i], acc[i][j]);
-                } else {
-                    acc[i][j] = mfma<KIND>(b0[j], a0[i], acc[i][j]);
-                }
+    for (int s = 0; s < STAGES; ++s)
+        if (s < g.steps) {
+            before_loads(s);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) load(i, s, s * STAGE);
+            after_loads();
+        }
+    if (g.steps >= STAGES) wait_barrier<(STAGES - 1) * LOADS>();
+    else wait_barrier<0>();
+#pragma unroll
+    for (int i = 0; i < (SPLIT ? 1 : TM); ++i) reada(a0, i, i, 0, 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) readb(b0, j, 0, 0);
+    if constexpr (SPLIT) {
+        reada(a1, 0, 0, 0, 1);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) readb(b1, j, 0, 1);
+    }
+    int at = 0;
+    auto step = [&](int s, auto more) {                    // more: stage s + STAGES exists
+        const int ahead = next(at);
+        __builtin_amdgcn_s_waitcnt(0xc07f);                // lgkmcnt(0): the first fragments
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            read_part(a1, b1, i, at, 1);
+            mul(a0, b0, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (more.value) {
+            wait_barrier<(STAGES - 2) * LOADS>();
+            before_loads(s + STAGES);
+        } else {
+            wait_barrier<0>();                             // the last stages: nothing newer is in flight
+        }
+        auto load_part = [&](int i) {
+            if constexpr (more.value) {
+#pragma unroll
+                for (int k = i * LOADS_ROW; k < (i + 1) * LOADS_ROW; ++k)
+                    if (k < LOADS) load(k, s + STAGES, at);
             }
-        if constexpr (KIND != F16_SPLIT) {
+        };
+        // behind the last step the reads for the next one find an old stage, and nobody uses them
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            load_part(i);
+            read_part(a0, b0, i, ahead, 0);
+            mul(a1, b1, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (more.value) after_loads();
+        at = ahead;
+    };
+    // The split form needs both halves of both operands at once.  The B fragments of a step stay in registers; the A
+    // fragments of block row i + 1 are read while row i is multiplied; in front of the last row everything of this stage
+    // has been read, and behind each of its blocks that block's B fragments of the next step are.
+    auto step_split = [&](int s, auto more) {
+        const int ahead = next(at);
+#pragma unroll
+        for (int i = 0; i < TM - 1; ++i) {
+            reada(a0, (i + 1) & 1, i + 1, at, 0);
+            reada(a1, (i + 1) & 1, i + 1, at, 1);
+            mul3(i, 0, TN);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (more.value) {
+            wait_barrier<(STAGES - 2) * LOADS>();
+            before_loads(s + STAGES);
+#pragma unroll
+            for (int k = 0; k < LOADS; ++k) load(k, s + STAGES, at);
+            after_loads();
+        } else {
+            wait_barrier<0>();
+        }
+        reada(a0, 0, 0, ahead, 0);
+        reada(a1, 0, 0, ahead, 1);
+#pragma unroll
+        for (int j = 0; j < TN; j += 2) {
+            mul3(TM - 1, j, 2);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = j; k < j + 2; ++k) readb(b0, k, ahead, 0), readb(b1, k, ahead, 1);
+        }
+        at = ahead;
+    };
+    int s = 0;
+    if constexpr (SPLIT) {
+        for (; s + STAGES < g.steps; ++s) step_split(s, Yes{});
+        for (; s < g.steps; ++s) step_split(s, No{});
+    } else {
+        for (; s + STAGES < g.steps; ++s) step(s, Yes{});
+        for (; s < g.steps; ++s) step(s, No{});
+    }
+    typename Epilogue::Col col[TN / 2];
+#pragma unroll
+    for (int j = 0; j < TN / 2; ++j) col[j] = epi.col(blockIdx.z, n0 + wn * TN * 16 + j * 32 + q * 8);
+    const bool turn = Epilogue::TURNED && !(g.lower && tm == tn);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int m = m0 + (wm * TM + i) * 16 + r;
+        typename Epilogue::Row row;
+        if (m < g.M) row = epi.row(blockIdx.z, m);
+#pragma unroll
+        for (int j = 0; j < TN / 2; ++j) {
+            const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][2 * j][e], v[4 + e] = (float)acc[i][2 * j + 1][e];
+            if (m < g.M && n < g.N) {
+                epi.put(blockIdx.z, m, n, v, row, col[j]);
+            } else if (Epilogue::TURNED) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = 0.f;    // zeros behind the rows of the turned tile
+            }
+            if constexpr (Epilogue::TURNED) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][2 * j][e] = v[e], acc[i][2 * j + 1][e] = v[4 + e];
+            }
+        }
+    }
+    // The tile once more, turned: through LDS (free now), as fp16 rows of BM values along m, a pass for each half of the
+    // split form.  Chunks of 8 values are permuted by the row so that the 16 lanes that write one column spread out.
+    if constexpr (Epilogue::TURNED) {
+        if (!turn) return;
+        static_assert(BM * BN * 2 <= STAGES * STAGE, "a turned tile fits into LDS");
+        constexpr int CHUNKS = BM / 8, MASK = CHUNKS % 32 == 0 ? 31 : CHUNKS % 16 == 0 ? 15 : 7;
+        _Float16 *t = (_Float16 *)smem;
+#pragma unroll
+        for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
+            __syncthreads();
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma<KIND>(b1[j], a1[i], acc[i][j]);
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int ml = (wm * TM + i) * 16 + r, nl = wn * TN * 16 + (j >> 1) * 32 + q * 8 + (j & 1) * 4 + e;
+                        const _Float16 h = (_Float16)acc[i][j][e];
+                        t[nl * BM + (((ml >> 3) ^ ((nl >> 3) & MASK)) << 3) + (ml & 7)] = h;
+                        if (SPLIT) acc[i][j][e] -= (float)h;
+                    }
+            __syncthreads();
+            for (int k = threadIdx.x; k < BN * CHUNKS; k += 64 * WAVES) {
+                const int nl = k / CHUNKS, c = k - nl * CHUNKS;
+                if (n0 + nl < g.N && m0 + c * 8 < g.M)
+                    epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * BM + ((c ^ ((nl >> 3) & MASK)) << 3)));
+            }
         }
-    };
-
-    stage(0, 0);
-    for (int s = 0; s < g.steps; ++s) {
-        // this wave's part of stage s has arrived, and its reads of the other stage have returned
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < g.steps) stage(s + 1, (s + 1) & 1);
-        compute(s & 1);
     }
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int m = m0 + (wm * TM + i) * 16 + (lane & 15), n = n0 + (wn * TN + j) * 16 + (lane >> 4) * 4;
-            if (m < g.M && n < g.N) epi(blockIdx.z, m, n, acc[i][j]);
-        }
 }
 
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, class Epilogue>
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
 static __global__ __launch_bounds__(64 * WAVES_M *WAVES_N) void k_gemm(Args g, Epilogue epi) {
-    gemm_tile<KIND, BM, BN, WAVES_M, WAVES_N>(g, epi);
+    gemm_tile<KIND, BM, BN, WAVES_M, WAVES_N, STAGES>(g, epi);
 }
 
 // ---- host side -------------------------------------------------------------------------
-// Largest tile that still gives most of the 256 compute units one; the small ones trade operand traffic for that.
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, class Epilogue>
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
 static int launch(Args g, int batch, const Epilogue &epi, hipStream_t st) {
     g.tiles_m = (g.M + BM - 1) / BM;
     g.tiles_n = (g.N + BN - 1) / BN;
-    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, Epilogue>), dim3((unsigned)(g.tiles_m * g.tiles_n), 1, (unsigned)batch),
+    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, STAGES, Epilogue>), dim3((unsigned)tiles_of(g), 1, (unsigned)batch),
                        dim3(64 * WAVES_M * WAVES_N), 0, st, g, epi);
     DPD_LAUNCH_CHECK();
     return DPD_OK;
 }
 
+// Which tile: the one whose rounds over the 256 compute units (one tile each) are estimated to take least.
+// Measured (4096 and 2048 rows, us): a round of steps costs about steps * per_step + fixed.
+struct TileCost {
+    int bm, bn;
+    float per_step, fixed;
+};
+constexpr TileCost TILES[] = {{256, 256, 1.35f, 10.f}, {256, 128, 0.82f, 7.f}, {192, 192, 0.8f, 8.f}, {128, 128, 0.46f, 4.5f}, {64, 64, 0.21f, 3.f}};
+
 template <int KIND, class Epilogue>
 static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st) {
-    auto tiles = [&](int b) { return (int64_t)((g.M + b - 1) / b) * ((g.N + b - 1) / b) * batch; };
-    if (tiles(256) >= 192) return launch<KIND, 256, 256, 2, 4>(g, batch, epi, st);
-    if (tiles(128) >= 128) return launch<KIND, 128, 128, 2, 2>(g, batch, epi, st);
-    return launch<KIND, 64, 64, 2, 2>(g, batch, epi, st);
+    int best = 0;
+    float least = 0.f;
+    for (int i = 0; i < 5; ++i) {
+        const TileCost &t = TILES[i];
+        if (g.lower && t.bm != t.bn) continue;
+        Args a = g;
+        a.tiles_m = (g.M + t.bm - 1) / t.bm, a.tiles_n = (g.N + t.bn - 1) / t.bn;
+        const int64_t rounds = ((int64_t)tiles_of(a) * batch + 255) / 256;
+        const float cost = (float)rounds * ((float)g.steps * (KIND == F16_SPLIT ? 1.5f : 1.f) * t.per_step + t.fixed);
+        if (i == 0 || cost < least) best = i, least = cost;
+    }
+    switch (best) {
+    case 0: return launch<KIND, 256, 256, 2, 4, 2>(g, batch, epi, st);
+    case 1: return launch<KIND, 256, 128, 4, 2, 3>(g, batch, epi, st);
+    case 2: return launch<KIND, 192, 192, 2, 2, 3>(g, batch, epi, st);
+    case 3: return launch<KIND, 128, 128, 2, 4, 4>(g, batch, epi, st);
+    default: return launch<KIND, 64, 64, 2, 2, 8>(g, batch, epi, st);
+    }
 }
 
 // A row of an operand may have at most this many bytes: 256 rows of a tile stay inside 32-bit offsets.
@@ -200,7 +413,6 @@ static inline int64_t pad_to(int64_t v, int64_t m) { return (v + m - 1) / m * m;
 }  // namespace nt
 
 // ---- element types of the entry points ----------------------------------------------------
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 template <class T>
 DEV float to_f32(T v) { return (float)v; }
@@ -212,18 +424,46 @@ DEV float load_any(const void *p, int type, int64_t i) {
     return type == DPD_F32 ? ((const float *)p)[i] : type == DPD_BF16 ? (float)((const __bf16 *)p)[i] : (float)((const _Float16 *)p)[i];
 }
 
-// Four consecutive values of one row; `whole`: all four lie inside the row and the address is aligned for one store.
+// Eight consecutive values of one row, the first `valid` of them; `whole`: the row's address is aligned for 16-byte
+// stores at every multiple of eight elements.
 template <class T>
-DEV void store4(T *p, f32x4_t v, int valid, bool whole) {
-    typedef T T4 __attribute__((ext_vector_type(4)));
-    if (whole && valid >= 4) {
-        *(T4 *)p = T4{from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+DEV void store8(T *p, const float *v, int valid, bool whole) {
+    if (whole && valid >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            *(f32x4_t *)p = f32x4_t{v[0], v[1], v[2], v[3]};
+            *((f32x4_t *)p + 1) = f32x4_t{v[4], v[5], v[6], v[7]};
+        } else {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+            T8 o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = from_f32<T>(v[i]);
+            *(T8 *)p = o;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             if (i < valid) p[i] = from_f32<T>(v[i]);
     }
 }
+template <class T>
+DEV void load8(const T *p, float *v, int valid, bool whole) {
+    if (whole && valid >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4_t a = *(const f32x4_t *)p, b = *((const f32x4_t *)p + 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+        } else {
+            typedef T T8 __attribute__((ext_vector_type(8)));
+            const T8 a = *(const T8 *)p;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_f32(a[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? to_f32(p[i]) : 0.f;
+    }
+}
+struct None {};
 
 static inline int type_size(int type) { return type == DPD_F32 ? 4 : 2; }
 

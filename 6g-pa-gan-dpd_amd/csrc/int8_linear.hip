@@ -80,16 +80,26 @@ struct ScaleOut {
     int64_t ldo;
     int N;
     bool whole;
-    DEV void operator()(int, int m, int n, nt::i32x4 acc) const {
-        const float s = sa[m];
-        f32x4_t v;
+    static constexpr bool TURNED = false;
+    typedef float Row;
+    struct Col {
+        float s[8], b[8];
+    };
+    DEV Row row(int, int m) const { return sa[m]; }
+    DEV Col col(int, int n) const {
+        Col c;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const int k = min(n + i, N - 1);
-            v[i] = (float)acc[i] * s * sb[k];
-            if (bias) v[i] += load_any(bias, bias_type, k);
+            c.s[i] = sb[k];
+            c.b[i] = bias ? load_any(bias, bias_type, k) : 0.f;
         }
-        store4(out + (int64_t)m * ldo + n, v, N - n, whole);
+        return c;
+    }
+    DEV void put(int, int m, int n, float *v, const Row &r, const Col &c) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * r * c.s[i] + c.b[i];
+        store8(out + (int64_t)m * ldo + n, v, N - n, whole);
     }
 };
 
@@ -99,9 +109,11 @@ struct PlainOut {
     int64_t ldo;
     int N;
     bool whole;
-    DEV void operator()(int, int m, int n, nt::f32x4 acc) const {
-        store4(out + (int64_t)m * ldo + n, f32x4_t{acc[0], acc[1], acc[2], acc[3]}, N - n, whole);
-    }
+    static constexpr bool TURNED = false;
+    typedef None Row, Col;
+    DEV Row row(int, int) const { return {}; }
+    DEV Col col(int, int) const { return {}; }
+    DEV void put(int, int m, int n, float *v, Row, Col) const { store8(out + (int64_t)m * ldo + n, v, N - n, whole); }
 };
 
 // rows of an int8 matrix at a stride that the product can read (a multiple of 128 bytes, zeros behind the row)
@@ -118,7 +130,7 @@ __global__ __launch_bounds__(256) void k_pad_rows(const int8_t *__restrict__ q, 
 bool readable(const int8_t *q, int64_t ld, int64_t K) { return ((uintptr_t)q & 15) == 0 && ld % 16 == 0 && K % 16 == 0; }
 
 template <class T>
-bool whole4(const T *p, int64_t ld) { return ((uintptr_t)p % (4 * sizeof(T))) == 0 && ld % 4 == 0; }
+bool whole8(const T *p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 template <class T>
 int int8_product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b, int64_t ldb, const float *sb, const void *bias,
@@ -127,7 +139,7 @@ int int8_product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
     g.a = (const char *)a, g.b = (const char *)b, g.lda = lda, g.ldb = ldb, g.M = (int)M, g.N = (int)N;
     g.steps = g.wrap = (int)((K + 127) / 128);
     g.tail = (int)(K - (int64_t)(g.steps - 1) * 128);
-    return nt::product<nt::I8>(g, 1, ScaleOut<T>{sa, sb, bias, bias_type, out, ldo, (int)N, whole4(out, ldo)}, st);
+    return nt::product<nt::I8>(g, 1, ScaleOut<T>{sa, sb, bias, bias_type, out, ldo, (int)N, whole8(out, ldo)}, st);
 }
 
 // ---- gradients ---------------------------------------------------------------------------
@@ -249,7 +261,7 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         nt::Args a{};
         a.a = (const char *)gs, a.lda = P * p.n_pad * 2, a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
         a.wrap = (int)(p.n_pad / 64), a.steps = P * a.wrap, a.tail = 128;
-        const int rc = nt::product<nt::BF16>(a, 1, PlainOut<T>{gx, K, (int)K, whole4(gx, K)}, st);
+        const int rc = nt::product<nt::BF16>(a, 1, PlainOut<T>{gx, K, (int)K, whole8(gx, K)}, st);
         if (rc) return rc;
     }
     if (gw) {
@@ -260,7 +272,7 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         a.wrap = (int)(p.m_pad / 64), a.steps = P * a.wrap, a.tail = 128;
         const int rc = with_type(gw_type, [&](auto t) {
             using W = decltype(t);
-            return nt::product<nt::BF16>(a, 1, PlainOut<W>{(W *)gw, K, (int)K, whole4((W *)gw, K)}, st);
+            return nt::product<nt::BF16>(a, 1, PlainOut<W>{(W *)gw, K, (int)K, whole8((W *)gw, K)}, st);
         });
         if (rc) return rc;
     }

@@ -45,13 +45,23 @@ template <class T>
 struct ToTensor {
     T *out;
     int64_t batch;
+    bool whole;                                       // rows of whole 16-byte pieces
     DEV void put(int z, int64_t i, float v) const { out[z * batch + i] = from_f32<T>(v); }
+    DEV void put8(int z, int64_t i, const float *v, int valid) const { store8(out + z * batch + i, v, valid, whole); }
 };
 template <class T>
 struct ToWeights {
     T *p;
     float keep, factor;                               // 1 - lr wd, lr sqrt(max(1, rows / cols))
+    bool whole;
     DEV void put(int, int64_t i, float v) const { p[i] = from_f32<T>(to_f32(p[i]) * keep - factor * v); }
+    DEV void put8(int, int64_t i, float *v, int valid) const {
+        float w[8];
+        load8(p + i, w, valid, whole);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = w[k] * keep - factor * v[k];
+        store8(p + i, v, valid, whole);
+    }
 };
 
 DEV double block_sum_d(double v, double *red) {       // over the 256 threads of a workgroup, the same value in all
@@ -187,7 +197,7 @@ template <class T>
 __global__ __launch_bounds__(256) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
     __shared__ float lds[SMALL_LDS];
     const int z = blockIdx.x;
-    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z]}, 0, tab.rows[z],
+    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
                   tab.cols[z], coef, steps, eps, lds);
 }
 
@@ -202,23 +212,25 @@ template <bool SPLIT>
 DEV int64_t img_col(int col) { return SPLIT ? (int64_t)(col >> 5) * 128 + (col & 31) * 2 : (int64_t)col * 2; }
 
 template <bool SPLIT>
-DEV f32x4_t img_load4(const Image &im, int z, int64_t row, int col) {
+DEV void img_load8(const Image &im, int z, int64_t row, int col, float *v) {
     const char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
-    const nt::f16x4 h = *(const nt::f16x4 *)p;
-    f32x4_t v = {(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    if (SPLIT) {
-        const nt::f16x4 l = *(const nt::f16x4 *)(p + 64);
+    const nt::f16x8 h = *(const nt::f16x8 *)p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += (float)l[i];
+    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+    if (SPLIT) {
+        const nt::f16x8 l = *(const nt::f16x8 *)(p + 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += (float)l[i];
     }
-    return v;
 }
 template <bool SPLIT>
-DEV void img_store4(const Image &im, int z, int64_t row, int col, f32x4_t v) {
+DEV void img_store8(const Image &im, int z, int64_t row, int col, const float *v) {
     char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
-    const nt::f16x4 h = {(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-    *(nt::f16x4 *)p = h;
-    if (SPLIT) *(nt::f16x4 *)(p + 64) = nt::f16x4{(_Float16)(v[0] - (float)h[0]), (_Float16)(v[1] - (float)h[1]), (_Float16)(v[2] - (float)h[2]), (_Float16)(v[3] - (float)h[3])};
+    nt::f16x8 h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i], l[i] = (_Float16)(v[i] - (float)h[i]);
+    *(nt::f16x8 *)p = h;
+    if (SPLIT) *(nt::f16x8 *)(p + 64) = l;
 }
 template <bool SPLIT>
 DEV void img_store1(const Image &im, int z, int64_t row, int col, float v) {
@@ -260,11 +272,20 @@ __global__ __launch_bounds__(256) void k_prepare(From from, int rows, int cols, 
     }
     __syncthreads();
     const Image &same = wide ? P : Q, &flip = wide ? Q : P;        // the image in x's orientation, and the other one
-    for (int e = t; e < 1024; e += 256) {
-        const int i = e >> 4, j = (e & 15) * 4;
-        const int64_t end_c = SPLIT ? same.ld / 4 : same.ld / 2, end_r = SPLIT ? flip.ld / 4 : flip.ld / 2;
-        if (r0 + i < rows && c0 + j < end_c) img_store4<SPLIT>(same, z, r0 + i, c0 + j, f32x4_t{tile[i][j], tile[i][j + 1], tile[i][j + 2], tile[i][j + 3]});
-        if (c0 + i < cols && r0 + j < end_r) img_store4<SPLIT>(flip, z, c0 + i, r0 + j, f32x4_t{tile[j][i], tile[j + 1][i], tile[j + 2][i], tile[j + 3][i]});
+    const int64_t end_c = SPLIT ? same.ld / 4 : same.ld / 2, end_r = SPLIT ? flip.ld / 4 : flip.ld / 2;
+    for (int e = t; e < 512; e += 256) {
+        const int i = e >> 3, j = (e & 7) * 8;
+        float v[8];
+        if (r0 + i < rows && c0 + j < end_c) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = tile[i][j + k];
+            img_store8<SPLIT>(same, z, r0 + i, c0 + j, v);
+        }
+        if (c0 + i < cols && r0 + j < end_r) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = tile[j + k][i];
+            img_store8<SPLIT>(flip, z, c0 + i, r0 + j, v);
+        }
     }
 }
 
@@ -283,58 +304,72 @@ __global__ __launch_bounds__(256) void k_zero_pads(Image a, int64_t ra, Image b,
     }
 }
 
+struct NoFactors {
+    static constexpr bool TURNED = false;
+    typedef None Row, Col;
+    DEV Row row(int, int) const { return {}; }
+    DEV Col col(int, int) const { return {}; }
+};
 template <bool SPLIT>
-struct GramOut {                       // A = X X^T (times T_SCALE)
+DEV void img_store_half(const Image &im, int z, int64_t row, int col, int half, nt::f16x8 v) {
+    *(nt::f16x8 *)(im.base + img_row(im, z, row) + img_col<SPLIT>(col) + half * 64) = v;
+}
+// The two symmetric products compute their tiles on and below the diagonal; a tile below it is stored turned as well.
+template <bool SPLIT>
+struct GramOut : NoFactors {           // A = X X^T (times T_SCALE); zeros behind the rows
+    static constexpr bool TURNED = true;
     Image A;
     float scale;
     int N;
-    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
-        f32x4_t v;
+    DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(A, z, row, col, half, v); }
+    DEV void put(int z, int m, int n, float *v, Row, Col) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? acc[i] * scale : 0.f;
-        img_store4<SPLIT>(A, z, m, n, v);
+        for (int i = 0; i < 8; ++i) v[i] = n + i < N ? v[i] * scale : 0.f;
+        img_store8<SPLIT>(A, z, m, n, v);
     }
 };
 template <bool SPLIT>
-struct PolyOut {                       // B = b A + c A A (times T_SCALE)
+struct PolyOut : NoFactors {           // B = b A + c A A (times T_SCALE)
+    static constexpr bool TURNED = true;
     Image A, B;
     float b, c;
     int N;
-    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
-        const f32x4_t a = img_load4<SPLIT>(A, z, m, n);
-        f32x4_t v;
+    DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(B, z, row, col, half, v); }
+    DEV void put(int z, int m, int n, float *v, Row, Col) const {
+        float a[8];
+        img_load8<SPLIT>(A, z, m, n, a);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? __builtin_fmaf(c, acc[i] * (1.f / T_SCALE), b * a[i]) : 0.f;
-        img_store4<SPLIT>(B, z, m, n, v);
+        for (int i = 0; i < 8; ++i) v[i] = n + i < N ? __builtin_fmaf(c, v[i] * (1.f / T_SCALE), b * a[i]) : 0.f;
+        img_store8<SPLIT>(B, z, m, n, v);
     }
 };
 template <bool SPLIT>
-struct NextOut {                       // X <- a X + B X into P (in place: a tile reads its own entries only) and the other Q
+struct NextOut : NoFactors {           // X <- a X + B X into P (in place: a tile reads its own entries only) and the other Q
+    static constexpr bool TURNED = true;
     Image P, Q;
     float a;
     int N;
-    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
-        const f32x4_t x = img_load4<SPLIT>(P, z, m, n);
-        f32x4_t v;
+    DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(Q, z, row, col, half, v); }
+    DEV void put(int z, int m, int n, float *v, Row, Col) const {
+        float x[8];
+        img_load8<SPLIT>(P, z, m, n, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = n + i < N ? __builtin_fmaf(a, x[i], acc[i] * (1.f / T_SCALE)) : 0.f;
-        img_store4<SPLIT>(P, z, m, n, v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) img_store1<SPLIT>(Q, z, n + i, m, v[i]);
+        for (int i = 0; i < 8; ++i) v[i] = n + i < N ? __builtin_fmaf(a, x[i], v[i] * (1.f / T_SCALE)) : 0.f;
+        img_store8<SPLIT>(P, z, m, n, v);
     }
 };
 template <bool SPLIT, class To>
-struct LastOut {                       // the last step: X in the orientation of the result (P, or Q for tall matrices)
+struct LastOut : NoFactors {           // the last step: X in the orientation of the result (P, or Q for tall matrices)
     Image X;
     float a, scale;                    // scale = 1 / S
     To to;
     int N;
-    DEV void operator()(int z, int m, int n, nt::f32x4 acc) const {
-        const f32x4_t x = img_load4<SPLIT>(X, z, m, n);
+    DEV void put(int z, int m, int n, float *v, Row, Col) const {
+        float x[8];
+        img_load8<SPLIT>(X, z, m, n, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < N) to.put(z, (int64_t)m * N + n + i, __builtin_fmaf(a, x[i], acc[i] * (1.f / T_SCALE)) * scale);
+        for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(a, x[i], v[i] * (1.f / T_SCALE)) * scale;
+        to.put8(z, (int64_t)m * N + n, v, N - n);
     }
 };
 
@@ -389,21 +424,21 @@ int large(const From &from, const To &to, int batch, int64_t rows, int64_t cols,
         hipLaunchKernelGGL((k_zero_pads<SPLIT>), dim3(grid_for((2 * r + c) * pad, 256), 1, batch), dim3(256), 0, st, A, (int64_t)r, B, (int64_t)r, Q2, (int64_t)c, r);
         DPD_LAUNCH_CHECK();
     }
-    auto product = [&](const Image &x, int M, const Image &y, int N, const auto &epi) {
+    auto product = [&](const Image &x, int M, const Image &y, int N, bool symmetric, const auto &epi) {
         nt::Args g{};
         g.a = x.base, g.lda = x.ld, g.a_batch = x.batch, g.b = y.base, g.ldb = y.ld, g.b_batch = y.batch, g.M = M, g.N = N;
-        g.steps = g.wrap = (int)(x.ld / nt::STEP), g.tail = nt::STEP;
+        g.steps = g.wrap = (int)(x.ld / nt::STEP), g.tail = nt::STEP, g.lower = symmetric;
         return nt::product<KIND>(g, batch, epi, st);
     };
     for (int k = 0; k < steps; ++k) {
         const float *f = coef + 3 * k;
-        int rc = product(P, r, P, r, GramOut<SPLIT>{A, T_SCALE / (S * S), r});
-        if (!rc) rc = product(A, r, A, r, PolyOut<SPLIT>{A, B, f[1], f[2], r});
+        int rc = product(P, r, P, r, true, GramOut<SPLIT>{{}, A, T_SCALE / (S * S), r});
+        if (!rc) rc = product(A, r, A, r, true, PolyOut<SPLIT>{{}, A, B, f[1], f[2], r});
         if (!rc && k + 1 < steps) {
-            rc = product(B, r, Q, c, NextOut<SPLIT>{P, Q2, f[0], c});
+            rc = product(B, r, Q, c, false, NextOut<SPLIT>{{}, P, Q2, f[0], c});
             std::swap(Q, Q2);
         } else if (!rc) {
-            rc = wide ? product(B, r, Q, c, LastOut<SPLIT, To>{P, f[0], 1.f / S, to, c}) : product(Q, c, B, r, LastOut<SPLIT, To>{Q, f[0], 1.f / S, to, r});
+            rc = wide ? product(B, r, Q, c, false, LastOut<SPLIT, To>{{}, P, f[0], 1.f / S, to, c}) : product(Q, c, B, r, false, LastOut<SPLIT, To>{{}, Q, f[0], 1.f / S, to, r});
         }
         if (rc) return rc;
     }
@@ -460,7 +495,7 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     if (is_small(rows, cols))
         return with_type(type, [&](auto t) {
             using T = decltype(t);
-            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols}, ToTensor<T>{(T *)out, rows * cols},
+            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols}, ToTensor<T>{(T *)out, rows * cols, false},
                                (int)rows, (int)cols, coef, steps, eps);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
@@ -471,7 +506,7 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const FromTensor<T> from{(const T *)x, rows * cols};
-        const ToTensor<T> to{(T *)out, rows * cols};
+        const ToTensor<T> to{(T *)out, rows * cols, ((uintptr_t)out & 15) == 0 && cols % 8 == 0};
         return accurate ? large<true>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st)
                         : large<false>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st);
     });
@@ -521,7 +556,7 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
             const float factor = (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0));
             if (!is_small(rows, cols)) {
                 const FromMomentum<T> from{(const T *)h_g[i], h_m[i], mu, nesterov};
-                const ToWeights<T> to{(T *)h_p[i], keep, factor};
+                const ToWeights<T> to{(T *)h_p[i], keep, factor, ((uintptr_t)h_p[i] & 15) == 0 && cols % 8 == 0};
                 const int rc = accurate ? large<true>(from, to, 1, rows, cols, steps, coef.v, eps, w, st) : large<false>(from, to, 1, rows, cols, steps, coef.v, eps, w, st);
                 if (rc) return rc;
                 continue;
