@@ -151,6 +151,14 @@ def device(t):
     return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(index):
+    """The current stream of a device as a plain integer (without the Python stream object where torch offers that)."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def stream():
     return c_p(torch.cuda.current_stream().cuda_stream)
 

@@ -36,17 +36,37 @@ DEV int quantise(float x, float s, float inv) {
     return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
-// One row per TEAM threads (a wave, or the whole workgroup).  The row is read twice: the second time from the cache.
-template <class T, int TEAM>
+// One row per TEAM threads (a wave, or the whole workgroup), VEC elements a piece: 16 bytes where the rows allow it, single
+// elements where not.  A thread keeps its first HELD pieces in registers between the two passes and reads the others
+// again.  Bound by memory: 2 + 1 bytes an element (bf16).
+template <class T, int TEAM, int VEC>
 __global__ __launch_bounds__(256) void k_quantize_rows(const T *__restrict__ x, int64_t rows, int cols, int64_t ldx,
                                                        int8_t *__restrict__ q, int64_t ldq, float *__restrict__ scale) {
+    constexpr int HELD = VEC == 1 ? 8 : 4;
+    typedef T TV __attribute__((ext_vector_type(VEC)));
+    typedef int8_t QV __attribute__((ext_vector_type(VEC)));
     __shared__ unsigned top4[4];
     const int t = threadIdx.x % TEAM;
     const int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
     if (TEAM == 64 && row >= rows) return;
-    const T *xr = x + row * ldx;
+    const TV *xr = (const TV *)(x + row * ldx);
+    const int pieces = cols / VEC;
     unsigned top = 0;
-    for (int i = t; i < cols; i += TEAM) top = max(top, abs_bits(to_f32(xr[i])));
+    TV held[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int i = t + h * TEAM;
+        held[h] = i < pieces ? xr[i] : TV{};
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(held[h][e])));
+    for (int i = t + HELD * TEAM; i < pieces; i += TEAM) {
+        const TV v = xr[i];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(v[e])));
+    }
     top = wave_umax(top);
     if (TEAM == 256) {
         if ((threadIdx.x & 63) == 0) top4[threadIdx.x >> 6] = top;
@@ -56,19 +76,32 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const T *__restrict__ x, 
     const float s = row_scale(top);
     const bool fine = top < 0x7f800000u;
     const float inv = 1.0f / s;
-    int8_t *qr = q + row * ldq;
-    for (int i = t; i < ldq; i += TEAM) qr[i] = (fine && i < cols) ? (int8_t)quantise(to_f32(xr[i]), s, inv) : (int8_t)0;
+    QV *qr = (QV *)(q + row * ldq);
+    auto put = [&](int i, TV v) {
+        QV o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] = fine ? (int8_t)quantise(to_f32(v[e]), s, inv) : (int8_t)0;
+        qr[i] = o;
+    };
+    const int all = (int)(ldq / VEC);                 // with the zeros behind the row
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (t + h * TEAM < all) put(t + h * TEAM, held[h]);
+    for (int i = t + HELD * TEAM; i < all; i += TEAM) put(i, i < pieces ? xr[i] : TV{});
     if (t == 0) scale[row] = s;
 }
 
 template <class T>
 int quantize_rows(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *q, int64_t ldq, float *scale, hipStream_t st) {
-    if (cols <= 1024)
-        hipLaunchKernelGGL((k_quantize_rows<T, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, x, rows, cols, ldx, q, ldq, scale);
-    else
-        hipLaunchKernelGGL((k_quantize_rows<T, 256>), dim3((unsigned)rows), dim3(256), 0, st, x, rows, cols, ldx, q, ldq, scale);
-    DPD_LAUNCH_CHECK();
-    return DPD_OK;
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && cols % V == 0 && ((uintptr_t)q & 15) == 0 && ldq % V == 0;
+    auto go = [&](auto kernel, int rows_per_block) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + rows_per_block - 1) / rows_per_block)), dim3(256), 0, st, x, rows, cols, ldx, q, ldq, scale);
+        DPD_LAUNCH_CHECK();
+        return DPD_OK;
+    };
+    if (vec) return cols <= 1024 ? go(k_quantize_rows<T, 64, V>, 4) : go(k_quantize_rows<T, 256, V>, 1);
+    return cols <= 1024 ? go(k_quantize_rows<T, 64, 1>, 4) : go(k_quantize_rows<T, 256, 1>, 1);
 }
 
 template <class T>
@@ -116,6 +149,137 @@ struct PlainOut {
     DEV void put(int, int m, int n, float *v, Row, Col) const { store8(out + (int64_t)m * ldo + n, v, N - n, whole); }
 };
 
+// Few tokens: a workgroup owns 16 output channels and reads their weights once, straight into the fragments of the
+// matrix instruction (64 bytes of 16 rows a load; the waves take the 64-byte steps of the rows in turn and are joined in
+// LDS: integer sums, so the order does not matter).  TB blocks of 16 tokens share the weight fragments; a token row beyond
+// the last one repeats it.  VEC > 0: the tokens are quantised here, VEC elements a piece, by every workgroup for itself,
+// while its first weights are on their way; VEC == 0: they come quantised.  Bound by the read of the weights and by latency.
+constexpr int FEW_HELD = 8;                             // pieces of the tokens that a thread quantises
+
+template <class T, int WAVES, int TB, int VEC>
+__global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T *__restrict__ x, int64_t ldx, int cols, const int8_t *__restrict__ qx, int64_t ld, int M,
+                                                           const int8_t *__restrict__ qw, ScaleOut<T> epi) {
+    constexpr int U = 8;                                // steps of a wave in flight
+    extern __shared__ __attribute__((aligned(16))) char few_lds[];
+    nt::i32x4 *part = (nt::i32x4 *)few_lds;             // [WAVES][TB][64]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, steps = (int)(ld / 64);
+    const int8_t *wr = qw + (int64_t)min(n0 + r, epi.N - 1) * ld + q * 16;
+    nt::i32x4 w[U];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = (i + u) * WAVES + wave;
+            w[u] = s < steps ? *(const nt::i32x4 *)(wr + (int64_t)s * 64) : nt::i32x4{0, 0, 0, 0};
+        }
+    };
+    fetch(0);
+    float scale_of_mine = 0.f;
+    const int8_t *tok[TB];
+    if constexpr (VEC > 0) {
+        typedef T TV __attribute__((ext_vector_type(VEC > 0 ? VEC : 1)));
+        typedef int8_t QV __attribute__((ext_vector_type(VEC > 0 ? VEC : 1)));
+        unsigned *tops = (unsigned *)(few_lds + WAVES * TB * 1024);     // [16]
+        int8_t *mine = (int8_t *)(tops + 16);                           // [M][ld]
+        const int pieces = cols / VEC, total = M * pieces;
+        if (threadIdx.x < 16) tops[threadIdx.x] = 0;
+        for (int i = threadIdx.x; i < M * (int)(ld - cols); i += 64 * WAVES) {      // zeros behind the rows
+            const int m = i / (int)(ld - cols);
+            mine[m * ld + cols + i - m * (int)(ld - cols)] = 0;
+        }
+        TV v[FEW_HELD];
+        int row[FEW_HELD];
+#pragma unroll
+        for (int h = 0; h < FEW_HELD; ++h) {
+            const int e = min((int)threadIdx.x + h * 64 * WAVES, total - 1);        // behind the last piece: again, harmless
+            row[h] = e / pieces;
+            v[h] = *(const TV *)(x + row[h] * ldx + (int64_t)(e - row[h] * pieces) * VEC);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < FEW_HELD; ++h) {
+            if (h * 64 * WAVES >= total) break;
+            unsigned top = 0;
+#pragma unroll
+            for (int e = 0; e < (VEC > 0 ? VEC : 1); ++e) top = max(top, abs_bits(to_f32(v[h][e])));
+            const int first = __builtin_amdgcn_readfirstlane(row[h]);
+            if (__all(row[h] == first)) {
+                top = wave_umax(top);
+                if (lane == 0) atomicMax(tops + first, top);
+            } else {
+                atomicMax(tops + row[h], top);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < FEW_HELD; ++h) {
+            const int e = (int)threadIdx.x + h * 64 * WAVES;
+            if (e >= total) break;
+            const unsigned top = tops[row[h]];
+            const float s = row_scale(top), inv = 1.0f / s;
+            QV o;
+#pragma unroll
+            for (int k = 0; k < (VEC > 0 ? VEC : 1); ++k) o[k] = top < 0x7f800000u ? (int8_t)quantise(to_f32(v[h][k]), s, inv) : (int8_t)0;
+            *(QV *)(mine + row[h] * ld + (e - row[h] * pieces) * VEC) = o;
+        }
+        __syncthreads();
+        scale_of_mine = row_scale(tops[min(r, M - 1)]);
+        tok[0] = mine + min(r, M - 1) * ld + q * 16;
+    } else {
+#pragma unroll
+        for (int b = 0; b < TB; ++b) tok[b] = qx + (int64_t)min(b * 16 + r, M - 1) * ld + q * 16;
+    }
+    nt::i32x4 acc[TB];
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[b] = nt::i32x4{0, 0, 0, 0};
+    for (int i = 0; i * WAVES < steps; i += U) {
+        nt::i32x4 now[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = w[u];
+        if ((i + U) * WAVES < steps) fetch(i + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = min((i + u) * WAVES + wave, steps - 1);         // behind the last step the weights are zeros
+#pragma unroll
+            for (int b = 0; b < TB; ++b) acc[b] = nt::mfma<nt::I8>(now[u], *(const nt::i32x4 *)(tok[b] + (int64_t)s * 64), acc[b]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < TB; ++b) part[(wave * TB + b) * 64 + lane] = acc[b];
+    __syncthreads();
+    if (wave >= TB) return;                             // wave b finishes token block b
+    nt::i32x4 sum = nt::i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) sum += part[(k * TB + wave) * 64 + lane];
+    const int m = wave * 16 + r, n = n0 + q * 4;
+    if (m >= M || n >= epi.N) return;
+    const float s = VEC > 0 ? scale_of_mine : epi.sa[m];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < epi.N) {
+            float v = (float)sum[e] * s * epi.sb[n + e];
+            if (epi.bias) v += load_any(epi.bias, epi.bias_type, n + e);
+            epi.out[(int64_t)m * epi.ldo + n + e] = from_f32<T>(v);
+        }
+}
+
+// Pieces of the tokens for one workgroup: 0 if it should get them quantised.
+template <class T>
+int fused_pieces(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, int threads) {
+    constexpr int V = 16 / sizeof(T);
+    if (M > 16 || M * ld > 32768) return 0;
+    const bool vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && K % V == 0;
+    return M * (K / (vec ? V : 1)) <= (int64_t)FEW_HELD * threads ? (vec ? V : 1) : 0;
+}
+
+template <class T, int WAVES, int TB, int VEC>
+int few_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, const int8_t *qx, int64_t ld, const int8_t *qw, const ScaleOut<T> &epi, hipStream_t st) {
+    const size_t lds = WAVES * TB * 1024 + (VEC ? 64 + M * ld : 0);
+    hipLaunchKernelGGL((k_few_tokens<T, WAVES, TB, VEC>), dim3((unsigned)((epi.N + 15) / 16)), dim3(64 * WAVES), lds, st, x, ldx, (int)K, qx, ld, (int)M, qw, epi);
+    DPD_LAUNCH_CHECK();
+    return DPD_OK;
+}
+
 // rows of an int8 matrix at a stride that the product can read (a multiple of 128 bytes, zeros behind the row)
 __global__ __launch_bounds__(256) void k_pad_rows(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld,
                                                   int8_t *__restrict__ out, int64_t ldo) {
@@ -149,37 +313,58 @@ template <class T>
 constexpr int planes_of() { return std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2; }
 
 template <int P>
-DEV void put_planes(__bf16 *p, int64_t plane, float v) {
+DEV void put_planes8(__bf16 *p, int64_t plane, const float *v) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rest[e] = v[e];
 #pragma unroll
     for (int i = P - 1; i >= 0; --i) {
-        const __bf16 h = (__bf16)v;
-        p[i * plane] = h;
-        v = fabsf((float)h) < INFINITY ? v - (float)h : 0.f;      // an infinity stays one: nothing is left of it
+        b8 o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[e] = (__bf16)rest[e];
+            rest[e] = fabsf((float)o[e]) < INFINITY ? rest[e] - (float)o[e] : 0.f;      // an infinity stays one: nothing is left of it
+        }
+        *(b8 *)(p + i * plane) = o;
     }
 }
 
 // One 64 x 64 tile of g [M, N]: gs[m, n] = g sw[n] (row-major, for gx), gt[n, m] = g sx[m] (transposed, for gw), each as
-// bf16 planes with zeros behind the rows, and this tile's column sums for gb.
+// bf16 planes with zeros behind the rows, and this tile's column sums for gb.  Pieces of 8 elements on every access; bound
+// by memory (2 + 2 or 4 bytes an element in bf16).
 template <class T>
-__global__ __launch_bounds__(256) void k_grad_images(const T *__restrict__ g, int64_t M, int N, int64_t ldg, const float *__restrict__ sw,
+__global__ __launch_bounds__(256) void k_grad_images(const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
                                                      const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad,
                                                      __bf16 *__restrict__ gt, int64_t m_pad, float *__restrict__ gb_part) {
     constexpr int P = planes_of<T>();
     __shared__ float t[64][65];
     const int64_t m0 = (int64_t)blockIdx.x * 64;
     const int n0 = blockIdx.y * 64;
-    for (int e = threadIdx.x; e < 4096; e += 256) {
-        const int i = e >> 6, j = e & 63;
-        const float v = (m0 + i < M && n0 + j < N) ? to_f32(g[(m0 + i) * ldg + n0 + j]) : 0.f;
-        t[i][j] = v;
-        if (gs && m0 + i < M) put_planes<P>(gs + (m0 + i) * (P * n_pad) + n0 + j, n_pad, n0 + j < N ? v * sw[n0 + j] : 0.f);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int e = threadIdx.x + h * 256, i = e >> 3, j = (e & 7) * 8;
+        float v[8] = {};
+        if (m0 + i < M && n0 + j < N) load8(g + (m0 + i) * ldg + n0 + j, v, N - n0 - j, whole);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[i][j + k] = v[k];
+        if (gs && m0 + i < M) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = n0 + j + k < N ? v[k] * sw[n0 + j + k] : 0.f;
+            put_planes8<P>(gs + (m0 + i) * (P * n_pad) + n0 + j, n_pad, v);
+        }
     }
     __syncthreads();
-    if (gt)
-        for (int e = threadIdx.x; e < 4096; e += 256) {
-            const int j = e >> 6, i = e & 63;
-            if (n0 + j < N) put_planes<P>(gt + (int64_t)(n0 + j) * (P * m_pad) + m0 + i, m_pad, m0 + i < M ? t[i][j] * sx[m0 + i] : 0.f);
+    if (gt) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = threadIdx.x + h * 256, j = e >> 3, i = (e & 7) * 8;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = m0 + i + k < M ? t[i + k][j] * sx[m0 + i + k] : 0.f;
+            if (n0 + j < N) put_planes8<P>(gt + (int64_t)(n0 + j) * (P * m_pad) + m0 + i, m_pad, v);
         }
+    }
     if (gb_part && threadIdx.x < 64 && n0 + threadIdx.x < N) {
         float s = 0.f;
         for (int i = 0; i < 64; ++i) s += t[i][threadIdx.x];
@@ -187,29 +372,60 @@ __global__ __launch_bounds__(256) void k_grad_images(const T *__restrict__ g, in
     }
 }
 
+// Sums the tiles' column sums in fp64: 32 columns a workgroup, 8 threads a column.
 template <class T>
 __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ part, int64_t blocks, int N, T *__restrict__ gb) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ double red[8][32];
+    const int c = threadIdx.x & 31, k = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
     double s = 0.0;
-    for (int64_t b = 0; b < blocks; ++b) s += (double)part[b * N + n];
-    gb[n] = from_f32<T>((float)s);
+    if (n < N)
+        for (int64_t b = k; b < blocks; b += 8) s += (double)part[b * N + n];
+    red[k][c] = s;
+    __syncthreads();
+    if (k == 0 && n < N) {
+        for (int i = 1; i < 8; ++i) s += red[i][c];
+        gb[n] = from_f32<T>((float)s);
+    }
 }
 
-// q [rows, cols] int8 -> out [cols, rows_pad] bf16 (exact), zeros behind the rows
-__global__ __launch_bounds__(256) void k_transpose_i8(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld,
-                                                      __bf16 *__restrict__ out, int64_t rows_pad) {
-    __shared__ int8_t t[64][68];
+// q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves (exact), or, with the
+// scales of the rows, their values rounded to bf16.
+__global__ __launch_bounds__(256) void k_transpose_i8(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld, bool whole,
+                                                      const float *__restrict__ scale, __bf16 *__restrict__ out, int64_t rows_pad) {
+    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+    typedef int8_t c16 __attribute__((ext_vector_type(16)));
+    __shared__ int8_t t[64][72];                      // [column][row]
     const int64_t r0 = (int64_t)blockIdx.x * 64;
     const int c0 = blockIdx.y * 64;
-    for (int e = threadIdx.x; e < 4096; e += 256) {
-        const int i = e >> 6, j = e & 63;
-        t[i][j] = (r0 + i < rows && c0 + j < cols) ? q[(r0 + i) * ld + c0 + j] : (int8_t)0;
+    {
+        const int i = threadIdx.x >> 2, j = (threadIdx.x & 3) * 16;
+        c16 v = {};
+        if (r0 + i < rows && c0 + j < cols) {
+            const int8_t *p = q + (r0 + i) * ld + c0 + j;
+            if (whole && (c0 + j + 16 <= cols || r0 + i + 1 < rows)) {      // the row's memory goes on to a multiple of 16 elements
+                v = *(const c16 *)p;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    if (c0 + j + k < cols) v[k] = p[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t[j + k][i] = v[k];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 4096; e += 256) {
-        const int j = e >> 6, i = e & 63;
-        if (c0 + j < cols) out[(int64_t)(c0 + j) * rows_pad + r0 + i] = (__bf16)(float)t[i][j];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int e = threadIdx.x + h * 256, j = e >> 3, i = (e & 7) * 8;
+        if (c0 + j >= cols) continue;
+        b8 o;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float v = (float)t[j][i + k];
+            if (scale) v = r0 + i + k < rows ? v * scale[r0 + i + k] : 0.f;
+            o[k] = (__bf16)v;
+        }
+        *(b8 *)(out + (int64_t)(c0 + j) * rows_pad + r0 + i) = o;
     }
 }
 
@@ -235,6 +451,8 @@ struct BackwardPlan {
     }
 };
 
+bool whole16(const int8_t *q, int64_t ld, int64_t cols) { return ((uintptr_t)q & 15) == 0 && ld % 16 == 0 && ld >= nt::pad_to(cols, 16); }
+
 template <class T>
 int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const int8_t *qx, int64_t ldqx, const float *sx,
               const int8_t *qw, int64_t ldqw, const float *sw, T *gx, void *gw, int gw_type, void *gb, int gb_type, char *ws, hipStream_t st) {
@@ -243,29 +461,36 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
     __bf16 *gs = gx ? (__bf16 *)(ws + p.gs) : nullptr, *wt = (__bf16 *)(ws + p.wt), *gt = gw ? (__bf16 *)(ws + p.gt) : nullptr,
            *xt = (__bf16 *)(ws + p.xt);
     float *part = gb ? (float *)(ws + p.part) : nullptr;
-    hipLaunchKernelGGL((k_grad_images<T>), dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 64)), dim3(256), 0, st, g, M, (int)N, ldg, sw,
-                       sx, gs, p.n_pad, gt, p.m_pad, part);
-    DPD_LAUNCH_CHECK();
+    // bf16 gradients whose rows the product can read are its operand as they are; the weight's scales then go into the other
+    // one, rounded to bf16 there instead of in g times scale (one rounding of 2^-8 a term either way)
+    const bool direct = P == 1 && ((uintptr_t)g & 15) == 0 && ldg % 8 == 0 && N % 8 == 0 && ldg * 2 <= nt::MAX_ROW_BYTES;
+    if (direct) gs = nullptr;
+    if (gs || gt || part) {
+        hipLaunchKernelGGL((k_grad_images<T>), dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 64)), dim3(256), 0, st, g, M, (int)N, ldg,
+                           whole8(g, ldg), sw, sx, gs, p.n_pad, gt, p.m_pad, part);
+        DPD_LAUNCH_CHECK();
+    }
     if (gb) {
         const int rc = with_type(gb_type, [&](auto t) {
             using B = decltype(t);
-            hipLaunchKernelGGL((k_bias_grad<B>), dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, part, p.m_pad / 64, (int)N, (B *)gb);
+            hipLaunchKernelGGL((k_bias_grad<B>), dim3((unsigned)((N + 31) / 32)), dim3(256), 0, st, part, p.m_pad / 64, (int)N, (B *)gb);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
         });
         if (rc) return rc;
     }
     if (gx) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.n_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qw, N, (int)K, ldqw, wt, p.n_pad);
+        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.n_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qw, N, (int)K, ldqw, whole16(qw, ldqw, K), direct ? sw : nullptr, wt, p.n_pad);
         DPD_LAUNCH_CHECK();
         nt::Args a{};
-        a.a = (const char *)gs, a.lda = P * p.n_pad * 2, a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
-        a.wrap = (int)(p.n_pad / 64), a.steps = P * a.wrap, a.tail = 128;
+        a.a = direct ? (const char *)g : (const char *)gs, a.lda = direct ? ldg * 2 : P * p.n_pad * 2;
+        a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
+        a.wrap = (int)(p.n_pad / 64), a.steps = P * a.wrap, a.tail = direct ? (int)(N * 2 - (int64_t)(a.steps - 1) * 128) : 128;
         const int rc = nt::product<nt::BF16>(a, 1, PlainOut<T>{gx, K, (int)K, whole8(gx, K)}, st);
         if (rc) return rc;
     }
     if (gw) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.m_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qx, M, (int)K, ldqx, xt, p.m_pad);
+        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.m_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qx, M, (int)K, ldqx, whole16(qx, ldqx, K), (const float *)nullptr, xt, p.m_pad);
         DPD_LAUNCH_CHECK();
         nt::Args a{};
         a.a = (const char *)gt, a.lda = P * p.m_pad * 2, a.b = (const char *)xt, a.ldb = p.m_pad * 2, a.M = (int)N, a.N = (int)K;
@@ -382,8 +607,22 @@ extern "C" int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, in
     hipStream_t st = as_stream(stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const int rc = quantize_rows((const T *)x, M, (int)K, ldx, qx, ld, sx, st);
-        return rc ? rc : int8_product(qx, ld, sx, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
+        const T *xt = (const T *)x;
+        const ScaleOut<T> epi{sx, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
+        // a workgroup of four waves: 16 channels each fill the chip from 4096 channels on; with fewer, and long rows, 16 waves
+        const bool tall = N < 2048 && ld >= 2048;
+        if (M <= 16) {
+            constexpr int V = 16 / sizeof(T);
+            const int vec = fused_pieces(xt, M, K, ldx, ld, tall ? 1024 : 256);
+            if (vec == V) return tall ? few_tokens<T, 16, 1, V>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, V>(xt, M, K, ldx, qx, ld, qw, epi, st);
+            if (vec == 1) return tall ? few_tokens<T, 16, 1, 1>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, 1>(xt, M, K, ldx, qx, ld, qw, epi, st);
+        }
+        const int rc = quantize_rows(xt, M, (int)K, ldx, qx, ld, sx, st);
+        if (rc) return rc;
+        if (M <= 16) return tall ? few_tokens<T, 16, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
+        if (M <= 32) return tall ? few_tokens<T, 16, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
+        if (M <= 64) return tall ? few_tokens<T, 16, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
+        return int8_product(qx, ld, sx, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
     });
 }
 

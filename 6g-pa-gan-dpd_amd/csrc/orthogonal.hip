@@ -26,6 +26,9 @@ template <class T>
 struct FromTensor {                                   // a matrix of a batch
     const T *x;
     int64_t batch;
+    bool whole;                                       // matrices and rows of whole 16-byte pieces
+    DEV void first8(int z, int64_t i, float *v, int valid) const { load8(x + z * batch + i, v, valid, whole); }
+    DEV void again8(int z, int64_t i, float *v, int valid) const { load8(x + z * batch + i, v, valid, whole); }
     DEV float first(int z, int64_t i) const { return to_f32(x[z * batch + i]); }
     DEV float again(int z, int64_t i) const { return to_f32(x[z * batch + i]); }
 };
@@ -35,6 +38,25 @@ struct FromMomentum {                                 // g and the momentum, whi
     float *m;
     float mu;
     int nesterov;
+    bool whole;
+    DEV void first8(int, int64_t i, float *v, int valid) const {
+        float w[8];
+        load8(m + i, w, valid, whole);
+        load8(g + i, v, valid, whole);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            w[k] = mu * w[k] + v[k];
+            v[k] = nesterov ? v[k] + mu * w[k] : w[k];
+        }
+        store8(m + i, w, valid, whole);
+    }
+    DEV void again8(int, int64_t i, float *v, int valid) const {
+        float w[8];
+        load8((const float *)m + i, w, valid, whole);
+        if (nesterov) load8(g + i, v, valid, whole);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = nesterov ? v[k] + mu * w[k] : w[k];
+    }
     DEV float first(int, int64_t i) const {
         m[i] = mu * m[i] + to_f32(g[i]);
         return again(0, i);
@@ -197,7 +219,7 @@ template <class T>
 __global__ __launch_bounds__(256) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
     __shared__ float lds[SMALL_LDS];
     const int z = blockIdx.x;
-    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
+    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov, false}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
                   tab.cols[z], coef, steps, eps, lds);
 }
 
@@ -246,9 +268,11 @@ __global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__re
     __shared__ double red[4];
     const int z = blockIdx.z;
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const double v = (double)from.first(z, i);
-        s += v * v;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+        float v[8];
+        from.first8(z, i, v, (int)(n - i < 8 ? n - i : 8));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += (double)v[k] * (double)v[k];
     }
     s = block_sum_d(s, red);
     if (threadIdx.x == 0) part[z * NORM_BLOCKS + blockIdx.x] = s;
@@ -266,9 +290,13 @@ __global__ __launch_bounds__(256) void k_prepare(From from, int rows, int cols, 
     const double norm = sqrt(block_sum_d(s, red)), inv = scale / (norm > eps ? norm : (norm == norm ? eps : norm));
     const bool wide = rows <= cols;
     const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;          // of x
-    for (int e = t; e < 4096; e += 256) {
-        const int i = e >> 6, j = e & 63;
-        tile[i][j] = (r0 + i < rows && c0 + j < cols) ? (float)((double)from.again(z, (int64_t)(r0 + i) * cols + c0 + j) * inv) : 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int e = t + h * 256, i = e >> 3, j = (e & 7) * 8;
+        float v[8] = {};
+        if (r0 + i < rows && c0 + j < cols) from.again8(z, (int64_t)(r0 + i) * cols + c0 + j, v, cols - c0 - j);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tile[i][j + k] = (float)((double)v[k] * inv);
     }
     __syncthreads();
     const Image &same = wide ? P : Q, &flip = wide ? Q : P;        // the image in x's orientation, and the other one
@@ -495,7 +523,7 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     if (is_small(rows, cols))
         return with_type(type, [&](auto t) {
             using T = decltype(t);
-            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols}, ToTensor<T>{(T *)out, rows * cols, false},
+            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols, false}, ToTensor<T>{(T *)out, rows * cols, false},
                                (int)rows, (int)cols, coef, steps, eps);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
@@ -505,7 +533,7 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const FromTensor<T> from{(const T *)x, rows * cols};
+        const FromTensor<T> from{(const T *)x, rows * cols, ((uintptr_t)x & 15) == 0 && cols % 8 == 0};
         const ToTensor<T> to{(T *)out, rows * cols, ((uintptr_t)out & 15) == 0 && cols % 8 == 0};
         return accurate ? large<true>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st)
                         : large<false>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st);
@@ -555,7 +583,7 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
             if (rows == 0 || cols == 0) continue;
             const float factor = (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0));
             if (!is_small(rows, cols)) {
-                const FromMomentum<T> from{(const T *)h_g[i], h_m[i], mu, nesterov};
+                const FromMomentum<T> from{(const T *)h_g[i], h_m[i], mu, nesterov, (((uintptr_t)h_g[i] | (uintptr_t)h_m[i]) & 15) == 0 && cols % 8 == 0};
                 const ToWeights<T> to{(T *)h_p[i], keep, factor, ((uintptr_t)h_p[i] & 15) == 0 && cols % 8 == 0};
                 const int rc = accurate ? large<true>(from, to, 1, rows, cols, steps, coef.v, eps, w, st) : large<false>(from, to, 1, rows, cols, steps, coef.v, eps, w, st);
                 if (rc) return rc;

@@ -199,30 +199,33 @@ class Int8Inference:
         self.scale = _check_scale(s, n, w.device, "scale").clone()
         bc, self._bias_type = _check_bias(b, n, w.device)
         self.bias = None if bc is None else bc.detach().clone()
-        self._w = (L.c_p(self.image.data_ptr()), L.c_p(self.scale.data_ptr()), L.c_p(0 if self.bias is None else self.bias.data_ptr()))
+        self._w = (self.image.data_ptr(), self.scale.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
+        self._fn = L.lib().dpd_int8_linear
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [..., K] -> [..., N] in the type of x.  `out` (optional: [..., N], contiguous, the type of x, apart from x in
         memory) receives the result in place of a new tensor."""
         k, n = self.in_features, self.out_features
-        t = _type(x, "x")
-        if x.dim() < 1 or x.shape[-1] != k:
-            raise ValueError(f"expected {k} input features, got {tuple(x.shape)}")
+        t = TYPES.get(x.dtype)
+        if t is None:
+            _type(x, "x")
+        shape = x.shape
+        if not shape or shape[-1] != k:
+            raise ValueError(f"expected {k} input features, got {tuple(shape)}")
         if x.device != self.device:
             raise RuntimeError(f"the weights are on {self.device}, the tokens on {x.device}")
-        x2, ldx = _rows(x.detach())
+        x2, ldx = _rows(x)
         m = x2.shape[0]
-        shape = (*x.shape[:-1], n)
         if out is None:
-            out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        elif tuple(out.shape) != shape or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device or out.requires_grad:
-            raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {shape} on {x.device} without gradient")
+            out = torch.empty((*shape[:-1], n), dtype=x.dtype, device=self.device)
+        elif out.shape != (*shape[:-1], n) or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device or out.requires_grad:
+            raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {(*shape[:-1], n)} on {x.device} without gradient")
         elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise RuntimeError("out must not share memory with x")
+        nbytes = m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256                # dpd_int8_linear_workspace_bytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        qw, sw, b = self._w
         with L.device(x):
-            nbytes = L.lib().dpd_int8_linear_workspace_bytes(m, n, k)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            qw, sw, b = self._w
-            L.call("dpd_int8_linear", L.c_p(x2.data_ptr()), t, m, k, ldx, qw, sw, b, self._bias_type, n, L.c_p(out.data_ptr()), n,
-                   L.c_p(ws.data_ptr()), nbytes, L.stream())
+            L.check(self._fn(x2.data_ptr(), t, m, k, ldx, qw, sw, b, self._bias_type, n, out.data_ptr(), n, ws.data_ptr(), nbytes,
+                             L.raw_stream(self.device.index)))
         return out

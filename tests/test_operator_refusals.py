@@ -156,3 +156,11 @@ def test_train_configuration_names_the_optimizer():
     with pytest.raises(ValueError, match="lion"):
         create_optimizers(gen, disc, config)
     assert build_parser().parse_args(["--optimizer", "muon"]).optimizer == "muon"
+
+
+def test_serving_workspace_formula():
+    """The engine computes the size of its scratch itself."""
+    from dpd_amd.utils.int8 import _row_bytes
+    for m, n, k in ((0, 4, 1), (1, 4, 1), (7, 9, 128), (64, 3, 129), (1000, 5, 4096)):
+        assert L.lib().dpd_int8_linear_workspace_bytes(m, n, k) == m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256
+        assert L.lib().dpd_int8_row_bytes(k) == _row_bytes(k)
