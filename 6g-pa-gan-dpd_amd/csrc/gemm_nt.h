@@ -8,6 +8,7 @@
 // The loop runs half a step ahead of itself: while the first fragments of a step are multiplied the second ones are
 // read, and while those are multiplied the first ones of the next step.  One barrier a step, between the halves: behind
 // it every wave has read all of this step's stage (which is filled again, STAGES steps ahead) and seen its successor.
+// WAVES_K groups of such waves take the steps in turn, each with its part of a stage, and are added at the end.
 //
 // LDS layout: row r keeps its 16-byte chunk c at position c ^ key(r).  The direct load writes lane after lane, so the
 // permutation is applied to the global chunk a lane asks for.  Keys are chosen so that the 16 lanes that read together
@@ -124,10 +125,10 @@ DEV void wait_barrier() {
     asm volatile("" ::: "memory");
 }
 
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int WAVES_K, int STAGES, class Epilogue>
 DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     constexpr int WAVES = WAVES_M * WAVES_N, TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
-    constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B, STAGE = (BM + BN) * STEP;
+    constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B, PART = (BM + BN) * STEP, STAGE = WAVES_K * PART;
     static_assert(LOADS_A >= 1 && LOADS_B >= 1 && LOADS_A * 8 * WAVES == BM && LOADS_B * 8 * WAVES == BN, "every wave loads whole groups of 8 rows");
     static_assert(TN % 2 == 0 && (TM % 2 == 0 || KIND != F16_SPLIT) && STAGES >= 2 && (STAGES - 2) * LOADS < 64, "pairs of blocks; the wait counter has 6 bits");
     static_assert(STAGES * STAGE <= 160 * 1024, "LDS of a compute unit");
@@ -135,8 +136,10 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     int tm, tn;
     tile_of(g, blockIdx.x, gridDim.x, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WAVES_N, wn = wave % WAVES_N;
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all_waves / WAVES, wave = all_waves % WAVES, wm = wave / WAVES_N, wn = wave % WAVES_N;
+    char *const mine = smem + group * PART;                // this group's part of every stage
+    const int steps = (g.steps + WAVES_K - 1) / WAVES_K;   // of a group: group k takes the steps k, k + WAVES_K, ...
 
     const char *ab = g.a + blockIdx.z * g.a_batch + (int64_t)m0 * g.lda, *bb = g.b + blockIdx.z * g.b_batch + (int64_t)n0 * g.ldb;
     // rows beyond the last read it again (their results are not stored); chunks beyond `tail` lie outside the resource
@@ -150,24 +153,29 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     for (int i = 0; i < LOADS_A; ++i) va[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.M - 1 - m0) * (int)g.lda + chunk_a(i));
 #pragma unroll
     for (int i = 0; i < LOADS_B; ++i) vb[i] = (unsigned)(min((i * WAVES + wave) * 8 + (lane >> 3), g.N - 1 - n0) * (int)g.ldb + chunk_b(i));
-    int wrapped = 0;                                       // step of the B operand that is loaded next
+    int wrapped = group % g.wrap;                          // step of the B operand that is loaded next
     auto load = [&](int i, int s, int at) {                // 8 rows: part i of LOADS
         if (i < LOADS_A)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *)(smem + at + (i * WAVES + wave) * 1024), 16, va[i], s * STEP, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void *)(mine + at + (i * WAVES + wave) * 1024), 16, va[i], (s * WAVES_K + group) * STEP, 0, 0);
         else
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(smem + at + BM * STEP + ((i - LOADS_A) * WAVES + wave) * 1024), 16, vb[i - LOADS_A],
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void *)(mine + at + BM * STEP + ((i - LOADS_A) * WAVES + wave) * 1024), 16, vb[i - LOADS_A],
                                                      wrapped * STEP, 0, 0);
     };
-    const int cut_step = g.tail == STEP ? -1 : g.steps - 1;
-    auto before_loads = [&](int s) {                       // chunks that the last step does not have
+    // chunks that the last step does not have, and steps that do not exist (a group's last): zeros
+    const int cut_step = g.tail == STEP && WAVES_K == 1 ? -1 : steps - 1;
+    auto before_loads = [&](int s) {
         if (s == cut_step) {
+            const int have = s * WAVES_K + group, tail = have < g.steps - 1 ? STEP : have == g.steps - 1 ? g.tail : 0;
 #pragma unroll
-            for (int i = 0; i < LOADS_A; ++i) va[i] = chunk_a(i) >= g.tail ? 0xfffffff0u : va[i];
+            for (int i = 0; i < LOADS_A; ++i) va[i] = chunk_a(i) >= tail ? 0xfffffff0u : va[i];
 #pragma unroll
-            for (int i = 0; i < LOADS_B; ++i) vb[i] = chunk_b(i) >= g.tail ? 0xfffffff0u : vb[i];
+            for (int i = 0; i < LOADS_B; ++i) vb[i] = chunk_b(i) >= tail ? 0xfffffff0u : vb[i];
         }
     };
-    auto after_loads = [&]() { wrapped = wrapped == g.wrap - 1 ? 0 : wrapped + 1; };
+    auto after_loads = [&]() {
+        wrapped += WAVES_K;
+        while (wrapped >= g.wrap) wrapped -= g.wrap;
+    };
 
     typename Acc<KIND>::type acc[TM][TN];
 #pragma unroll
@@ -177,7 +185,7 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
 
     // fragment c (0 or 1) of block i of A, of block j of B: the keys do not depend on i and j
     const int r = lane & 15, q = lane >> 4;
-    const char *pa = smem + (wm * TM * 16 + r) * STEP, *pb = smem + (BM + wn * TN * 16) * STEP;
+    const char *pa = mine + (wm * TM * 16 + r) * STEP, *pb = mine + (BM + wn * TN * 16) * STEP;
     const int ka[2] = {(q ^ key_a(r)) * 16, ((4 + q) ^ key_a(r)) * 16};
     const int kb[2] = {b_row(0, r) * STEP + (q ^ key_b(b_row(0, r))) * 16, b_row(0, r) * STEP + ((4 + q) ^ key_b(b_row(0, r))) * 16};
     constexpr bool SPLIT = KIND == F16_SPLIT;
@@ -210,13 +218,13 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
 
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
-        if (s < g.steps) {
+        if (s < steps) {
             before_loads(s);
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) load(i, s, s * STAGE);
             after_loads();
         }
-    if (g.steps >= STAGES) wait_barrier<(STAGES - 1) * LOADS>();
+    if (steps >= STAGES) wait_barrier<(STAGES - 1) * LOADS>();
     else wait_barrier<0>();
 #pragma unroll
     for (int i = 0; i < (SPLIT ? 1 : TM); ++i) reada(a0, i, i, 0, 0);
@@ -295,11 +303,33 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     };
     int s = 0;
     if constexpr (SPLIT) {
-        for (; s + STAGES < g.steps; ++s) step_split(s, Yes{});
-        for (; s < g.steps; ++s) step_split(s, No{});
+        for (; s + STAGES < steps; ++s) step_split(s, Yes{});
+        for (; s < steps; ++s) step_split(s, No{});
     } else {
-        for (; s + STAGES < g.steps; ++s) step(s, Yes{});
-        for (; s < g.steps; ++s) step(s, No{});
+        for (; s + STAGES < steps; ++s) step(s, Yes{});
+        for (; s < steps; ++s) step(s, No{});
+    }
+    if constexpr (WAVES_K > 1) {                           // the groups' sums meet in the first one, in order
+        static_assert((WAVES_K - 1) * BM * BN * 4 <= STAGES * STAGE, "the partial tiles fit into LDS");
+        typedef typename Acc<KIND>::type V;
+        V *parts = (V *)smem;
+        __syncthreads();
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) parts[(((group - 1) * WAVES + wave) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
+        }
+        __syncthreads();
+        if (group > 0 && !Epilogue::TURNED) return;
+        if (group == 0) {
+#pragma unroll
+            for (int k = 0; k < WAVES_K - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] += parts[((k * WAVES + wave) * TM * TN + i * TN + j) * 64 + lane];
+        }
     }
     typename Epilogue::Col col[TN / 2];
 #pragma unroll
@@ -316,6 +346,7 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
             float v[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][2 * j][e], v[4 + e] = (float)acc[i][2 * j + 1][e];
+            if (WAVES_K > 1 && group > 0) continue;
             if (m < g.M && n < g.N) {
                 epi.put(blockIdx.z, m, n, v, row, col[j]);
             } else if (Epilogue::TURNED) {
@@ -344,13 +375,14 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
+                        if (WAVES_K > 1 && group > 0) break;
                         const int ml = (wm * TM + i) * 16 + r, nl = wn * TN * 16 + (j >> 1) * 32 + q * 8 + (j & 1) * 4 + e;
                         const _Float16 h = (_Float16)acc[i][j][e];
                         t[nl * BM + (((ml >> 3) ^ ((nl >> 3) & MASK)) << 3) + (ml & 7)] = h;
                         if (SPLIT) acc[i][j][e] -= (float)h;
                     }
             __syncthreads();
-            for (int k = threadIdx.x; k < BN * CHUNKS; k += 64 * WAVES) {
+            for (int k = threadIdx.x; k < BN * CHUNKS; k += 64 * WAVES * WAVES_K) {
                 const int nl = k / CHUNKS, c = k - nl * CHUNKS;
                 if (n0 + nl < g.N && m0 + c * 8 < g.M)
                     epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * BM + ((c ^ ((nl >> 3) & MASK)) << 3)));
@@ -359,49 +391,55 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     }
 }
 
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
-static __global__ __launch_bounds__(64 * WAVES_M *WAVES_N) void k_gemm(Args g, Epilogue epi) {
-    gemm_tile<KIND, BM, BN, WAVES_M, WAVES_N, STAGES>(g, epi);
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int WAVES_K, int STAGES, class Epilogue>
+static __global__ __launch_bounds__(64 * WAVES_M *WAVES_N *WAVES_K) void k_gemm(Args g, Epilogue epi) {
+    gemm_tile<KIND, BM, BN, WAVES_M, WAVES_N, WAVES_K, STAGES>(g, epi);
 }
 
 // ---- host side -------------------------------------------------------------------------
-template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int STAGES, class Epilogue>
+template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int WAVES_K, int STAGES, class Epilogue>
 static int launch(Args g, int batch, const Epilogue &epi, hipStream_t st) {
     g.tiles_m = (g.M + BM - 1) / BM;
     g.tiles_n = (g.N + BN - 1) / BN;
-    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, STAGES, Epilogue>), dim3((unsigned)tiles_of(g), 1, (unsigned)batch),
-                       dim3(64 * WAVES_M * WAVES_N), 0, st, g, epi);
+    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, WAVES_K, STAGES, Epilogue>), dim3((unsigned)tiles_of(g), 1, (unsigned)batch),
+                       dim3(64 * WAVES_M * WAVES_N * WAVES_K), 0, st, g, epi);
     DPD_LAUNCH_CHECK();
     return DPD_OK;
 }
 
-// Which tile: the one whose rounds over the 256 compute units (one tile each) are estimated to take least.
-// Measured (4096 and 2048 rows, us): a round of steps costs about steps * per_step + fixed.
+// Which tile: the one whose rounds over the 256 compute units (one workgroup each) are estimated to take least.  Measured
+// with fp16 operands and a full round (1024 to 4096 rows, us): steps * per_step + fixed; the split form takes 1.45 times as
+// long a step, and needs an even number of block rows a wave.
 struct TileCost {
     int bm, bn;
     float per_step, fixed;
+    bool split;
 };
-constexpr TileCost TILES[] = {{256, 256, 1.35f, 10.f}, {256, 128, 0.82f, 7.f}, {192, 192, 0.8f, 8.f}, {128, 128, 0.46f, 4.5f}, {64, 64, 0.21f, 3.f}};
+constexpr TileCost TILES[] = {{256, 256, 1.35f, 10.f, true}, {256, 128, 0.88f, 6.5f, true}, {192, 192, 0.92f, 7.f, true}, {128, 128, 0.49f, 4.3f, true},
+                              {128, 64, 0.33f, 4.f, true},   {96, 96, 0.29f, 4.f, false},   {64, 64, 0.19f, 3.1f, true}};
 
 template <int KIND, class Epilogue>
 static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st) {
-    int best = 0;
+    int best = -1;
     float least = 0.f;
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 7; ++i) {
         const TileCost &t = TILES[i];
-        if (g.lower && t.bm != t.bn) continue;
+        if ((g.lower && t.bm != t.bn) || (KIND == F16_SPLIT && !t.split)) continue;
         Args a = g;
         a.tiles_m = (g.M + t.bm - 1) / t.bm, a.tiles_n = (g.N + t.bn - 1) / t.bn;
         const int64_t rounds = ((int64_t)tiles_of(a) * batch + 255) / 256;
-        const float cost = (float)rounds * ((float)g.steps * (KIND == F16_SPLIT ? 1.5f : 1.f) * t.per_step + t.fixed);
-        if (i == 0 || cost < least) best = i, least = cost;
+        const float cost = (float)rounds * ((float)g.steps * (KIND == F16_SPLIT ? 1.45f : 1.f) * t.per_step + t.fixed);
+        if (best < 0 || cost < least) best = i, least = cost;
     }
     switch (best) {
-    case 0: return launch<KIND, 256, 256, 2, 4, 2>(g, batch, epi, st);
-    case 1: return launch<KIND, 256, 128, 4, 2, 3>(g, batch, epi, st);
-    case 2: return launch<KIND, 192, 192, 2, 2, 3>(g, batch, epi, st);
-    case 3: return launch<KIND, 128, 128, 2, 4, 4>(g, batch, epi, st);
-    default: return launch<KIND, 64, 64, 2, 2, 8>(g, batch, epi, st);
+    case 0: return launch<KIND, 256, 256, 2, 4, 1, 2>(g, batch, epi, st);
+    case 1: return launch<KIND, 256, 128, 4, 2, 1, 3>(g, batch, epi, st);
+    case 2: return launch<KIND, 192, 192, 2, 2, 1, 3>(g, batch, epi, st);
+    case 3: return launch<KIND, 128, 128, 2, 4, 1, 4>(g, batch, epi, st);
+    case 4: return launch<KIND, 128, 64, 4, 2, 1, 6>(g, batch, epi, st);
+    case 5:
+        if constexpr (KIND != F16_SPLIT) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
+    default: return launch<KIND, 64, 64, 2, 2, 2, 4>(g, batch, epi, st);
     }
 }
 

@@ -389,39 +389,49 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ par
 }
 
 // q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves (exact), or, with the
-// scales of the rows, their values rounded to bf16.
+// scales of the rows, their values rounded to bf16.  A wave takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it
+// turns in registers; the words meet in LDS (4 rows of a column a word) and leave as 16 bytes of 8 rows.  Bound by memory.
 __global__ __launch_bounds__(256) void k_transpose_i8(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld, bool whole,
                                                       const float *__restrict__ scale, __bf16 *__restrict__ out, int64_t rows_pad) {
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-    typedef int8_t c16 __attribute__((ext_vector_type(16)));
-    __shared__ int8_t t[64][72];                      // [column][row]
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    __shared__ unsigned t[64][66];                    // [column][4 rows], 256 rows
+    const int64_t r0 = (int64_t)blockIdx.x * 256;
     const int c0 = blockIdx.y * 64;
     {
-        const int i = threadIdx.x >> 2, j = (threadIdx.x & 3) * 16;
-        c16 v = {};
-        if (r0 + i < rows && c0 + j < cols) {
-            const int8_t *p = q + (r0 + i) * ld + c0 + j;
-            if (whole && (c0 + j + 16 <= cols || r0 + i + 1 < rows)) {      // the row's memory goes on to a multiple of 16 elements
-                v = *(const c16 *)p;
-            } else {
+        const int i = (threadIdx.x >> 2) * 4, j = (threadIdx.x & 3) * 16;
+        u4 v[4];
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    if (c0 + j + k < cols) v[k] = p[k];
+        for (int a = 0; a < 4; ++a) {
+            v[a] = u4{0, 0, 0, 0};
+            if (r0 + i + a < rows && c0 + j < cols) {
+                const int8_t *p = q + (r0 + i + a) * ld + c0 + j;
+                if (whole && (c0 + j + 16 <= cols || r0 + i + a + 1 < rows)) {      // the row's memory goes on to a multiple of 16
+                    v[a] = *(const u4 *)p;
+                } else {
+                    for (int k = 0; k < 16 && c0 + j + k < cols; ++k) v[a][k >> 2] |= (unsigned)(uint8_t)p[k] << (8 * (k & 3));
+                }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) t[j + k][i] = v[k];
+        for (int w = 0; w < 4; ++w) {                 // 4 rows x 4 columns of bytes
+            const unsigned lo01 = __builtin_amdgcn_perm(v[1][w], v[0][w], 0x05010400), hi01 = __builtin_amdgcn_perm(v[1][w], v[0][w], 0x07030602);
+            const unsigned lo23 = __builtin_amdgcn_perm(v[3][w], v[2][w], 0x05010400), hi23 = __builtin_amdgcn_perm(v[3][w], v[2][w], 0x07030602);
+            t[j + w * 4 + 0][i >> 2] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100);
+            t[j + w * 4 + 1][i >> 2] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302);
+            t[j + w * 4 + 2][i >> 2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100);
+            t[j + w * 4 + 3][i >> 2] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
+        }
     }
     __syncthreads();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int e = threadIdx.x + h * 256, j = e >> 3, i = (e & 7) * 8;
-        if (c0 + j >= cols) continue;
+    for (int h = 0; h < 8; ++h) {
+        const int e = threadIdx.x + h * 256, j = e >> 5, i = (e & 31) * 8;
+        if (c0 + j >= cols || r0 + i >= rows_pad) continue;
         b8 o;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            float v = (float)t[j][i + k];
+            float v = (float)(int8_t)(t[j][(i + k) >> 2] >> (8 * (k & 3)));
             if (scale) v = r0 + i + k < rows ? v * scale[r0 + i + k] : 0.f;
             o[k] = (__bf16)v;
         }
@@ -480,7 +490,7 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         if (rc) return rc;
     }
     if (gx) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.n_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qw, N, (int)K, ldqw, whole16(qw, ldqw, K), direct ? sw : nullptr, wt, p.n_pad);
+        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)((p.n_pad + 255) / 256), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qw, N, (int)K, ldqw, whole16(qw, ldqw, K), direct ? sw : nullptr, wt, p.n_pad);
         DPD_LAUNCH_CHECK();
         nt::Args a{};
         a.a = direct ? (const char *)g : (const char *)gs, a.lda = direct ? ldg * 2 : P * p.n_pad * 2;
@@ -490,7 +500,7 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         if (rc) return rc;
     }
     if (gw) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)(p.m_pad / 64), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qx, M, (int)K, ldqx, whole16(qx, ldqx, K), (const float *)nullptr, xt, p.m_pad);
+        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)((p.m_pad + 255) / 256), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qx, M, (int)K, ldqx, whole16(qx, ldqx, K), (const float *)nullptr, xt, p.m_pad);
         DPD_LAUNCH_CHECK();
         nt::Args a{};
         a.a = (const char *)gt, a.lda = P * p.m_pad * 2, a.b = (const char *)xt, a.ldb = p.m_pad * 2, a.M = (int)N, a.N = (int)K;

@@ -95,115 +95,119 @@ DEV double block_sum_d(double v, double *red) {       // over the 256 threads of
 }
 
 // ---- small matrices --------------------------------------------------------------------------
-constexpr int SMALL_R = 64, SMALL_C = 128, XS = SMALL_C + 1, AS = SMALL_R + 1;
+// One workgroup, one matrix, in fp32: r <= c after the transposition, X [r][c], A and B [r][r] in LDS, padded with zeros
+// to whole 16 x 16 blocks.  A wave forms a block with v_mfma_f32_16x16x4_f32 (32 cycles for 4 of the sum's terms: these, the
+// LDS reads in front of them and three barriers a step are the time): 16 terms from one 16-byte read of each factor, lane
+// q of a row taking terms 4 q .. 4 q + 3 of them, which for both factors is the same order.
+// Row strides are 4 modulo 64 words: 16 rows of 16 bytes touch every bank as often.
+constexpr int SMALL_R = 64, SMALL_C = 128, XS = SMALL_C + 4, AS = SMALL_R + 4;
+constexpr int SMALL_LDS = SMALL_R * XS + 2 * SMALL_R * AS;
 
-// One workgroup, one matrix: r <= c after the transposition, X [r][c], A and B [r][r] in LDS.  A thread forms 4 x 4
-// blocks of a product (8 LDS reads for 16 FMAs).
-template <class From, class To>
+DEV f32x4_t mfma_f32(float a, float b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+template <int WAVES>
+DEV double group_sum_d(double v, double *red) {       // over the workgroup, the same value in all threads
+    v = wave_sum_d(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) s += red[i];
+    return s;
+}
+
+template <int WAVES, class From, class To>
 DEV void small_iterate(const From &from, const To &to, int z, int rows, int cols, const Coef &coef, int steps, double eps, float *lds) {
-    __shared__ double red[4];
+    __shared__ double red[WAVES];
+    constexpr int THREADS = 64 * WAVES, MAX_BLOCKS = (SMALL_R / 16) * (SMALL_C / 16) / WAVES;      // of X, a wave
     float *X = lds, *A = X + SMALL_R * XS, *B = A + SMALL_R * AS;
     const bool wide = rows <= cols;
     const int r = wide ? rows : cols, c = wide ? cols : rows, n = rows * cols, t = threadIdx.x;
-    const int r4 = (r + 3) >> 2, c4 = (c + 3) >> 2;
-    for (int e = t; e < SMALL_R * XS + 2 * SMALL_R * AS; e += 256) lds[e] = 0.f;
+    const int rb = (r + 15) >> 4, cb = (c + 15) >> 4, lane = t & 63, wave = t >> 6, i16 = lane & 15, q = lane >> 4;
+    for (int e = t; e < SMALL_R * XS; e += THREADS) X[e] = 0.f;
     __syncthreads();
     double s = 0.0;
-    for (int e = t; e < n; e += 256) {
+    for (int e = t; e < n; e += THREADS) {
         const int i = e / cols, j = e - i * cols;
         const float v = from.first(z, e);
         X[wide ? i * XS + j : j * XS + i] = v;
         s += (double)v * (double)v;
     }
-    const double norm = sqrt(block_sum_d(s, red)), inv = 1.0 / (norm > eps ? norm : (norm == norm ? eps : norm));
-    for (int e = t; e < n; e += 256) {
-        const int i = e / cols, j = e - i * cols, at = wide ? i * XS + j : j * XS + i;
+    const double norm = sqrt(group_sum_d<WAVES>(s, red)), inv = 1.0 / (norm > eps ? norm : (norm == norm ? eps : norm));
+    for (int e = t; e < r * c; e += THREADS) {
+        const int i = e / c, at = i * XS + e - i * c;
         X[at] = (float)((double)X[at] * inv);
     }
     __syncthreads();
+    // sum over `blocks` groups of 16 terms of rows u (of U) and v (of V), both contiguous along the sum
+    auto dot = [&](const float *U, const float *V, int blocks, f32x4_t acc) {
+        for (int k = 0; k < blocks; ++k) {
+            const f32x4_t u = *(const f32x4_t *)(U + k * 16 + q * 4), v = *(const f32x4_t *)(V + k * 16 + q * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc = mfma_f32(u[e], v[e], acc);
+        }
+        return acc;
+    };
     for (int k = 0; k < steps; ++k) {
-        const float ca = coef.v[3 * k], cb = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
-        for (int e = t; e < r4 * r4; e += 256) {               // A = X X^T
-            const int i = (e / r4) * 4, j = (e % r4) * 4;
-            float acc[4][4] = {};
-            for (int q = 0; q < c; ++q) {
-                float u[4], v[4];
+        const float ca = coef.v[3 * k], cb3 = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
+        for (int b = wave; b < rb * rb; b += WAVES) {          // A = X X^T
+            const int bi = b / rb, bj = b - bi * rb;
+            const f32x4_t acc = dot(X + (bi * 16 + i16) * XS, X + (bj * 16 + i16) * XS, cb, f32x4_t{0, 0, 0, 0});
 #pragma unroll
-                for (int d = 0; d < 4; ++d) u[d] = X[(i + d) * XS + q], v[d] = X[(j + d) * XS + q];
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) acc[d][f] = __builtin_fmaf(u[d], v[f], acc[d][f]);
-            }
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) A[(i + d) * AS + j + f] = acc[d][f];
+            for (int e = 0; e < 4; ++e) A[(bi * 16 + q * 4 + e) * AS + bj * 16 + i16] = acc[e];
         }
         __syncthreads();
-        for (int e = t; e < r4 * r4; e += 256) {               // B = b A + c A A
-            const int i = (e / r4) * 4, j = (e % r4) * 4;
-            float acc[4][4] = {};
-            for (int q = 0; q < r; ++q) {
-                float u[4], v[4];
+        for (int b = wave; b < rb * rb; b += WAVES) {          // B = b A + c A A (the second factor by its rows: A is symmetric)
+            const int bi = b / rb, bj = b - bi * rb;
+            const f32x4_t acc = dot(A + (bi * 16 + i16) * AS, A + (bj * 16 + i16) * AS, rb, f32x4_t{0, 0, 0, 0});
 #pragma unroll
-                for (int d = 0; d < 4; ++d) u[d] = A[(i + d) * AS + q], v[d] = A[q * AS + j + d];
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) acc[d][f] = __builtin_fmaf(u[d], v[f], acc[d][f]);
-            }
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) B[(i + d) * AS + j + f] = __builtin_fmaf(cc, acc[d][f], cb * A[(i + d) * AS + j + f]);
-        }
-        __syncthreads();
-        float next[2][4][4];                                   // X <- a X + B X, written once every thread has read X
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = t + h * 256;
-            if (e >= r4 * c4) break;
-            const int i = (e / c4) * 4, j = (e % c4) * 4;
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) next[h][d][f] = ca * X[(i + d) * XS + j + f];
-            for (int q = 0; q < r; ++q) {
-                float u[4], v[4];
-#pragma unroll
-                for (int d = 0; d < 4; ++d) u[d] = B[(i + d) * AS + q], v[d] = X[q * XS + j + d];
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) next[h][d][f] = __builtin_fmaf(u[d], v[f], next[h][d][f]);
+            for (int e = 0; e < 4; ++e) {
+                const int at = (bi * 16 + q * 4 + e) * AS + bj * 16 + i16;
+                B[at] = __builtin_fmaf(cc, acc[e], cb3 * A[at]);
             }
         }
         __syncthreads();
+        f32x4_t next[MAX_BLOCKS];                              // X <- a X + B X, written once every wave has read X
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = t + h * 256;
-            if (e >= r4 * c4) break;
-            const int i = (e / c4) * 4, j = (e % c4) * 4;
+        for (int h = 0; h < MAX_BLOCKS; ++h) {
+            const int b = wave + h * WAVES;
+            if (b >= rb * cb) break;
+            const int bi = b / cb, bj = b - bi * cb;
+            f32x4_t acc;
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
+            for (int e = 0; e < 4; ++e) acc[e] = ca * X[(bi * 16 + q * 4 + e) * XS + bj * 16 + i16];
+            for (int m = 0; m < rb; ++m) {
+                const f32x4_t u = *(const f32x4_t *)(B + (bi * 16 + i16) * AS + m * 16 + q * 4);
 #pragma unroll
-                for (int f = 0; f < 4; ++f) X[(i + d) * XS + j + f] = next[h][d][f];
+                for (int e = 0; e < 4; ++e) acc = mfma_f32(u[e], X[(m * 16 + q * 4 + e) * XS + bj * 16 + i16], acc);
+            }
+            next[h] = acc;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < MAX_BLOCKS; ++h) {
+            const int b = wave + h * WAVES;
+            if (b >= rb * cb) break;
+            const int bi = b / cb, bj = b - bi * cb;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) X[(bi * 16 + q * 4 + e) * XS + bj * 16 + i16] = next[h][e];
         }
         __syncthreads();
     }
-    for (int e = t; e < n; e += 256) {
+    for (int e = t; e < n; e += THREADS) {
         const int i = e / cols, j = e - i * cols;
         to.put(z, e, X[wide ? i * XS + j : j * XS + i]);
     }
 }
 
-constexpr int SMALL_LDS = SMALL_R * XS + 2 * SMALL_R * AS;
+// Waves of a workgroup: 4 hold up to 32 x 32, 16 everything up to 64 x 128.
+inline bool needs_16_waves(int64_t rows, int64_t cols) { return rows > 32 || cols > 32; }
 
-template <class T>
-__global__ __launch_bounds__(256) void k_small(FromTensor<T> from, ToTensor<T> to, int rows, int cols, Coef coef, int steps, double eps) {
-    __shared__ float lds[SMALL_LDS];
-    small_iterate(from, to, blockIdx.x, rows, cols, coef, steps, eps, lds);
+template <int WAVES, class T>
+__global__ __launch_bounds__(64 * WAVES) void k_small(FromTensor<T> from, ToTensor<T> to, int rows, int cols, Coef coef, int steps, double eps) {
+    __shared__ __attribute__((aligned(16))) float lds[SMALL_LDS];
+    small_iterate<WAVES>(from, to, blockIdx.x, rows, cols, coef, steps, eps, lds);
 }
 
 constexpr int TABLE = 24;              // matrices of one launch: the table travels with the kernel's arguments
@@ -216,10 +220,10 @@ struct SmallTable {
 };
 
 template <class T>
-__global__ __launch_bounds__(256) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
-    __shared__ float lds[SMALL_LDS];
+__global__ __launch_bounds__(1024) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
+    __shared__ __attribute__((aligned(16))) float lds[SMALL_LDS];
     const int z = blockIdx.x;
-    small_iterate(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov, false}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
+    small_iterate<16>(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov, false}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
                   tab.cols[z], coef, steps, eps, lds);
 }
 
@@ -523,8 +527,12 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     if (is_small(rows, cols))
         return with_type(type, [&](auto t) {
             using T = decltype(t);
-            hipLaunchKernelGGL((k_small<T>), dim3((unsigned)batch), dim3(256), 0, st, FromTensor<T>{(const T *)x, rows * cols, false}, ToTensor<T>{(T *)out, rows * cols, false},
-                               (int)rows, (int)cols, coef, steps, eps);
+            const FromTensor<T> from{(const T *)x, rows * cols, false};
+            const ToTensor<T> to{(T *)out, rows * cols, false};
+            if (needs_16_waves(rows, cols))
+                hipLaunchKernelGGL((k_small<16, T>), dim3((unsigned)batch), dim3(1024), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
+            else
+                hipLaunchKernelGGL((k_small<4, T>), dim3((unsigned)batch), dim3(256), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
         });
@@ -573,7 +581,7 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
         SmallTable tab{};
         int used = 0;
         auto flush = [&]() {
-            if (used) hipLaunchKernelGGL((k_small_muon<T>), dim3(used), dim3(256), 0, st, tab, mu, nesterov, keep, coef, steps, eps);
+            if (used) hipLaunchKernelGGL((k_small_muon<T>), dim3(used), dim3(1024), 0, st, tab, mu, nesterov, keep, coef, steps, eps);
             used = 0;
             DPD_LAUNCH_CHECK();
             return DPD_OK;
