@@ -70,6 +70,7 @@ PROTOTYPES = {
     "dpd_int8_row_bytes": [c_l],
     "dpd_int8_linear_workspace_bytes": [c_l, c_l, c_l],
     "dpd_int8_linear": [c_p, c_i, c_l, c_l, c_l, c_p, c_p, c_p, c_i, c_l, c_p, c_l, c_p, c_sz, c_p],
+    "dpd_int8_linear_forward": [c_p, c_i, c_l, c_l, c_l, c_p, c_i, c_l, c_l, c_p, c_i, c_p, c_l, c_p, c_p, c_p, c_p, c_p],
     "dpd_int8_linear_backward_workspace_bytes": [c_l, c_l, c_l, c_i, c_i, c_i, c_i],
     "dpd_int8_linear_backward": [c_p, c_i, c_l, c_l, c_l, c_l, c_p, c_l, c_p, c_p, c_l, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_sz, c_p],
     "dpd_orthogonalize_workspace_bytes": [c_l, c_l, c_l, c_i],
@@ -157,6 +158,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 def raw_stream(index):
     """The current stream of a device as a plain integer (without the Python stream object where torch offers that)."""
     return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def entry(name):
+    """An entry point of the library for callers that invoke it often: check(entry(name)(...)) is call(name, ...)."""
+    handle = lib()
+    if not hasattr(handle, name):
+        raise RuntimeError(f"libdpd_hip.so does not export {name}: rebuild the library")
+    return getattr(handle, name)
 
 
 def stream():

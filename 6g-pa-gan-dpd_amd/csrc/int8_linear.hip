@@ -334,13 +334,12 @@ DEV void put_planes8(__bf16 *p, int64_t plane, const float *v) {
 // bf16 planes with zeros behind the rows, and this tile's column sums for gb.  Pieces of 8 elements on every access; bound
 // by memory (2 + 2 or 4 bytes an element in bf16).
 template <class T>
-__global__ __launch_bounds__(256) void k_grad_images(const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
-                                                     const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad,
-                                                     __bf16 *__restrict__ gt, int64_t m_pad, float *__restrict__ gb_part) {
+DEV void grad_images(int bx, int by, float (*t)[65], const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
+                     const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad, __bf16 *__restrict__ gt, int64_t m_pad,
+                     float *__restrict__ gb_part) {
     constexpr int P = planes_of<T>();
-    __shared__ float t[64][65];
-    const int64_t m0 = (int64_t)blockIdx.x * 64;
-    const int n0 = blockIdx.y * 64;
+    const int64_t m0 = (int64_t)bx * 64;
+    const int n0 = by * 64;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int e = threadIdx.x + h * 256, i = e >> 3, j = (e & 7) * 8;
@@ -368,7 +367,7 @@ __global__ __launch_bounds__(256) void k_grad_images(const T *__restrict__ g, in
     if (gb_part && threadIdx.x < 64 && n0 + threadIdx.x < N) {
         float s = 0.f;
         for (int i = 0; i < 64; ++i) s += t[i][threadIdx.x];
-        gb_part[(int64_t)blockIdx.x * N + n0 + threadIdx.x] = s;
+        gb_part[(int64_t)bx * N + n0 + threadIdx.x] = s;
     }
 }
 
@@ -391,13 +390,28 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ par
 // q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves (exact), or, with the
 // scales of the rows, their values rounded to bf16.  A wave takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it
 // turns in registers; the words meet in LDS (4 rows of a column a word) and leave as 16 bytes of 8 rows.  Bound by memory.
-__global__ __launch_bounds__(256) void k_transpose_i8(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld, bool whole,
-                                                      const float *__restrict__ scale, __bf16 *__restrict__ out, int64_t rows_pad) {
+struct Turn {
+    const int8_t *q;
+    int64_t rows, ld;
+    int cols;
+    bool whole;
+    const float *scale;
+    __bf16 *out;
+    int64_t rows_pad;
+    int bx, by;                                       // workgroups along the rows and the columns; none: 0
+};
+
+DEV void transpose_i8(int bx, int by, unsigned (*t)[66], const Turn &a) {
+    const int8_t *__restrict__ q = a.q;
+    const int64_t rows = a.rows, ld = a.ld, rows_pad = a.rows_pad;
+    const int cols = a.cols;
+    const bool whole = a.whole;
+    const float *__restrict__ scale = a.scale;
+    __bf16 *__restrict__ out = a.out;
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
     typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    __shared__ unsigned t[64][66];                    // [column][4 rows], 256 rows
-    const int64_t r0 = (int64_t)blockIdx.x * 256;
-    const int c0 = blockIdx.y * 64;
+    const int64_t r0 = (int64_t)bx * 256;             // t: [column][4 rows], 256 rows
+    const int c0 = by * 64;
     {
         const int i = (threadIdx.x >> 2) * 4, j = (threadIdx.x & 3) * 16;
         u4 v[4];
@@ -423,20 +437,44 @@ __global__ __launch_bounds__(256) void k_transpose_i8(const int8_t *__restrict__
             t[j + w * 4 + 3][i >> 2] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302);
         }
     }
+    const int i = (threadIdx.x & 31) * 8;             // this thread's rows
+    float f[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = r0 + i + k < rows ? (scale ? scale[r0 + i + k] : 1.f) : 0.f;
     __syncthreads();
+    if (r0 + i >= rows_pad) return;
 #pragma unroll
     for (int h = 0; h < 8; ++h) {
-        const int e = threadIdx.x + h * 256, j = e >> 5, i = (e & 31) * 8;
-        if (c0 + j >= cols || r0 + i >= rows_pad) continue;
+        const int j = (threadIdx.x >> 5) + h * 8;
+        if (c0 + j >= cols) return;
         b8 o;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float v = (float)(int8_t)(t[j][(i + k) >> 2] >> (8 * (k & 3)));
-            if (scale) v = r0 + i + k < rows ? v * scale[r0 + i + k] : 0.f;
-            o[k] = (__bf16)v;
-        }
+        for (int k = 0; k < 8; ++k) o[k] = (__bf16)((float)(int8_t)(t[j][(i + k) >> 2] >> (8 * (k & 3))) * f[k]);
         *(b8 *)(out + (int64_t)(c0 + j) * rows_pad + r0 + i) = o;
     }
+}
+
+// Everything that the two products of the backward read, in one launch: the images of g, and both 8-bit factors turned.
+template <class T>
+__global__ __launch_bounds__(256) void k_backward_images(const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
+                                                         const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad, __bf16 *__restrict__ gt,
+                                                         int64_t m_pad, float *__restrict__ gb_part, int gx, int gy, Turn w, Turn x) {
+    __shared__ union {
+        float f[64][65];
+        unsigned u[64][66];
+    } lds;
+    int id = blockIdx.x;
+    if (id < gx * gy) {
+        grad_images(id % gx, id / gx, lds.f, g, M, N, ldg, whole, sw, sx, gs, n_pad, gt, m_pad, gb_part);
+        return;
+    }
+    id -= gx * gy;
+    if (id < w.bx * w.by) {
+        transpose_i8(id % w.bx, id / w.bx, lds.u, w);
+        return;
+    }
+    id -= w.bx * w.by;
+    transpose_i8(id % x.bx, id / x.bx, lds.u, x);
 }
 
 int planes_for(int type) { return type == DPD_F32 ? 3 : type == DPD_BF16 ? 1 : 2; }
@@ -475,11 +513,18 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
     // one, rounded to bf16 there instead of in g times scale (one rounding of 2^-8 a term either way)
     const bool direct = P == 1 && ((uintptr_t)g & 15) == 0 && ldg % 8 == 0 && N % 8 == 0 && ldg * 2 <= nt::MAX_ROW_BYTES;
     if (direct) gs = nullptr;
-    if (gs || gt || part) {
-        hipLaunchKernelGGL((k_grad_images<T>), dim3((unsigned)(p.m_pad / 64), (unsigned)(p.n_pad / 64)), dim3(256), 0, st, g, M, (int)N, ldg,
-                           whole8(g, ldg), sw, sx, gs, p.n_pad, gt, p.m_pad, part);
-        DPD_LAUNCH_CHECK();
-    }
+    auto turn = [&](bool want, const int8_t *q, int64_t rows, int64_t ld, const float *scale, __bf16 *out, int64_t rows_pad) {
+        Turn a{q, rows, ld, (int)K, whole16(q, ld, K), scale, out, rows_pad, 0, 0};
+        if (want) a.bx = (int)((rows_pad + 255) / 256), a.by = (int)((K + 63) / 64);
+        return a;
+    };
+    const Turn tw = turn(gx, qw, N, ldqw, direct ? sw : nullptr, wt, p.n_pad), tx = turn(gw, qx, M, ldqx, nullptr, xt, p.m_pad);
+    const int bx = gs || gt || part ? (int)(p.m_pad / 64) : 0, by = (int)(p.n_pad / 64);
+    const int64_t blocks = (int64_t)bx * by + (int64_t)tw.bx * tw.by + (int64_t)tx.bx * tx.by;
+    DPD_REQUIRE(blocks <= INT32_MAX, DPD_ERR_SHAPE, "int8_linear_backward: %lld x %lld gradients are too many for one call", (long long)M, (long long)N);
+    hipLaunchKernelGGL((k_backward_images<T>), dim3((unsigned)blocks), dim3(256), 0, st, g, M, (int)N, ldg, whole8(g, ldg), sw, sx, gs, p.n_pad, gt,
+                       p.m_pad, part, bx, by, tw, tx);
+    DPD_LAUNCH_CHECK();
     if (gb) {
         const int rc = with_type(gb_type, [&](auto t) {
             using B = decltype(t);
@@ -490,8 +535,6 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         if (rc) return rc;
     }
     if (gx) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)((p.n_pad + 255) / 256), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qw, N, (int)K, ldqw, whole16(qw, ldqw, K), direct ? sw : nullptr, wt, p.n_pad);
-        DPD_LAUNCH_CHECK();
         nt::Args a{};
         a.a = direct ? (const char *)g : (const char *)gs, a.lda = direct ? ldg * 2 : P * p.n_pad * 2;
         a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
@@ -500,8 +543,6 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
         if (rc) return rc;
     }
     if (gw) {
-        hipLaunchKernelGGL(k_transpose_i8, dim3((unsigned)((p.m_pad + 255) / 256), (unsigned)((K + 63) / 64)), dim3(256), 0, st, qx, M, (int)K, ldqx, whole16(qx, ldqx, K), (const float *)nullptr, xt, p.m_pad);
-        DPD_LAUNCH_CHECK();
         nt::Args a{};
         a.a = (const char *)gt, a.lda = P * p.m_pad * 2, a.b = (const char *)xt, a.ldb = p.m_pad * 2, a.M = (int)N, a.N = (int)K;
         a.wrap = (int)(p.m_pad / 64), a.steps = P * a.wrap, a.tail = 128;
@@ -633,6 +674,32 @@ extern "C" int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, in
         if (M <= 32) return tall ? few_tokens<T, 16, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
         if (M <= 64) return tall ? few_tokens<T, 16, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
         return int8_product(qx, ld, sx, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
+    });
+}
+
+extern "C" int dpd_int8_linear_forward(const void *x, int type, int64_t M, int64_t K, int64_t ldx, const void *w, int w_type, int64_t N, int64_t ldw,
+                                       const void *bias, int bias_type, void *out, int64_t ldo, int8_t *qx, float *x_scale, int8_t *qw, float *w_scale,
+                                       void *stream) {
+    DPD_REQUIRE(is_type(type) && is_type(w_type) && (!bias || is_type(bias_type)), DPD_ERR_INVALID_ARG, "int8_linear_forward: element type");
+    if (const int rc = check_sizes("int8_linear_forward", M, N, K)) return rc;
+    DPD_REQUIRE((M == 0 || (x && qx && x_scale)) && (N == 0 || (w && qw && w_scale)) && (M == 0 || N == 0 || out), DPD_ERR_INVALID_ARG,
+                "int8_linear_forward: null pointer");
+    DPD_REQUIRE(ldx >= K && ldw >= K && ldo >= N, DPD_ERR_INVALID_ARG, "int8_linear_forward: row stride");
+    DPD_REQUIRE((((uintptr_t)qx | (uintptr_t)qw) & 15) == 0, DPD_ERR_INVALID_ARG, "int8_linear_forward: the images are 16-byte aligned");
+    const int64_t ld = nt::pad_to(K, 128);
+    hipStream_t st = as_stream(stream);
+    auto quantize = [&](const void *p, int t, int64_t rows, int64_t stride, int8_t *q, float *scale) {
+        return rows == 0 ? DPD_OK : with_type(t, [&](auto e) {
+            using T = decltype(e);
+            return quantize_rows((const T *)p, rows, (int)K, stride, q, ld, scale, st);
+        });
+    };
+    int rc = quantize(x, type, M, ldx, qx, x_scale);
+    if (!rc) rc = quantize(w, w_type, N, ldw, qw, w_scale);
+    if (rc || M == 0 || N == 0) return rc;
+    return with_type(type, [&](auto e) {
+        using T = decltype(e);
+        return int8_product(qx, ld, x_scale, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
     });
 }
 

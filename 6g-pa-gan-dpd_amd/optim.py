@@ -7,6 +7,8 @@ import torch
 from . import _lib as L
 from .utils.orthogonal import COEFFICIENTS, Coefficients, coefficient_table, wants_accurate
 
+# autograd sees that the weights changed (the public form of the same call walks its argument as a tree first)
+_bump_versions = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
 _PTR, _I64 = ctypes.c_void_p, ctypes.c_int64
 
 
@@ -74,31 +76,40 @@ class Muon(torch.optim.Optimizer):
 
     def _matrices(self, group):
         sets: Dict = {}
+        types, state = L.TYPES, self.state
         for p in group["params"]:
             g = p.grad
             if g is None:
                 continue
             if p.dim() != 2 or g.is_sparse:
                 raise ValueError(f"a weight matrix with a dense gradient is expected, got {tuple(p.shape)}, sparse = {g.is_sparse}")
+            dtype, device = p.dtype, p.device
             L.need_gpu(p, g)
-            if p.dtype not in L.TYPES or g.dtype != p.dtype or not p.is_contiguous():
-                raise RuntimeError(f"weights must be contiguous float32, bfloat16 or float16 with gradients of their type, got {p.dtype} / {g.dtype}")
-            state = self.state[p]
-            m = state.get("momentum_buffer")
+            if dtype not in types or g.dtype != dtype or not p.is_contiguous():
+                raise RuntimeError(f"weights must be contiguous float32, bfloat16 or float16 with gradients of their type, got {dtype} / {g.dtype}")
+            own = state[p]
+            m = own.get("momentum_buffer")
             if m is None:
-                m = state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
-            elif m.dtype != torch.float32 or m.shape != p.shape or not m.is_contiguous() or m.device != p.device:
-                raise RuntimeError(f"the momentum of a weight must be a contiguous float32 tensor of its shape on {p.device}, got {m.dtype} {tuple(m.shape)}")
-            sets.setdefault((p.dtype, p.device), []).append((p, g.contiguous(), m))
-        for (dtype, _), items in sets.items():
-            n = len(items)
-            ptrs = [(_PTR * n)(*(t[i].data_ptr() for t in items)) for i in range(3)]
-            rows, cols = (_I64 * n)(*(t[0].shape[0] for t in items)), (_I64 * n)(*(t[0].shape[1] for t in items))
+                m = own["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+            elif m.dtype != torch.float32 or m.shape != p.shape or not m.is_contiguous() or m.device != device:
+                raise RuntimeError(f"the momentum of a weight must be a contiguous float32 tensor of its shape on {device}, got {m.dtype} {tuple(m.shape)}")
+            items = sets.get((dtype, device))
+            if items is None:
+                items = sets[(dtype, device)] = ([], [], [])
+            for column, t in zip(items, (p, g if g.is_contiguous() else g.contiguous(), m)):
+                column.append(t)
+        for (dtype, device), items in sets.items():
+            n = len(items[0])
+            pointers, sizes = _PTR * n, _I64 * n
+            shapes = [p.shape for p in items[0]]
+            rows, cols = sizes(*[s[0] for s in shapes]), sizes(*[s[1] for s in shapes])
             acc, steps = wants_accurate(group["accurate"], dtype), int(group["steps"])
             coef = coefficient_table(group["coefficients"], steps)
             with L.device(items[0][0]):
-                nbytes = L.lib().dpd_muon_workspace_bytes(n, rows, cols, acc)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=items[0][0].device)
-                L.call("dpd_muon_step", n, *ptrs, rows, cols, L.TYPES[dtype], float(group["lr"]), float(group["momentum"]), int(group["nesterov"]),
-                       float(group["weight_decay"]), steps, coef, float(group["eps"]), acc, L.c_p(ws.data_ptr()), nbytes, L.stream())
-            torch.autograd.graph.increment_version([t[0] for t in items])
+                nbytes = L.entry("dpd_muon_workspace_bytes")(n, rows, cols, acc)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                L.check(L.entry("dpd_muon_step")(
+                    n, *[pointers(*[t.data_ptr() for t in column]) for column in items], rows, cols, types[dtype], float(group["lr"]),
+                    float(group["momentum"]), int(group["nesterov"]), float(group["weight_decay"]), steps, coef, float(group["eps"]), acc,
+                    ws.data_ptr(), nbytes, L.raw_stream(device.index)))
+            _bump_versions(items[0])

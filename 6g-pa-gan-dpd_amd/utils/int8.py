@@ -102,6 +102,11 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
         return _matmul(a2, lda, sa, b2, ldb, sb, bc, bt, m, n, k, out_dtype).view(*a.shape[:-1], n)
 
 
+def _addresses(kept, m, n, ld):
+    base = kept.data_ptr()
+    return base, base + m * ld, base + (m + n) * ld, base + (m + n) * ld + 4 * m
+
+
 class _Int8LinearFn(torch.autograd.Function):
     """Both factors quantised on the way; the backward reads the 8-bit factors, so x and the weight are not kept."""
 
@@ -110,37 +115,42 @@ class _Int8LinearFn(torch.autograd.Function):
         x2, ldx = _rows(x)
         w2, ldw = _rows(weight)
         (m, k), n = x2.shape, w2.shape[0]
-        ld = _row_bytes(k)
+        ld, dev = _row_bytes(k), x.device
+        bc, bt = _check_bias(bias, n, dev)
+        out = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=dev)
+        # one buffer for what the backward reads: qx [m, ld], qw [n, ld], the scales of x, the scales of the weight
+        kept = torch.empty((m + n) * (ld + 4), dtype=torch.int8, device=dev)
+        at = _addresses(kept, m, n, ld)
         with L.device(x):
-            qx, sx = _quantize(x2, ldx, ld)
-            qw, sw = _quantize(w2, ldw, ld)
-            bc, bt = _check_bias(bias, n, x.device)
-            out = _matmul(qx, ld, sx, qw, ld, sw, bc, bt, m, n, ld, x.dtype)      # both images carry zeros behind the rows
-        ctx.save_for_backward(qx, sx, qw, sw)
+            L.check(L.entry("dpd_int8_linear_forward")(
+                x2.data_ptr(), TYPES[x.dtype], m, k, ldx, w2.data_ptr(), TYPES[weight.dtype], n, ldw, 0 if bc is None else bc.data_ptr(), bt,
+                out.data_ptr(), n, at[0], at[2], at[1], at[3], L.raw_stream(dev.index)))
+        ctx.save_for_backward(kept)
         ctx.sizes, ctx.lead, ctx.types = (m, n, k, ld), x.shape[:-1], (x.dtype, weight.dtype, bias.dtype if bias is not None else None)
-        return out.view(*x.shape[:-1], n)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gy):
-        qx, sx, qw, sw = ctx.saved_tensors
+        kept, = ctx.saved_tensors
         m, n, k, ld = ctx.sizes
         tx, tw, tb = ctx.types
         need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         need_b = tb is not None and ctx.needs_input_grad[2]
-        dev = qx.device
+        dev = kept.device
         g2, ldg = _rows(gy)
-        gx = torch.empty(m, k, dtype=tx, device=dev) if need_x else None
+        gx = torch.empty((*ctx.lead, k), dtype=tx, device=dev) if need_x else None
         gw = torch.empty(n, k, dtype=tw, device=dev) if need_w else None
         gb = torch.empty(n, dtype=tb, device=dev) if need_b else None
-        ptr = lambda t: L.c_p(t.data_ptr() if t is not None else 0)
-        t = TYPES[tx]
-        with L.device(qx):
-            nbytes = L.lib().dpd_int8_linear_backward_workspace_bytes(m, n, k, t, need_x, need_w, need_b)
+        ptr = lambda t: t.data_ptr() if t is not None else 0
+        t, (qx, qw, sx, sw) = TYPES[tx], _addresses(kept, m, n, ld)
+        with L.device(kept):
+            nbytes = L.entry("dpd_int8_linear_backward_workspace_bytes")(m, n, k, t, need_x, need_w, need_b)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            L.call("dpd_int8_linear_backward", ptr(g2), t, m, n, k, ldg, ptr(qx), ld, ptr(sx), ptr(qw), ld, ptr(sw), ptr(gx), ptr(gw), TYPES[tw],
-                   ptr(gb), TYPES[tb] if need_b else 0, ptr(ws), nbytes, L.stream())
-        return gx.view(*ctx.lead, k) if need_x else None, gw, gb
+            L.check(L.entry("dpd_int8_linear_backward")(
+                g2.data_ptr(), t, m, n, k, ldg, qx, ld, sx, qw, ld, sw, ptr(gx), ptr(gw), TYPES[tw], ptr(gb), TYPES[tb] if need_b else 0,
+                ws.data_ptr(), nbytes, L.raw_stream(dev.index)))
+        return gx, gw, gb
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -15,7 +15,10 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)      # steep at zero: singular values e
 
 @lru_cache(maxsize=64)
 def _table(coefficients, steps: int):
-    flat = [float(v) for c in coefficients for v in c] if isinstance(coefficients[0], tuple) else [float(v) for v in coefficients] * steps
+    rows = coefficients if coefficients and isinstance(coefficients[0], tuple) else (coefficients,) * steps
+    if len(rows) != steps or any(not isinstance(r, tuple) or len(r) != 3 for r in rows):
+        raise ValueError(f"coefficients must be one triple (a, b, c) or one for each of {steps} steps")
+    flat = [float(v) for r in rows for v in r]
     return (ctypes.c_float * len(flat))(*flat)
 
 
@@ -23,11 +26,9 @@ def coefficient_table(coefficients: Coefficients, steps: int):
     """steps triples as a host array; one triple serves every step."""
     if not 1 <= int(steps) <= 32:
         raise ValueError(f"steps must be 1 to 32, got {steps}")
-    c = tuple(tuple(v) if isinstance(v, (tuple, list)) else v for v in coefficients)
-    rows = c if c and isinstance(c[0], tuple) else (c,) * int(steps)
-    if len(rows) != int(steps) or any(not isinstance(r, tuple) or len(r) != 3 for r in rows):
-        raise ValueError(f"coefficients must be one triple (a, b, c) or one for each of {steps} steps")
-    return _table(c, int(steps))
+    if type(coefficients) is not tuple or (coefficients and type(coefficients[0]) is list):
+        coefficients = tuple(tuple(v) if isinstance(v, (tuple, list)) else v for v in coefficients)
+    return _table(coefficients, int(steps))
 
 
 def wants_accurate(accurate: Optional[bool], dtype: torch.dtype) -> int:
@@ -60,8 +61,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
     out = torch.empty_like(xc)
     acc = wants_accurate(accurate, x.dtype)
     with L.device(x):
-        nbytes = L.lib().dpd_orthogonalize_workspace_bytes(batch, rows, cols, acc)
+        nbytes = L.entry("dpd_orthogonalize_workspace_bytes")(batch, rows, cols, acc)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        L.call("dpd_orthogonalize", L.c_p(xc.data_ptr()), L.TYPES[x.dtype], batch, rows, cols, int(steps), coef, float(eps), acc,
-               L.c_p(out.data_ptr()), L.c_p(ws.data_ptr()), nbytes, L.stream())
+        L.check(L.entry("dpd_orthogonalize")(xc.data_ptr(), L.TYPES[x.dtype], batch, rows, cols, int(steps), coef, float(eps), acc, out.data_ptr(),
+                                             ws.data_ptr(), nbytes, L.raw_stream(x.device.index)))
     return out

@@ -388,6 +388,13 @@ size_t dpd_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, int64_t ldx, const int8_t *qw, const float *w_scale,
                     const void *bias, int bias_type, int64_t N, void *out, int64_t ldo, void *ws, size_t ws_bytes, void *stream);
 
+/* The same with a floating-point weight w [N, K] that is quantised in this call, for training: qx [M, row bytes], x_scale
+ * [M], qw [N, row bytes] (16-byte aligned, row bytes = dpd_int8_row_bytes(K)) and w_scale [N] are outputs, what the backward
+ * reads. */
+int dpd_int8_linear_forward(const void *x, int type, int64_t M, int64_t K, int64_t ldx, const void *w, int w_type, int64_t N,
+                            int64_t ldw, const void *bias, int bias_type, void *out, int64_t ldo, int8_t *qx, float *x_scale,
+                            int8_t *qw, float *w_scale, void *stream);
+
 /* Its straight-through gradients (the quantisers count as the identity): gx [M, K] = g (qw w_scale) in the type of g,
  * gw [N, K] = g^T (qx x_scale), gb [N] = column sums of g; each may be NULL.  Products on the bf16 matrix cores: the
  * 8-bit factor is exact there, g times a scale is rounded to bf16 once (type bf16), held in two bf16 terms (fp16) or in
