@@ -407,39 +407,61 @@ static int launch(Args g, int batch, const Epilogue &epi, hipStream_t st) {
     return DPD_OK;
 }
 
-// Which tile: the one whose rounds over the 256 compute units (one workgroup each) are estimated to take least.  Measured
-// with fp16 operands and a full round (1024 to 4096 rows, us): steps * per_step + fixed; the split form takes 1.45 times as
-// long a step, and needs an even number of block rows a wave.
-struct TileCost {
-    int bm, bn;
-    float per_step, fixed;
-    bool split;
+// Which tile: the one whose rounds over the 256 compute units are estimated to take least.  A round has one workgroup on
+// every compute unit, or two where 80 KB of LDS hold one; it takes steps * per + fixed.  Measured with full rounds of 1024 to
+// 4096 rows, fp16 operands (int8 and bf16 take the same time a step) and the split form, us.
+struct Round {
+    float per, fixed;
 };
-constexpr TileCost TILES[] = {{256, 256, 1.35f, 10.f, true}, {256, 128, 0.88f, 6.5f, true}, {192, 192, 0.92f, 7.f, true}, {128, 128, 0.49f, 4.3f, true},
-                              {128, 64, 0.33f, 4.f, true},   {96, 96, 0.29f, 4.f, false},   {64, 64, 0.19f, 3.1f, true}};
+struct Tile {
+    int bm, bn;
+    Round one, two;              // one and two workgroups on a compute unit (per == 0: does not fit)
+    Round split_one, split_two;
+};
+constexpr Tile TILES[] = {
+    {256, 256, {1.35f, 10.f}, {}, {2.2f, 7.f}, {}},
+    {256, 128, {0.885f, 6.4f}, {}, {1.28f, 4.8f}, {}},
+    {192, 192, {0.94f, 7.f}, {}, {1.28f, 8.f}, {}},
+    {128, 128, {0.48f, 4.4f}, {}, {0.615f, 6.1f}, {}},
+    {128, 128, {0.685f, 1.2f}, {0.904f, 5.6f}, {0.7f, 4.f}, {1.33f, 2.2f}},
+    {128, 64, {0.32f, 3.1f}, {0.565f, 3.8f}, {0.4175f, 2.8f}, {0.7075f, 4.1f}},
+    {96, 96, {0.29f, 4.f}, {}, {}, {}},                                       // an odd number of block rows a wave: not split
+    {64, 64, {0.19f, 3.1f}, {}, {0.2475f, 2.9f}, {}},
+    {64, 64, {0.208f, 2.9f}, {0.377f, 2.6f}, {0.35f, 0.5f}, {0.39f, 3.8f}},
+};
+
+static inline int best_tile(const Args &g, int batch, bool split) {
+    int best = -1;
+    float least = 0.f;
+    for (int i = 0; i < (int)(sizeof(TILES) / sizeof(TILES[0])); ++i) {
+        const Tile &t = TILES[i];
+        const Round one = split ? t.split_one : t.one, two = split ? t.split_two : t.two;
+        if ((g.lower && t.bm != t.bn) || one.per == 0.f) continue;
+        Args a = g;
+        a.tiles_m = (g.M + t.bm - 1) / t.bm, a.tiles_n = (g.N + t.bn - 1) / t.bn;
+        const int64_t tiles = (int64_t)tiles_of(a) * batch, size = two.per > 0.f ? 512 : 256, rest = tiles % size;
+        const float c1 = (float)g.steps * one.per + one.fixed, c2 = (float)g.steps * two.per + two.fixed;
+        const float cost = (float)(tiles / size) * (size == 512 ? c2 : c1) + (rest == 0 ? 0.f : rest > 256 ? c2 : c1);
+        if (best < 0 || cost < least) best = i, least = cost;
+    }
+    return best;
+}
 
 template <int KIND, class Epilogue>
 static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st) {
-    int best = -1;
-    float least = 0.f;
-    for (int i = 0; i < 7; ++i) {
-        const TileCost &t = TILES[i];
-        if ((g.lower && t.bm != t.bn) || (KIND == F16_SPLIT && !t.split)) continue;
-        Args a = g;
-        a.tiles_m = (g.M + t.bm - 1) / t.bm, a.tiles_n = (g.N + t.bn - 1) / t.bn;
-        const int64_t rounds = ((int64_t)tiles_of(a) * batch + 255) / 256;
-        const float cost = (float)rounds * ((float)g.steps * (KIND == F16_SPLIT ? 1.45f : 1.f) * t.per_step + t.fixed);
-        if (best < 0 || cost < least) best = i, least = cost;
-    }
-    switch (best) {
+    constexpr bool SPLIT = KIND == F16_SPLIT;
+    switch (best_tile(g, batch, SPLIT)) {
     case 0: return launch<KIND, 256, 256, 2, 4, 1, 2>(g, batch, epi, st);
     case 1: return launch<KIND, 256, 128, 4, 2, 1, 3>(g, batch, epi, st);
     case 2: return launch<KIND, 192, 192, 2, 2, 1, 3>(g, batch, epi, st);
-    case 3: return launch<KIND, 128, 128, 2, 4, 1, 4>(g, batch, epi, st);
-    case 4: return launch<KIND, 128, 64, 4, 2, 1, 6>(g, batch, epi, st);
-    case 5:
-        if constexpr (KIND != F16_SPLIT) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
-    default: return launch<KIND, 64, 64, 2, 2, 2, 4>(g, batch, epi, st);
+    case 3: return launch<KIND, 128, 128, 2, SPLIT ? 2 : 4, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
+    case 4: return launch<KIND, 128, 128, 2, 4, 1, 2>(g, batch, epi, st);
+    case 5: return launch<KIND, 128, 64, 2, 2, 1, 3>(g, batch, epi, st);
+    case 6:
+        if constexpr (!SPLIT) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
+        [[fallthrough]];
+    case 7: return launch<KIND, 64, 64, 2, 2, 2, 4>(g, batch, epi, st);
+    default: return launch<KIND, 64, 64, 2, 2, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
     }
 }
 
