@@ -335,27 +335,45 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
 #pragma unroll
     for (int j = 0; j < TN / 2; ++j) col[j] = epi.col(blockIdx.z, n0 + wn * TN * 16 + j * 32 + q * 8);
     const bool turn = Epilogue::TURNED && !(g.lower && tm == tn);
+    constexpr int AHEAD = SPLIT ? 2 : TM % 4 == 0 ? 4 : TM;    // block rows whose inputs are read together, in front of their use
+    static_assert(TM % AHEAD == 0, "whole groups of block rows");
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-        const int m = m0 + (wm * TM + i) * 16 + r;
-        typename Epilogue::Row row;
-        if (m < g.M) row = epi.row(blockIdx.z, m);
+    for (int i0 = 0; i0 < TM; i0 += AHEAD) {
+        typename Epilogue::Row row[AHEAD];
+        typename Epilogue::Pre pre[AHEAD][TN / 2];
+        if (WAVES_K == 1 || group == 0) {
 #pragma unroll
-        for (int j = 0; j < TN / 2; ++j) {
-            const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
-            float v[8];
+            for (int k = 0; k < AHEAD; ++k) {
+                const int m = m0 + (wm * TM + i0 + k) * 16 + r;
+                if (m >= g.M) continue;
+                row[k] = epi.row(blockIdx.z, m);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][2 * j][e], v[4 + e] = (float)acc[i][2 * j + 1][e];
-            if (WAVES_K > 1 && group > 0) continue;
-            if (m < g.M && n < g.N) {
-                epi.put(blockIdx.z, m, n, v, row, col[j]);
-            } else if (Epilogue::TURNED) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.f;    // zeros behind the rows of the turned tile
+                for (int j = 0; j < TN / 2; ++j) {
+                    const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
+                    if (n < g.N) pre[k][j] = epi.pre(blockIdx.z, m, n);
+                }
             }
-            if constexpr (Epilogue::TURNED) {
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][2 * j][e] = v[e], acc[i][2 * j + 1][e] = v[4 + e];
+        for (int k = 0; k < AHEAD; ++k) {
+            const int i = i0 + k, m = m0 + (wm * TM + i) * 16 + r;
+#pragma unroll
+            for (int j = 0; j < TN / 2; ++j) {
+                const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][2 * j][e], v[4 + e] = (float)acc[i][2 * j + 1][e];
+                if (WAVES_K > 1 && group > 0) continue;
+                if (m < g.M && n < g.N) {
+                    epi.put(blockIdx.z, m, n, v, row[k], col[j], pre[k][j]);
+                } else if (Epilogue::TURNED) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = 0.f;    // zeros behind the rows of the turned tile
+                }
+                if constexpr (Epilogue::TURNED) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][2 * j][e] = v[e], acc[i][2 * j + 1][e] = v[4 + e];
+                }
             }
         }
     }
@@ -378,14 +396,14 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
                         if (WAVES_K > 1 && group > 0) break;
                         const int ml = (wm * TM + i) * 16 + r, nl = wn * TN * 16 + (j >> 1) * 32 + q * 8 + (j & 1) * 4 + e;
                         const _Float16 h = (_Float16)acc[i][j][e];
-                        t[nl * BM + (((ml >> 3) ^ ((nl >> 3) & MASK)) << 3) + (ml & 7)] = h;
+                        t[nl * BM + (((ml >> 3) ^ ((nl >> 2) & MASK)) << 3) + (ml & 7)] = h;
                         if (SPLIT) acc[i][j][e] -= (float)h;
                     }
             __syncthreads();
             for (int k = threadIdx.x; k < BN * CHUNKS; k += 64 * WAVES * WAVES_K) {
                 const int nl = k / CHUNKS, c = k - nl * CHUNKS;
                 if (n0 + nl < g.N && m0 + c * 8 < g.M)
-                    epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * BM + ((c ^ ((nl >> 3) & MASK)) << 3)));
+                    epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * BM + ((c ^ ((nl >> 2) & MASK)) << 3)));
             }
         }
     }

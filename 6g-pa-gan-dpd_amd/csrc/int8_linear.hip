@@ -115,6 +115,8 @@ struct ScaleOut {
     bool whole;
     static constexpr bool TURNED = false;
     typedef float Row;
+    typedef None Pre;
+    DEV Pre pre(int, int, int) const { return {}; }
     struct Col {
         float s[8], b[8];
     };
@@ -129,7 +131,7 @@ struct ScaleOut {
         }
         return c;
     }
-    DEV void put(int, int m, int n, float *v, const Row &r, const Col &c) const {
+    DEV void put(int, int m, int n, float *v, const Row &r, const Col &c, Pre) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = v[i] * r * c.s[i] + c.b[i];
         store8(out + (int64_t)m * ldo + n, v, N - n, whole);
@@ -143,10 +145,11 @@ struct PlainOut {
     int N;
     bool whole;
     static constexpr bool TURNED = false;
-    typedef None Row, Col;
+    typedef None Row, Col, Pre;
+    DEV Pre pre(int, int, int) const { return {}; }
     DEV Row row(int, int) const { return {}; }
     DEV Col col(int, int) const { return {}; }
-    DEV void put(int, int m, int n, float *v, Row, Col) const { store8(out + (int64_t)m * ldo + n, v, N - n, whole); }
+    DEV void put(int, int m, int n, float *v, Row, Col, Pre) const { store8(out + (int64_t)m * ldo + n, v, N - n, whole); }
 };
 
 // Few tokens: a workgroup owns 16 output channels and reads their weights once, straight into the fragments of the

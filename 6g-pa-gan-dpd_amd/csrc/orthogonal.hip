@@ -27,6 +27,8 @@ struct FromTensor {                                   // a matrix of a batch
     const T *x;
     int64_t batch;
     bool whole;                                       // matrices and rows of whole 16-byte pieces
+    bool is_wide;
+    DEV bool wide(int) const { return is_wide; }
     DEV void first8(int z, int64_t i, float *v, int valid) const { load8(x + z * batch + i, v, valid, whole); }
     DEV void again8(int z, int64_t i, float *v, int valid) const { load8(x + z * batch + i, v, valid, whole); }
     DEV float first(int z, int64_t i) const { return to_f32(x[z * batch + i]); }
@@ -38,30 +40,41 @@ struct FromMomentum {                                 // g and the momentum, whi
     float *m;
     float mu;
     int nesterov;
-    bool whole;
-    DEV void first8(int, int64_t i, float *v, int valid) const {
+    DEV float first(int, int64_t i) const {
+        const float w = mu * m[i] + to_f32(g[i]);
+        m[i] = w;
+        return nesterov ? to_f32(g[i]) + mu * w : w;
+    }
+};
+constexpr int TOGETHER = 8;                           // large matrices of one size that go through the products together
+template <class T>
+struct FromMomenta {                                  // the same for several matrices, with pieces of 8
+    const T *g[TOGETHER];
+    float *m[TOGETHER];
+    float mu;
+    int nesterov;
+    unsigned whole_bits, wide_bits;
+    DEV bool wide(int z) const { return wide_bits >> z & 1; }
+    DEV void first8(int z, int64_t i, float *v, int valid) const {
+        const bool whole = whole_bits >> z & 1;
         float w[8];
-        load8(m + i, w, valid, whole);
-        load8(g + i, v, valid, whole);
+        load8((const float *)m[z] + i, w, valid, whole);
+        load8(g[z] + i, v, valid, whole);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             w[k] = mu * w[k] + v[k];
             v[k] = nesterov ? v[k] + mu * w[k] : w[k];
         }
-        store8(m + i, w, valid, whole);
+        store8(m[z] + i, w, valid, whole);
     }
-    DEV void again8(int, int64_t i, float *v, int valid) const {
+    DEV void again8(int z, int64_t i, float *v, int valid) const {
+        const bool whole = whole_bits >> z & 1;
         float w[8];
-        load8((const float *)m + i, w, valid, whole);
-        if (nesterov) load8(g + i, v, valid, whole);
+        load8((const float *)m[z] + i, w, valid, whole);
+        if (nesterov) load8(g[z] + i, v, valid, whole);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = nesterov ? v[k] + mu * w[k] : w[k];
     }
-    DEV float first(int, int64_t i) const {
-        m[i] = mu * m[i] + to_f32(g[i]);
-        return again(0, i);
-    }
-    DEV float again(int, int64_t i) const { return nesterov ? to_f32(g[i]) + mu * m[i] : m[i]; }
 };
 template <class T>
 struct ToTensor {
@@ -75,14 +88,20 @@ template <class T>
 struct ToWeights {
     T *p;
     float keep, factor;                               // 1 - lr wd, lr sqrt(max(1, rows / cols))
-    bool whole;
     DEV void put(int, int64_t i, float v) const { p[i] = from_f32<T>(to_f32(p[i]) * keep - factor * v); }
-    DEV void put8(int, int64_t i, float *v, int valid) const {
+};
+template <class T>
+struct ToManyWeights {
+    T *p[TOGETHER];
+    float keep, factor;
+    unsigned whole_bits;
+    DEV void put8(int z, int64_t i, float *v, int valid) const {
+        const bool whole = whole_bits >> z & 1;
         float w[8];
-        load8(p + i, w, valid, whole);
+        load8((const T *)p[z] + i, w, valid, whole);
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = w[k] * keep - factor * v[k];
-        store8(p + i, v, valid, whole);
+        store8(p[z] + i, v, valid, whole);
     }
 };
 
@@ -223,7 +242,7 @@ template <class T>
 __global__ __launch_bounds__(1024) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
     __shared__ __attribute__((aligned(16))) float lds[SMALL_LDS];
     const int z = blockIdx.x;
-    small_iterate<16>(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov, false}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z], false}, 0, tab.rows[z],
+    small_iterate<16>(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z]}, 0, tab.rows[z],
                   tab.cols[z], coef, steps, eps, lds);
 }
 
@@ -238,16 +257,17 @@ template <bool SPLIT>
 DEV int64_t img_col(int col) { return SPLIT ? (int64_t)(col >> 5) * 128 + (col & 31) * 2 : (int64_t)col * 2; }
 
 template <bool SPLIT>
-DEV void img_load8(const Image &im, int z, int64_t row, int col, float *v) {
+struct Eight {                         // eight values of an image as they lie there
+    nt::f16x8 h[SPLIT ? 2 : 1];
+    DEV float operator[](int i) const { return SPLIT ? (float)h[0][i] + (float)h[SPLIT ? 1 : 0][i] : (float)h[0][i]; }
+};
+template <bool SPLIT>
+DEV Eight<SPLIT> img_load8(const Image &im, int z, int64_t row, int col) {
     const char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
-    const nt::f16x8 h = *(const nt::f16x8 *)p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
-    if (SPLIT) {
-        const nt::f16x8 l = *(const nt::f16x8 *)(p + 64);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += (float)l[i];
-    }
+    Eight<SPLIT> v;
+    v.h[0] = *(const nt::f16x8 *)p;
+    if (SPLIT) v.h[SPLIT ? 1 : 0] = *(const nt::f16x8 *)(p + 64);
+    return v;
 }
 template <bool SPLIT>
 DEV void img_store8(const Image &im, int z, int64_t row, int col, const float *v) {
@@ -284,7 +304,7 @@ __global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__re
 
 // X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.
 template <class From, bool SPLIT>
-__global__ __launch_bounds__(256) void k_prepare(From from, int rows, int cols, const double *__restrict__ part, int blocks, double eps, double scale,
+__global__ __launch_bounds__(256) void k_prepare(From from, int r, int c, const double *__restrict__ part, int blocks, double eps, double scale,
                                                  Image P, Image Q) {
     __shared__ double red[4];
     __shared__ float tile[64][65];
@@ -292,8 +312,9 @@ __global__ __launch_bounds__(256) void k_prepare(From from, int rows, int cols, 
     double s = 0.0;
     for (int i = t; i < blocks; i += 256) s += part[z * NORM_BLOCKS + i];
     const double norm = sqrt(block_sum_d(s, red)), inv = scale / (norm > eps ? norm : (norm == norm ? eps : norm));
-    const bool wide = rows <= cols;
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;          // of x
+    const bool wide = from.wide(z);
+    const int rows = wide ? r : c, cols = wide ? c : r;            // of x, and the tile's place in it
+    const int r0 = (wide ? blockIdx.y : blockIdx.x) * 64, c0 = (wide ? blockIdx.x : blockIdx.y) * 64;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int e = t + h * 256, i = e >> 3, j = (e & 7) * 8;
@@ -338,7 +359,8 @@ __global__ __launch_bounds__(256) void k_zero_pads(Image a, int64_t ra, Image b,
 
 struct NoFactors {
     static constexpr bool TURNED = false;
-    typedef None Row, Col;
+    typedef None Row, Col, Pre;
+    DEV Pre pre(int, int, int) const { return {}; }
     DEV Row row(int, int) const { return {}; }
     DEV Col col(int, int) const { return {}; }
 };
@@ -354,7 +376,7 @@ struct GramOut : NoFactors {           // A = X X^T (times T_SCALE); zeros behin
     float scale;
     int N;
     DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(A, z, row, col, half, v); }
-    DEV void put(int z, int m, int n, float *v, Row, Col) const {
+    DEV void put(int z, int m, int n, float *v, Row, Col, Pre) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = n + i < N ? v[i] * scale : 0.f;
         img_store8<SPLIT>(A, z, m, n, v);
@@ -367,9 +389,9 @@ struct PolyOut : NoFactors {           // B = b A + c A A (times T_SCALE)
     float b, c;
     int N;
     DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(B, z, row, col, half, v); }
-    DEV void put(int z, int m, int n, float *v, Row, Col) const {
-        float a[8];
-        img_load8<SPLIT>(A, z, m, n, a);
+    typedef Eight<SPLIT> Pre;
+    DEV Pre pre(int z, int m, int n) const { return img_load8<SPLIT>(A, z, m, n); }
+    DEV void put(int z, int m, int n, float *v, Row, Col, const Pre &a) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = n + i < N ? __builtin_fmaf(c, v[i] * (1.f / T_SCALE), b * a[i]) : 0.f;
         img_store8<SPLIT>(B, z, m, n, v);
@@ -382,9 +404,9 @@ struct NextOut : NoFactors {           // X <- a X + B X into P (in place: a til
     float a;
     int N;
     DEV void put_turned(int z, int row, int col, int half, nt::f16x8 v) const { img_store_half<SPLIT>(Q, z, row, col, half, v); }
-    DEV void put(int z, int m, int n, float *v, Row, Col) const {
-        float x[8];
-        img_load8<SPLIT>(P, z, m, n, x);
+    typedef Eight<SPLIT> Pre;
+    DEV Pre pre(int z, int m, int n) const { return img_load8<SPLIT>(P, z, m, n); }
+    DEV void put(int z, int m, int n, float *v, Row, Col, const Pre &x) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = n + i < N ? __builtin_fmaf(a, x[i], v[i] * (1.f / T_SCALE)) : 0.f;
         img_store8<SPLIT>(P, z, m, n, v);
@@ -396,9 +418,9 @@ struct LastOut : NoFactors {           // the last step: X in the orientation of
     float a, scale;                    // scale = 1 / S
     To to;
     int N;
-    DEV void put(int z, int m, int n, float *v, Row, Col) const {
-        float x[8];
-        img_load8<SPLIT>(X, z, m, n, x);
+    typedef Eight<SPLIT> Pre;
+    DEV Pre pre(int z, int m, int n) const { return img_load8<SPLIT>(X, z, m, n); }
+    DEV void put(int z, int m, int n, float *v, Row, Col, const Pre &x) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(a, x[i], v[i] * (1.f / T_SCALE)) * scale;
         to.put8(z, (int64_t)m * N + n, v, N - n);
@@ -433,44 +455,55 @@ bool is_small(int64_t rows, int64_t cols) {
     return r <= SMALL_R && c <= SMALL_C;
 }
 
+// `batch` matrices of short side r and long side c, the first `wides` of them with rows <= cols.  `to_wide`, `to_tall`: where
+// the two kinds go, counted from the first of each.
 template <bool SPLIT, class From, class To>
-int large(const From &from, const To &to, int batch, int64_t rows, int64_t cols, int steps, const float *coef, double eps, char *ws, hipStream_t st) {
+int large(const From &from, const To &to_wide, const To &to_tall, int batch, int wides, int64_t r64, int64_t c64, int steps, const float *coef, double eps,
+          char *ws, hipStream_t st) {
     constexpr int KIND = SPLIT ? nt::F16_SPLIT : nt::F16;
-    const Plan pl(batch, rows, cols, SPLIT);
+    const Plan pl(batch, r64, c64, SPLIT);
     const int r = (int)pl.r, c = (int)pl.c;
-    const bool wide = rows <= cols;
     double *part = (double *)(ws + pl.part);
     const Image P{ws + pl.p, pl.ld_c, r * pl.ld_c}, A{ws + pl.a, pl.ld_r, r * pl.ld_r}, B{ws + pl.b, pl.ld_r, r * pl.ld_r};
     Image Q{ws + pl.q0, pl.ld_r, c * pl.ld_r}, Q2{ws + pl.q1, pl.ld_r, c * pl.ld_r};
     int log_s = 0;
     while (log_s < 14 && (int64_t)1 << (2 * log_s + 2) <= (int64_t)r * c) ++log_s;
     const float S = (float)(1 << log_s);
-    const int blocks = grid_for(rows * cols, 256 * 8, NORM_BLOCKS);
-    hipLaunchKernelGGL((k_norm<From>), dim3(blocks, 1, batch), dim3(256), 0, st, from, rows * cols, part);
+    const int64_t n = (int64_t)r * c;
+    const int blocks = grid_for(n, 256 * 8, NORM_BLOCKS);
+    hipLaunchKernelGGL((k_norm<From>), dim3(blocks, 1, batch), dim3(256), 0, st, from, n, part);
     DPD_LAUNCH_CHECK();
-    hipLaunchKernelGGL((k_prepare<From, SPLIT>), dim3((unsigned)((cols + 63) / 64), (unsigned)((rows + 63) / 64), batch), dim3(256), 0, st, from, (int)rows,
-                       (int)cols, part, blocks, eps, (double)S, P, Q);
+    hipLaunchKernelGGL((k_prepare<From, SPLIT>), dim3((unsigned)((c + 63) / 64), (unsigned)((r + 63) / 64), batch), dim3(256), 0, st, from, r, c, part, blocks,
+                       eps, (double)S, P, Q);
     DPD_LAUNCH_CHECK();
     const int64_t pad = (SPLIT ? pl.ld_r / 4 : pl.ld_r / 2) - r;
     if (pad) {
         hipLaunchKernelGGL((k_zero_pads<SPLIT>), dim3(grid_for((2 * r + c) * pad, 256), 1, batch), dim3(256), 0, st, A, (int64_t)r, B, (int64_t)r, Q2, (int64_t)c, r);
         DPD_LAUNCH_CHECK();
     }
-    auto product = [&](const Image &x, int M, const Image &y, int N, bool symmetric, const auto &epi) {
+    auto product = [&](const Image &x, int M, const Image &y, int N, bool symmetric, int many, const auto &epi) {
         nt::Args g{};
         g.a = x.base, g.lda = x.ld, g.a_batch = x.batch, g.b = y.base, g.ldb = y.ld, g.b_batch = y.batch, g.M = M, g.N = N;
         g.steps = g.wrap = (int)(x.ld / nt::STEP), g.tail = nt::STEP, g.lower = symmetric;
-        return nt::product<KIND>(g, batch, epi, st);
+        return nt::product<KIND>(g, many, epi, st);
+    };
+    auto from_z = [](Image im, int z) {
+        im.base += z * im.batch;
+        return im;
     };
     for (int k = 0; k < steps; ++k) {
         const float *f = coef + 3 * k;
-        int rc = product(P, r, P, r, true, GramOut<SPLIT>{{}, A, T_SCALE / (S * S), r});
-        if (!rc) rc = product(A, r, A, r, true, PolyOut<SPLIT>{{}, A, B, f[1], f[2], r});
+        int rc = product(P, r, P, r, true, batch, GramOut<SPLIT>{{}, A, T_SCALE / (S * S), r});
+        if (!rc) rc = product(A, r, A, r, true, batch, PolyOut<SPLIT>{{}, A, B, f[1], f[2], r});
         if (!rc && k + 1 < steps) {
-            rc = product(B, r, Q, c, false, NextOut<SPLIT>{{}, P, Q2, f[0], c});
+            rc = product(B, r, Q, c, false, batch, NextOut<SPLIT>{{}, P, Q2, f[0], c});
             std::swap(Q, Q2);
         } else if (!rc) {
-            rc = wide ? product(B, r, Q, c, false, LastOut<SPLIT, To>{{}, P, f[0], 1.f / S, to, c}) : product(Q, c, B, r, false, LastOut<SPLIT, To>{{}, Q, f[0], 1.f / S, to, r});
+            if (wides) rc = product(B, r, Q, c, false, wides, LastOut<SPLIT, To>{{}, P, f[0], 1.f / S, to_wide, c});
+            if (!rc && batch > wides) {
+                const Image q = from_z(Q, wides);
+                rc = product(q, c, from_z(B, wides), r, false, batch - wides, LastOut<SPLIT, To>{{}, q, f[0], 1.f / S, to_tall, r});
+            }
         }
         if (rc) return rc;
     }
@@ -527,7 +560,7 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     if (is_small(rows, cols))
         return with_type(type, [&](auto t) {
             using T = decltype(t);
-            const FromTensor<T> from{(const T *)x, rows * cols, false};
+            const FromTensor<T> from{(const T *)x, rows * cols, false, rows <= cols};
             const ToTensor<T> to{(T *)out, rows * cols, false};
             if (needs_16_waves(rows, cols))
                 hipLaunchKernelGGL((k_small<16, T>), dim3((unsigned)batch), dim3(1024), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
@@ -541,17 +574,50 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        const FromTensor<T> from{(const T *)x, rows * cols, ((uintptr_t)x & 15) == 0 && cols % 8 == 0};
+        const FromTensor<T> from{(const T *)x, rows * cols, ((uintptr_t)x & 15) == 0 && cols % 8 == 0, rows <= cols};
         const ToTensor<T> to{(T *)out, rows * cols, ((uintptr_t)out & 15) == 0 && cols % 8 == 0};
-        return accurate ? large<true>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st)
-                        : large<false>(from, to, (int)batch, rows, cols, steps, coef.v, eps, w, st);
+        const int wides = rows <= cols ? (int)batch : 0;
+        return accurate ? large<true>(from, to, to, (int)batch, wides, rows, cols, steps, coef.v, eps, w, st)
+                        : large<false>(from, to, to, (int)batch, wides, rows, cols, steps, coef.v, eps, w, st);
     });
+}
+
+// Large matrices with the same two sides share the launches of the products: up to TOGETHER of them, and no more than a
+// gigabyte of workspace (a matrix that takes more goes alone).  The first of such a set finds its members.
+struct Set {
+    int index[TOGETHER], n, wides;
+    int64_t r, c;
+};
+static int set_limit(int64_t r, int64_t c, int accurate) {
+    const int64_t one = Plan(1, r, c, accurate != 0).total, fit = ((int64_t)1 << 30) / one;
+    return fit < 1 ? 1 : fit > TOGETHER ? TOGETHER : (int)fit;
+}
+static bool leads_set(int i, int n, const int64_t *rows, const int64_t *cols, int accurate, Set *out) {
+    auto lo = [&](int k) { return rows[k] < cols[k] ? rows[k] : cols[k]; };
+    auto hi = [&](int k) { return rows[k] < cols[k] ? cols[k] : rows[k]; };
+    const int64_t r = lo(i), c = hi(i);
+    if (r <= 0 || is_small(r, c)) return false;
+    const int limit = set_limit(r, c, accurate);
+    int before = 0;
+    for (int k = 0; k < i; ++k) before += lo(k) == r && hi(k) == c;
+    if (before % limit) return false;
+    *out = Set{{}, 0, 0, r, c};
+    int found[TOGETHER], m = 0;
+    for (int k = i; k < n && m < limit; ++k)
+        if (lo(k) == r && hi(k) == c) found[m++] = k;
+    for (int tall = 0; tall < 2; ++tall)               // those with rows <= cols first
+        for (int k = 0; k < m; ++k)
+            if ((rows[found[k]] > cols[found[k]]) == (tall == 1)) out->index[out->n++] = found[k], out->wides += !tall;
+    return true;
 }
 
 extern "C" size_t dpd_muon_workspace_bytes(int n, const int64_t *h_rows, const int64_t *h_cols, int accurate) {
     size_t most = 256;
+    if (!h_rows || !h_cols) return most;
     for (int i = 0; i < n; ++i) {
-        const size_t b = dpd_orthogonalize_workspace_bytes(1, h_rows[i], h_cols[i], accurate);
+        Set s;
+        if (!leads_set(i, n, h_rows, h_cols, accurate, &s)) continue;
+        const size_t b = (size_t)Plan(s.n, s.r, s.c, accurate != 0).total + 256;
         most = b > most ? b : most;
     }
     return most;
@@ -589,11 +655,23 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
         for (int i = 0; i < n; ++i) {
             const int64_t rows = h_rows[i], cols = h_cols[i];
             if (rows == 0 || cols == 0) continue;
-            const float factor = (float)(lr * sqrt(rows > cols ? (double)rows / (double)cols : 1.0));
+            auto factor_of = [&](int k) { return (float)(lr * sqrt(h_rows[k] > h_cols[k] ? (double)h_rows[k] / (double)h_cols[k] : 1.0)); };
+            const float factor = factor_of(i);
             if (!is_small(rows, cols)) {
-                const FromMomentum<T> from{(const T *)h_g[i], h_m[i], mu, nesterov, (((uintptr_t)h_g[i] | (uintptr_t)h_m[i]) & 15) == 0 && cols % 8 == 0};
-                const ToWeights<T> to{(T *)h_p[i], keep, factor, ((uintptr_t)h_p[i] & 15) == 0 && cols % 8 == 0};
-                const int rc = accurate ? large<true>(from, to, 1, rows, cols, steps, coef.v, eps, w, st) : large<false>(from, to, 1, rows, cols, steps, coef.v, eps, w, st);
+                Set s;
+                if (!leads_set(i, n, h_rows, h_cols, accurate, &s)) continue;          // went with an earlier one
+                FromMomenta<T> from{{}, {}, mu, nesterov, 0, 0};
+                ToManyWeights<T> to[2] = {{{}, keep, 0.f, 0}, {{}, keep, 0.f, 0}};
+                for (int k = 0; k < s.n; ++k) {
+                    const int j = s.index[k], tall = k >= s.wides, at = tall ? k - s.wides : k;
+                    from.g[k] = (const T *)h_g[j], from.m[k] = h_m[j];
+                    from.whole_bits |= (unsigned)((((uintptr_t)h_g[j] | (uintptr_t)h_m[j]) & 15) == 0 && h_cols[j] % 8 == 0) << k;
+                    from.wide_bits |= (unsigned)!tall << k;
+                    to[tall].p[at] = (T *)h_p[j], to[tall].factor = factor_of(j);
+                    to[tall].whole_bits |= (unsigned)(((uintptr_t)h_p[j] & 15) == 0 && h_cols[j] % 8 == 0) << at;
+                }
+                const int rc = accurate ? large<true>(from, to[0], to[1], s.n, s.wides, s.r, s.c, steps, coef.v, eps, w, st)
+                                        : large<false>(from, to[0], to[1], s.n, s.wides, s.r, s.c, steps, coef.v, eps, w, st);
                 if (rc) return rc;
                 continue;
             }

@@ -239,6 +239,24 @@ def test_muon_many_matrices_and_refusals():
     assert torch.equal(q, r)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_muon_matrices_of_one_size_go_together(dtype):
+    """Wide and tall matrices of the same two sides share launches: each comes out as it does alone (the tile that is chosen
+    may differ, and with it the order of a sum), within the tolerance of its step."""
+    shapes = [(70, 200), (200, 70), (96, 96), (70, 200), (200, 70), (96, 96), (200, 70)] + [(130, 66)] * 9 + [(40, 40), (66, 130)]
+    ps = [torch.nn.Parameter(update(r, c, i).to(dtype).to(DEV)) for i, (r, c) in enumerate(shapes)]
+    p0 = [p.detach().cpu() for p in ps]
+    for i, p in enumerate(ps):
+        p.grad = update(*p.shape, 300 + i).to(dtype).to(DEV)
+    opt = Muon(ps, lr=0.05, momentum=0.9)
+    opt.step()
+    for p, before in zip(ps, p0):
+        want, m, u, f = muon_oracle(before, p.grad.cpu(), torch.zeros(p.shape), 0.05, 0.9, True, 0.0)
+        tol = f * (allowed(u, oo.iterate(u), dtype != torch.bfloat16) + 500 * 2.0 ** -22) + (U[dtype] + 2.0 ** -22) * float(want.norm()) * 1.01
+        assert float((p.detach().cpu().double() - want).norm()) <= tol, p.shape
+        assert torch.equal(opt.state[p]["momentum_buffer"], p.grad.float())
+
+
 def test_muon_in_a_graph():
     ps = [torch.nn.Parameter(update(r, c, r).to(DEV)) for r, c in ((30, 32), (140, 90))]
     for p in ps:
