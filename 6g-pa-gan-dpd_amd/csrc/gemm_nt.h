@@ -131,8 +131,9 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B, PART = (BM + BN) * STEP, STAGE = WAVES_K * PART;
     static_assert(LOADS_A >= 1 && LOADS_B >= 1 && LOADS_A * 8 * WAVES == BM && LOADS_B * 8 * WAVES == BN, "every wave loads whole groups of 8 rows");
     static_assert(TN % 2 == 0 && (TM % 2 == 0 || KIND != F16_SPLIT) && STAGES >= 2 && (STAGES - 2) * LOADS < 64, "pairs of blocks; the wait counter has 6 bits");
-    static_assert(STAGES * STAGE <= 160 * 1024, "LDS of a compute unit");
-    __shared__ __attribute__((aligned(256))) char smem[STAGES * STAGE];
+    constexpr int PITCH = BM + 8, TURN_BYTES = Epilogue::TURNED ? BN * PITCH * 2 : 0, LDS = STAGES * STAGE > TURN_BYTES ? STAGES * STAGE : TURN_BYTES;
+    static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
+    __shared__ __attribute__((aligned(256))) char smem[LDS];
     int tm, tn;
     tile_of(g, blockIdx.x, gridDim.x, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
@@ -375,35 +376,39 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
                     for (int e = 0; e < 4; ++e) acc[i][2 * j][e] = v[e], acc[i][2 * j + 1][e] = v[4 + e];
                 }
             }
+            if (Epilogue::TURNED) __builtin_amdgcn_sched_barrier(0);
         }
     }
     // The tile once more, turned: through LDS (free now), as fp16 rows of BM values along m, a pass for each half of the
-    // split form.  Chunks of 8 values are permuted by the row so that the 16 lanes that write one column spread out.
+    // split form.
     if constexpr (Epilogue::TURNED) {
         if (!turn) return;
-        static_assert(BM * BN * 2 <= STAGES * STAGE, "a turned tile fits into LDS");
-        constexpr int CHUNKS = BM / 8, MASK = CHUNKS % 32 == 0 ? 31 : CHUNKS % 16 == 0 ? 15 : 7;
-        _Float16 *t = (_Float16 *)smem;
-#pragma unroll
+        constexpr int CHUNKS = BM / 8;
+        _Float16 *t = (_Float16 *)smem, *mine_t = t + (wn * TN * 16 + q * 8) * PITCH + wm * TM * 16 + r;
+#pragma unroll 1
         for (int half = 0; half < (SPLIT ? 2 : 1); ++half) {
             __syncthreads();
+            if (WAVES_K == 1 || group == 0) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (WAVES_K > 1 && group > 0) break;
-                        const int ml = (wm * TM + i) * 16 + r, nl = wn * TN * 16 + (j >> 1) * 32 + q * 8 + (j & 1) * 4 + e;
-                        const _Float16 h = (_Float16)acc[i][j][e];
-                        t[nl * BM + (((ml >> 3) ^ ((nl >> 2) & MASK)) << 3) + (ml & 7)] = h;
-                        if (SPLIT) acc[i][j][e] -= (float)h;
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            float v = acc[i][j][e];
+                            if (SPLIT) {
+                                asm volatile("" : "+v"(v));    // nothing of one pass is kept for the other: registers
+                                v -= half ? (float)(_Float16)v : 0.f;
+                            }
+                            mine_t[((j >> 1) * 32 + (j & 1) * 4 + e) * PITCH + i * 16] = (_Float16)v;
+                        }
+                    __builtin_amdgcn_sched_barrier(0);         // one block row's conversions at a time: registers
+                }
+            }
             __syncthreads();
             for (int k = threadIdx.x; k < BN * CHUNKS; k += 64 * WAVES * WAVES_K) {
                 const int nl = k / CHUNKS, c = k - nl * CHUNKS;
-                if (n0 + nl < g.N && m0 + c * 8 < g.M)
-                    epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * BM + ((c ^ ((nl >> 2) & MASK)) << 3)));
+                if (n0 + nl < g.N && m0 + c * 8 < g.M) epi.put_turned(blockIdx.z, n0 + nl, m0 + c * 8, half, *(const f16x8 *)(t + nl * PITCH + c * 8));
             }
         }
     }
@@ -471,7 +476,7 @@ static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st
     switch (best_tile(g, batch, SPLIT)) {
     case 0: return launch<KIND, 256, 256, 2, 4, 1, 2>(g, batch, epi, st);
     case 1: return launch<KIND, 256, 128, 4, 2, 1, 3>(g, batch, epi, st);
-    case 2: return launch<KIND, 192, 192, 2, 2, 1, 3>(g, batch, epi, st);
+    case 2: return launch<KIND, 192, 192, SPLIT ? 2 : 4, 2, 1, 3>(g, batch, epi, st);
     case 3: return launch<KIND, 128, 128, 2, SPLIT ? 2 : 4, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
     case 4: return launch<KIND, 128, 128, 2, 4, 1, 2>(g, batch, epi, st);
     case 5: return launch<KIND, 128, 64, 2, 2, 1, 3>(g, batch, epi, st);

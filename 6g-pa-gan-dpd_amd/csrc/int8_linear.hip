@@ -1,7 +1,7 @@
 // The 8-bit linear layer: rows quantised with one scale each, the int8 product of two sets of such rows, and the
 // straight-through gradients.
 //
-//   quantiser   s = fl32(max(max|x|, 2^-100) / 127),  q = round-half-even(x / s) of the exact quotient
+//   quantiser   s = fl32(max(max|x|, 2^-100) fl32(1 / 127)),  q = round-half-even(x / s) of the exact quotient
 //   product     y[m, n] = ((sum_k qa[m, k] qb[n, k]) * sa[m]) * sb[n] + bias[n]     (the sum exactly, in int32)
 //   gradients   gx = g (qw sw),  gw = g^T (qx sx),  gb = column sums of g
 #include <type_traits>
@@ -22,7 +22,7 @@ DEV unsigned wave_umax(unsigned v) {
 
 // The scale of a row from the largest |x| (as bits); NaN if the row holds a NaN or an infinity.
 DEV float row_scale(unsigned top) {
-    return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(top), SCALE_FLOOR) / 127.0f;
+    return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(top), SCALE_FLOOR) * (1.0f / 127.0f);
 }
 
 // round-half-even(x / s) of the exact quotient.  x * inv is off by less than 2^-15, so rint gives the integer or its

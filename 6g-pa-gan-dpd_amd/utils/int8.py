@@ -59,7 +59,7 @@ def _row_bytes(k: int) -> int:
 
 
 def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(q, scale) of the rows of x [..., K]: scale = max(max|row|, 2^-100) / 127 in fp32, q = round-half-even(row / scale)
+    """(q, scale) of the rows of x [..., K]: scale = max(max|row|, 2^-100) times fl32(1 / 127) in fp32, q = round-half-even(row / scale)
     as int8.  A row that holds a NaN or an infinity gets the scale NaN and zeros, so every product with it is NaN."""
     L.need_gpu(x)
     x = x.detach()

@@ -367,7 +367,7 @@ int dpd_q88_matrix_infer(const int16_t *iq, int64_t B, int64_t S, const void *im
 #define DPD_BF16 1
 #define DPD_F16 2
 
-/* Rows of x [rows, cols] in 8 bits with one scale each: scale[r] = max(max|x[r]|, 2^-100) / 127 (rounded once to fp32),
+/* Rows of x [rows, cols] in 8 bits with one scale each: scale[r] = max(max|x[r]|, 2^-100) * fl32(1 / 127) in fp32,
  * q = the integer nearest to the exact x / scale, ties to even (|q| <= 127).  A row that holds a NaN or an infinity gets
  * the scale NaN and zeros.  q [rows, ldq]: the columns cols..ldq-1 are set to zero. */
 int dpd_quantize_rows_int8(const void *x, int type, int64_t rows, int64_t cols, int64_t ldx, int8_t *q, int64_t ldq,

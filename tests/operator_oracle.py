@@ -12,7 +12,7 @@ def quantize_rows(x):
     x = x.float().cpu()
     top = x.abs().amax(-1, keepdim=True)
     bad = ~torch.isfinite(x).all(-1, keepdim=True)
-    s = torch.where(bad, torch.full_like(top, float("nan")), torch.clamp_min(top, 2.0 ** -100) / 127)
+    s = torch.where(bad, torch.full_like(top, float("nan")), torch.clamp_min(top, 2.0 ** -100) * torch.tensor(1 / 127, dtype=torch.float32))
     q = torch.where(bad, torch.zeros((), dtype=torch.float64), torch.round(x.double() / s.double()))
     return q.to(torch.int8), s[..., 0]
 
