@@ -451,6 +451,8 @@ constexpr Tile TILES[] = {
     {96, 96, {0.29f, 4.f}, {}, {}, {}},                                       // an odd number of block rows a wave: not split
     {64, 64, {0.19f, 3.1f}, {}, {0.2475f, 2.9f}, {}},
     {64, 64, {0.208f, 2.9f}, {0.377f, 2.6f}, {0.35f, 0.5f}, {0.39f, 3.8f}},
+    {64, 32, {0.131f, 2.9f}, {}, {0.131f, 3.2f}, {}},
+    {32, 32, {0.071f, 3.2f}, {}, {0.08f, 3.2f}, {}},
 };
 
 static inline int best_tile(const Args &g, int batch, bool split) {
@@ -484,7 +486,9 @@ static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st
         if constexpr (!SPLIT) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
         [[fallthrough]];
     case 7: return launch<KIND, 64, 64, 2, 2, 2, 4>(g, batch, epi, st);
-    default: return launch<KIND, 64, 64, 2, 2, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
+    case 8: return launch<KIND, 64, 64, 2, 2, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
+    case 9: return launch<KIND, 64, 32, 2, 1, 4, 3>(g, batch, epi, st);
+    default: return launch<KIND, 32, 32, 1, 1, 4, 3>(g, batch, epi, st);
     }
 }
 

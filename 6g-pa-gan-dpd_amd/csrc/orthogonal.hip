@@ -278,14 +278,6 @@ DEV void img_store8(const Image &im, int z, int64_t row, int col, const float *v
     *(nt::f16x8 *)p = h;
     if (SPLIT) *(nt::f16x8 *)(p + 64) = l;
 }
-template <bool SPLIT>
-DEV void img_store1(const Image &im, int z, int64_t row, int col, float v) {
-    char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
-    const _Float16 h = (_Float16)v;
-    *(_Float16 *)p = h;
-    if (SPLIT) *(_Float16 *)(p + 64) = (_Float16)(v - (float)h);
-}
-
 // Sum of squares of each matrix (and, for the optimiser, the new momentum): NORM_BLOCKS fp64 partial sums each.
 template <class From>
 __global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__restrict__ part) {
@@ -302,16 +294,31 @@ __global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__re
     if (threadIdx.x == 0) part[z * NORM_BLOCKS + blockIdx.x] = s;
 }
 
-// X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.
+// 64 rows of an image from `row`: zeros from column `from` to the end of the row (16-byte pieces; `from` rounded down to 8,
+// the columns in front of it are written later, by the products).
+template <bool SPLIT>
+DEV void zero_pads(const Image &im, int z, int row, int rows, int from) {
+    const int end = (int)(SPLIT ? im.ld / 4 : im.ld / 2), first = from & ~7, pieces = (end - first) / 8;
+    const float zero[8] = {};
+    for (int e = threadIdx.x; e < 64 * pieces; e += 256) {
+        const int i = row + e / pieces, j = first + e % pieces * 8;
+        if (i < rows) img_store8<SPLIT>(im, z, i, j, zero);
+    }
+}
+
+// X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.  The images
+// that the products fill first get the zeros behind their rows here too.
 template <class From, bool SPLIT>
 __global__ __launch_bounds__(256) void k_prepare(From from, int r, int c, const double *__restrict__ part, int blocks, double eps, double scale,
-                                                 Image P, Image Q) {
+                                                 Image P, Image Q, Image Q2, Image A, Image B) {
     __shared__ double red[4];
     __shared__ float tile[64][65];
     const int z = blockIdx.z, t = threadIdx.x;
     double s = 0.0;
     for (int i = t; i < blocks; i += 256) s += part[z * NORM_BLOCKS + i];
     const double norm = sqrt(block_sum_d(s, red)), inv = scale / (norm > eps ? norm : (norm == norm ? eps : norm));
+    if (blockIdx.y == 0) zero_pads<SPLIT>(Q2, z, blockIdx.x * 64, c, r);
+    if (blockIdx.x == 0) zero_pads<SPLIT>(A, z, blockIdx.y * 64, r, r), zero_pads<SPLIT>(B, z, blockIdx.y * 64, r, r);
     const bool wide = from.wide(z);
     const int rows = wide ? r : c, cols = wide ? c : r;            // of x, and the tile's place in it
     const int r0 = (wide ? blockIdx.y : blockIdx.x) * 64, c0 = (wide ? blockIdx.x : blockIdx.y) * 64;
@@ -339,21 +346,6 @@ __global__ __launch_bounds__(256) void k_prepare(From from, int r, int c, const 
             for (int k = 0; k < 8; ++k) v[k] = tile[j + k][i];
             img_store8<SPLIT>(flip, z, c0 + i, r0 + j, v);
         }
-    }
-}
-
-// zeros behind column `from` of the rows of up to three images (16-bit words; both halves of a block in the split form)
-template <bool SPLIT>
-__global__ __launch_bounds__(256) void k_zero_pads(Image a, int64_t ra, Image b, int64_t rb, Image c, int64_t rc, int from) {
-    const int z = blockIdx.z, pad = (int)((SPLIT ? a.ld / 4 : a.ld / 2) - from);
-    const int64_t total = (ra + rb + rc) * pad;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < total; e += (int64_t)gridDim.x * 256) {
-        int64_t row = e / pad;
-        const int col = from + (int)(e - row * pad);
-        const Image *im = &a;
-        if (row >= ra) row -= ra, im = &b;
-        if (im == &b && row >= rb) row -= rb, im = &c;
-        img_store1<SPLIT>(*im, z, row, col, 0.f);
     }
 }
 
@@ -474,13 +466,8 @@ int large(const From &from, const To &to_wide, const To &to_tall, int batch, int
     hipLaunchKernelGGL((k_norm<From>), dim3(blocks, 1, batch), dim3(256), 0, st, from, n, part);
     DPD_LAUNCH_CHECK();
     hipLaunchKernelGGL((k_prepare<From, SPLIT>), dim3((unsigned)((c + 63) / 64), (unsigned)((r + 63) / 64), batch), dim3(256), 0, st, from, r, c, part, blocks,
-                       eps, (double)S, P, Q);
+                       eps, (double)S, P, Q, Q2, A, B);
     DPD_LAUNCH_CHECK();
-    const int64_t pad = (SPLIT ? pl.ld_r / 4 : pl.ld_r / 2) - r;
-    if (pad) {
-        hipLaunchKernelGGL((k_zero_pads<SPLIT>), dim3(grid_for((2 * r + c) * pad, 256), 1, batch), dim3(256), 0, st, A, (int64_t)r, B, (int64_t)r, Q2, (int64_t)c, r);
-        DPD_LAUNCH_CHECK();
-    }
     auto product = [&](const Image &x, int M, const Image &y, int N, bool symmetric, int many, const auto &epi) {
         nt::Args g{};
         g.a = x.base, g.lda = x.ld, g.a_batch = x.batch, g.b = y.base, g.ldb = y.ld, g.b_batch = y.batch, g.M = M, g.N = N;
