@@ -45,6 +45,7 @@ struct FromMomentum {                                 // g and the momentum, whi
         m[i] = w;
         return nesterov ? to_f32(g[i]) + mu * w : w;
     }
+    DEV float again(int, int64_t i) const { return nesterov ? to_f32(g[i]) + mu * m[i] : m[i]; }
 };
 constexpr int TOGETHER = 8;                           // large matrices of one size that go through the products together
 template <class T>
@@ -238,12 +239,232 @@ struct SmallTable {
     float factor[TABLE];
 };
 
+// ---- matrices that fit into one compute unit as fp16 factors --------------------------------------
+// One workgroup of 16 waves, one matrix: X [r][c] and A, overwritten by B, [r][r] in LDS as fp16, scaled as the images of
+// the large path are (one term, or two planes in the split form), padded with zeros to whole 32 x 32 blocks.  A wave forms
+// such blocks on v_mfma_f32_16x16x32_f16 (four 16 x 16 tiles from two fragments of each factor; a tile's lane holds four
+// successive columns of one row).  The sums of A and A A run along rows of LDS; that of B X runs down the columns of X,
+// which the transposing read ds_read_b64_tr_b16 gives (4 rows of 16 columns each).  Rows are 16 bytes longer than their
+// padded length, so that 16 of them spread over the banks.  Five barriers a step instead of three launches.
+constexpr int FIT_LDS = 150 * 1024, FIT_WAVES = 16, FIT_BLOCKS = 3;     // blocks of X that a wave holds
+
+__host__ DEV int64_t fit_bytes(int64_t r, int64_t c, bool split) {
+    const int64_t r32 = (r + 31) & ~31, c32 = (c + 31) & ~31;
+    return r32 * (c32 + 8 + r32 + 8) * (split ? 4 : 2);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) char lds_byte;
+
+DEV nt::f16x8 read_down(const _Float16 *p, int pitch) {        // 8 rows of one column, out of what 16 lanes point at
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * pitch));
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(nt::f16x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <bool SPLIT>
+struct Plane {                          // a factor in LDS
+    _Float16 *h, *l;
+    int pitch;
+    DEV f32x4_t get4(int row, int col) const {
+        const nt::f16x4 a = *(const nt::f16x4 *)(h + row * pitch + col);
+        f32x4_t v = {(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
+        if (SPLIT) {
+            const nt::f16x4 b = *(const nt::f16x4 *)(l + row * pitch + col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += (float)b[e];
+        }
+        return v;
+    }
+    DEV void put4(int row, int col, f32x4_t v) const {
+        nt::f16x4 a, b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = (_Float16)v[e], b[e] = (_Float16)(v[e] - (float)a[e]);
+        *(nt::f16x4 *)(h + row * pitch + col) = a;
+        if (SPLIT) *(nt::f16x4 *)(l + row * pitch + col) = b;
+    }
+    DEV void put(int row, int col, float v) const {
+        const _Float16 a = (_Float16)v;
+        h[row * pitch + col] = a;
+        if (SPLIT) l[row * pitch + col] = (_Float16)(v - (float)a);
+    }
+};
+
+template <int N>
+struct Block {                          // N x N tiles of a product: tile (ti, tj), row ti * 16 + (lane & 15), columns tj * 16 + 4 (lane >> 4) + 0..3
+    f32x4_t t[N][N];
+};
+
+// sum over n terms of rows u0.. of U and rows v0.. of V (DOWN: of columns v0.. of V, whose rows the sum runs along)
+template <bool SPLIT, bool DOWN, int N>
+DEV Block<N> block_product(const Plane<SPLIT> &U, int u0, const Plane<SPLIT> &V, int v0, int n, int lane) {
+    const int r = lane & 15, q = lane >> 4;
+    Block<N> b;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) b.t[i][j] = f32x4_t{0, 0, 0, 0};
+    const int u_at = (u0 + r) * U.pitch + q * 8, v_at = DOWN ? (q * 8 + (r >> 2)) * V.pitch + v0 + (r & 3) * 4 : (v0 + r) * V.pitch + q * 8;
+#pragma unroll 2
+    for (int k = 0; k < n; k += 32) {
+        nt::f16x8 uh[N], ul[N], vh[N], vl[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = u_at + i * 16 * U.pitch + k;
+            uh[i] = *(const nt::f16x8 *)(U.h + at);
+            if (SPLIT) ul[i] = *(const nt::f16x8 *)(U.l + at);
+            if (DOWN) {
+                const int to = v_at + k * V.pitch + i * 16;
+                vh[i] = read_down(V.h + to, V.pitch);
+                if (SPLIT) vl[i] = read_down(V.l + to, V.pitch);
+            } else {
+                const int to = v_at + i * 16 * V.pitch + k;
+                vh[i] = *(const nt::f16x8 *)(V.h + to);
+                if (SPLIT) vl[i] = *(const nt::f16x8 *)(V.l + to);
+            }
+        }
+        auto add = [&](const nt::f16x8 *v, const nt::f16x8 *u) {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) b.t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j], u[i], b.t[i][j], 0, 0, 0);
+        };
+        if (SPLIT) add(vl, uh), add(vh, ul);
+        add(vh, uh);
+    }
+    return b;
+}
+
+// A = X X^T (times T_SCALE), then B = b A + c A A in its place, by blocks of N x N tiles: at most one a wave.
+template <bool SPLIT, int N>
+DEV void fit_poly(const Plane<SPLIT> &X, const Plane<SPLIT> &A, int r32, int c32, float S, float cb3, float cc, int wave, int lane) {
+    const int i16 = lane & 15, q = lane >> 4, side = r32 / (16 * N), ba = wave / side, bj = wave - ba * side;
+    const bool has = wave < side * side;
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) f(i, j, (ba * N + i) * 16 + i16, (bj * N + j) * 16 + q * 4);
+    };
+    Block<N> b;
+    if (has) {
+        b = block_product<SPLIT, false, N>(X, ba * N * 16, X, bj * N * 16, c32, lane);
+        each([&](int i, int j, int row, int col) {
+            f32x4_t v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = b.t[i][j][e] * (T_SCALE / (S * S));
+            A.put4(row, col, v);
+        });
+    }
+    __syncthreads();
+    if (has) {                                         // the second factor by its rows: A is symmetric
+        b = block_product<SPLIT, false, N>(A, ba * N * 16, A, bj * N * 16, r32, lane);
+        each([&](int i, int j, int row, int col) {
+            const f32x4_t a = A.get4(row, col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b.t[i][j][e] = __builtin_fmaf(cc, b.t[i][j][e] * (1.f / T_SCALE), cb3 * a[e]);
+        });
+    }
+    __syncthreads();
+    if (has) each([&](int i, int j, int row, int col) { A.put4(row, col, b.t[i][j]); });
+    __syncthreads();
+}
+
+template <bool SPLIT, class From, class To>
+DEV void fit_iterate(const From &from, const To &to, int z, int rows, int cols, const Coef &coef, int steps, double eps, _Float16 *lds) {
+    __shared__ double red[FIT_WAVES];
+    const bool wide = rows <= cols;
+    const int r = wide ? rows : cols, c = wide ? cols : rows, n = rows * cols, t = threadIdx.x;
+    const int r32 = (r + 31) & ~31, c32 = (c + 31) & ~31, rb = r32 >> 5, cb = c32 >> 5;
+    const int wave0 = __builtin_amdgcn_readfirstlane(t >> 6);
+    Plane<SPLIT> X{lds, lds + r32 * (c32 + 8), c32 + 8}, A;
+    A.h = lds + r32 * (c32 + 8) * (SPLIT ? 2 : 1), A.l = A.h + r32 * (r32 + 8), A.pitch = r32 + 8;
+    int log_s = 0;
+    while (log_s < 14 && (int64_t)1 << (2 * log_s + 2) <= (int64_t)r * c) ++log_s;
+    const float S = (float)(1 << log_s);
+    for (int e = t; e < r32 * (c32 + 8) * (SPLIT ? 2 : 1) / 8; e += 64 * FIT_WAVES) ((f32x4_t *)lds)[e] = f32x4_t{0, 0, 0, 0};
+    double s = 0.0;
+    for (int e = t; e < n; e += 64 * FIT_WAVES) {
+        const float v = from.first(z, e);
+        s += (double)v * (double)v;
+    }
+    const double norm = sqrt(group_sum_d<FIT_WAVES>(s, red)), inv = (double)S / (norm > eps ? norm : (norm == norm ? eps : norm));
+    for (int e = t; e < n; e += 64 * FIT_WAVES) {      // the same thread saw the same elements: no barrier for the momentum
+        const int i = e / cols, j = e - i * cols;
+        const float v = (float)((double)from.again(z, e) * inv);
+        X.put(wide ? i : j, wide ? j : i, v);
+    }
+    __syncthreads();
+    for (int k = 0; k < steps; ++k) {
+        // the compiler would keep every address of a step in registers through the loop: they are formed anew instead
+        int wave = wave0, lane = t & 63;
+        asm volatile("" : "+s"(wave), "+v"(lane));
+        const int i16 = lane & 15, q = lane >> 4;
+        const float ca = coef.v[3 * k], cb3 = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
+        if (r32 <= 64) fit_poly<SPLIT, 1>(X, A, r32, c32, S, cb3, cc, wave, lane);       // 16 tiles for 16 waves
+        else fit_poly<SPLIT, 2>(X, A, r32, c32, S, cb3, cc, wave, lane);
+        const bool last = k + 1 == steps;
+        Block<2> x[FIT_BLOCKS];                           // X <- a X + B X, written once every wave has read X
+#pragma unroll
+        for (int h = 0; h < FIT_BLOCKS; ++h) {
+            const int id = wave + h * FIT_WAVES, bi = id / cb, bc = id - bi * cb;
+            if (id < rb * cb) {
+                x[h] = block_product<SPLIT, true, 2>(A, bi * 32, X, bc * 32, r32, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const f32x4_t old = X.get4(bi * 32 + i * 16 + i16, bc * 32 + j * 16 + q * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[h].t[i][j][e] = __builtin_fmaf(ca, old[e], x[h].t[i][j][e] * (1.f / T_SCALE));
+                    }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < FIT_BLOCKS; ++h) {
+            const int id = wave + h * FIT_WAVES, bi = id / cb, bc = id - bi * cb;
+            if (id < rb * cb) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int row = bi * 32 + i * 16 + i16, col = bc * 32 + j * 16 + q * 4;
+                        if (!last) {
+                            X.put4(row, col, x[h].t[i][j]);
+                        } else if (row < r) {          // in fp32, where it belongs
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (col + e < c) to.put(z, wide ? (int64_t)row * cols + col + e : (int64_t)(col + e) * cols + row, x[h].t[i][j][e] * (1.f / S));
+                        }
+                    }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <bool SPLIT, class T>
+__global__ __launch_bounds__(64 * FIT_WAVES) void k_fit(FromTensor<T> from, ToTensor<T> to, int rows, int cols, Coef coef, int steps, double eps) {
+    __shared__ __attribute__((aligned(16))) _Float16 lds[FIT_LDS / 2];
+    fit_iterate<SPLIT>(from, to, blockIdx.x, rows, cols, coef, steps, eps, lds);
+}
+
 template <class T>
 __global__ __launch_bounds__(1024) void k_small_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
     __shared__ __attribute__((aligned(16))) float lds[SMALL_LDS];
     const int z = blockIdx.x;
     small_iterate<16>(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z]}, 0, tab.rows[z],
                   tab.cols[z], coef, steps, eps, lds);
+}
+
+template <bool SPLIT, class T>
+__global__ __launch_bounds__(64 * FIT_WAVES) void k_fit_muon(SmallTable tab, float mu, int nesterov, float keep, Coef coef, int steps, double eps) {
+    __shared__ __attribute__((aligned(16))) _Float16 lds[FIT_LDS / 2];
+    const int z = blockIdx.x;
+    fit_iterate<SPLIT>(FromMomentum<T>{(const T *)tab.g[z], tab.m[z], mu, nesterov}, ToWeights<T>{(T *)tab.p[z], keep, tab.factor[z]}, 0, tab.rows[z],
+                       tab.cols[z], coef, steps, eps, lds);
 }
 
 // ---- large matrices ----------------------------------------------------------------------------
@@ -449,6 +670,12 @@ bool is_small(int64_t rows, int64_t cols) {
 
 // `batch` matrices of short side r and long side c, the first `wides` of them with rows <= cols.  `to_wide`, `to_tall`: where
 // the two kinds go, counted from the first of each.
+// One compute unit holds the matrix (it needs no workspace then, like a small one).
+bool fits(int64_t rows, int64_t cols, bool split) {
+    const int64_t r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
+    return r <= 128 && c <= 65536 && fit_bytes(r, c, split) <= FIT_LDS && ((r + 31) / 32) * ((c + 31) / 32) <= FIT_WAVES * FIT_BLOCKS;
+}
+
 template <bool SPLIT, class From, class To>
 int large(const From &from, const To &to_wide, const To &to_tall, int batch, int wides, int64_t r64, int64_t c64, int steps, const float *coef, double eps,
           char *ws, hipStream_t st) {
@@ -529,7 +756,7 @@ int check_matrix(const char *who, int64_t rows, int64_t cols) {
 }  // namespace
 
 extern "C" size_t dpd_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int accurate) {
-    if (batch <= 0 || rows <= 0 || cols <= 0 || is_small(rows, cols)) return 256;
+    if (batch <= 0 || rows <= 0 || cols <= 0 || is_small(rows, cols) || fits(rows, cols, accurate != 0)) return 256;
     return (size_t)Plan(batch, rows, cols, accurate != 0).total + 256;
 }
 
@@ -553,6 +780,16 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
                 hipLaunchKernelGGL((k_small<16, T>), dim3((unsigned)batch), dim3(1024), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
             else
                 hipLaunchKernelGGL((k_small<4, T>), dim3((unsigned)batch), dim3(256), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
+            DPD_LAUNCH_CHECK();
+            return DPD_OK;
+        });
+    if (fits(rows, cols, accurate != 0))
+        return with_type(type, [&](auto t) {
+            using T = decltype(t);
+            const FromTensor<T> from{(const T *)x, rows * cols, false, rows <= cols};
+            const ToTensor<T> to{(T *)out, rows * cols, false};
+            if (accurate) hipLaunchKernelGGL((k_fit<true, T>), dim3((unsigned)batch), dim3(64 * FIT_WAVES), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
+            else hipLaunchKernelGGL((k_fit<false, T>), dim3((unsigned)batch), dim3(64 * FIT_WAVES), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
         });
@@ -583,7 +820,7 @@ static bool leads_set(int i, int n, const int64_t *rows, const int64_t *cols, in
     auto lo = [&](int k) { return rows[k] < cols[k] ? rows[k] : cols[k]; };
     auto hi = [&](int k) { return rows[k] < cols[k] ? cols[k] : rows[k]; };
     const int64_t r = lo(i), c = hi(i);
-    if (r <= 0 || is_small(r, c)) return false;
+    if (r <= 0 || is_small(r, c) || fits(r, c, accurate != 0)) return false;
     const int limit = set_limit(r, c, accurate);
     int before = 0;
     for (int k = 0; k < i; ++k) before += lo(k) == r && hi(k) == c;
@@ -621,7 +858,7 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
         if (const int rc = check_matrix("muon_step", h_rows[i], h_cols[i])) return rc;
         const bool empty = h_rows[i] == 0 || h_cols[i] == 0;
         DPD_REQUIRE(empty || (h_p[i] && h_g[i] && h_m[i]), DPD_ERR_INVALID_ARG, "muon_step: null pointer (matrix %d)", i);
-        any_large = any_large || (!empty && !is_small(h_rows[i], h_cols[i]));
+        any_large = any_large || (!empty && !is_small(h_rows[i], h_cols[i]) && !fits(h_rows[i], h_cols[i], accurate != 0));
     }
     DPD_REQUIRE(!any_large || (ws && ws_bytes >= dpd_muon_workspace_bytes(n, h_rows, h_cols, accurate)), DPD_ERR_WORKSPACE, "muon_step: workspace");
     char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
@@ -631,11 +868,15 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
     const float keep = (float)(1.0 - lr * weight_decay), mu = (float)momentum;
     return with_type(p_type, [&](auto t) {
         using T = decltype(t);
-        SmallTable tab{};
-        int used = 0;
-        auto flush = [&]() {
-            if (used) hipLaunchKernelGGL((k_small_muon<T>), dim3(used), dim3(1024), 0, st, tab, mu, nesterov, keep, coef, steps, eps);
-            used = 0;
+        SmallTable tabs[2]{};                      // small ones, and those that fit into a compute unit
+        int used[2] = {0, 0};
+        auto flush = [&](int kind) {
+            const int many = used[kind];
+            used[kind] = 0;
+            if (!many) return DPD_OK;
+            if (kind == 0) hipLaunchKernelGGL((k_small_muon<T>), dim3(many), dim3(1024), 0, st, tabs[0], mu, nesterov, keep, coef, steps, eps);
+            else if (accurate) hipLaunchKernelGGL((k_fit_muon<true, T>), dim3(many), dim3(64 * FIT_WAVES), 0, st, tabs[1], mu, nesterov, keep, coef, steps, eps);
+            else hipLaunchKernelGGL((k_fit_muon<false, T>), dim3(many), dim3(64 * FIT_WAVES), 0, st, tabs[1], mu, nesterov, keep, coef, steps, eps);
             DPD_LAUNCH_CHECK();
             return DPD_OK;
         };
@@ -644,7 +885,8 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
             if (rows == 0 || cols == 0) continue;
             auto factor_of = [&](int k) { return (float)(lr * sqrt(h_rows[k] > h_cols[k] ? (double)h_rows[k] / (double)h_cols[k] : 1.0)); };
             const float factor = factor_of(i);
-            if (!is_small(rows, cols)) {
+            const int kind = is_small(rows, cols) ? 0 : fits(rows, cols, accurate != 0) ? 1 : 2;
+            if (kind == 2) {
                 Set s;
                 if (!leads_set(i, n, h_rows, h_cols, accurate, &s)) continue;          // went with an earlier one
                 FromMomenta<T> from{{}, {}, mu, nesterov, 0, 0};
@@ -662,10 +904,13 @@ extern "C" int dpd_muon_step(int n, void *const *h_p, const void *const *h_g, fl
                 if (rc) return rc;
                 continue;
             }
-            tab.p[used] = h_p[i], tab.g[used] = h_g[i], tab.m[used] = h_m[i], tab.rows[used] = (int)rows, tab.cols[used] = (int)cols, tab.factor[used] = factor;
-            if (++used == TABLE)
-                if (const int rc = flush()) return rc;
+            SmallTable &tab = tabs[kind];
+            const int at = used[kind]++;
+            tab.p[at] = h_p[i], tab.g[at] = h_g[i], tab.m[at] = h_m[i], tab.rows[at] = (int)rows, tab.cols[at] = (int)cols, tab.factor[at] = factor;
+            if (at + 1 == TABLE)
+                if (const int rc = flush(kind)) return rc;
         }
-        return flush();
+        const int rc = flush(0);
+        return rc ? rc : flush(1);
     });
 }

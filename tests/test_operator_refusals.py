@@ -99,7 +99,8 @@ def test_workspace_sizes():
     lib = L.lib()
     assert lib.dpd_int8_row_bytes(1) == 128 and lib.dpd_int8_row_bytes(128) == 128 and lib.dpd_int8_row_bytes(129) == 256
     assert lib.dpd_orthogonalize_workspace_bytes(1, 64, 128, 1) == 256                    # runs without one
-    assert lib.dpd_orthogonalize_workspace_bytes(1, 65, 128, 0) > 256
+    assert lib.dpd_orthogonalize_workspace_bytes(1, 128, 129, 0) == 256 and lib.dpd_orthogonalize_workspace_bytes(1, 129, 129, 0) > 256
+    assert lib.dpd_orthogonalize_workspace_bytes(1, 64, 512, 1) == 256 and lib.dpd_orthogonalize_workspace_bytes(1, 64, 640, 1) > 256
     assert lib.dpd_orthogonalize_workspace_bytes(2, 4096, 4096, 1) > lib.dpd_orthogonalize_workspace_bytes(2, 4096, 4096, 0) > 2 * 4096 * 4096 * 10
     assert lib.dpd_int8_linear_backward_workspace_bytes(10, 10, 10, 0, 0, 0, 0) == 256
 
