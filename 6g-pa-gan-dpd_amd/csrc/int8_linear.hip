@@ -654,23 +654,22 @@ extern "C" int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, in
     DPD_REQUIRE(x && qw && w_scale && out, DPD_ERR_INVALID_ARG, "int8_linear: null pointer");
     DPD_REQUIRE(ldx >= K && ldo >= N, DPD_ERR_INVALID_ARG, "int8_linear: row stride");
     DPD_REQUIRE(((uintptr_t)qw & 15) == 0, DPD_ERR_INVALID_ARG, "int8_linear: the weight image is 16-byte aligned");
-    DPD_REQUIRE(ws && ws_bytes >= dpd_int8_linear_workspace_bytes(M, N, K), DPD_ERR_WORKSPACE, "int8_linear: workspace");
     const int64_t ld = nt::pad_to(K, 128);
-    float *sx = (float *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
-    int8_t *qx = (int8_t *)sx + nt::pad_to(M * 4, 256);
+    // a workgroup of four waves: 16 channels each fill the chip from 4096 channels on; with fewer, and long rows, 16 waves
+    const bool tall = N < 2048 && ld >= 2048;
     hipStream_t st = as_stream(stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const T *xt = (const T *)x;
+        constexpr int V = 16 / sizeof(T);
+        const int vec = fused_pieces(xt, M, K, ldx, ld, tall ? 1024 : 256);
+        const bool enough = ws && ws_bytes >= dpd_int8_linear_workspace_bytes(M, N, K);
+        DPD_REQUIRE(vec || enough, DPD_ERR_WORKSPACE, "int8_linear: workspace");
+        float *sx = (float *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+        int8_t *qx = (int8_t *)sx + nt::pad_to(M * 4, 256);
         const ScaleOut<T> epi{sx, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
-        // a workgroup of four waves: 16 channels each fill the chip from 4096 channels on; with fewer, and long rows, 16 waves
-        const bool tall = N < 2048 && ld >= 2048;
-        if (M <= 16) {
-            constexpr int V = 16 / sizeof(T);
-            const int vec = fused_pieces(xt, M, K, ldx, ld, tall ? 1024 : 256);
-            if (vec == V) return tall ? few_tokens<T, 16, 1, V>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, V>(xt, M, K, ldx, qx, ld, qw, epi, st);
-            if (vec == 1) return tall ? few_tokens<T, 16, 1, 1>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, 1>(xt, M, K, ldx, qx, ld, qw, epi, st);
-        }
+        if (vec == V) return tall ? few_tokens<T, 16, 1, V>(xt, M, K, ldx, nullptr, ld, qw, epi, st) : few_tokens<T, 4, 1, V>(xt, M, K, ldx, nullptr, ld, qw, epi, st);
+        if (vec == 1) return tall ? few_tokens<T, 16, 1, 1>(xt, M, K, ldx, nullptr, ld, qw, epi, st) : few_tokens<T, 4, 1, 1>(xt, M, K, ldx, nullptr, ld, qw, epi, st);
         const int rc = quantize_rows(xt, M, (int)K, ldx, qx, ld, sx, st);
         if (rc) return rc;
         if (M <= 16) return tall ? few_tokens<T, 16, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);

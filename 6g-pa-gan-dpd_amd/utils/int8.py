@@ -13,6 +13,7 @@ from torch.autograd.function import once_differentiable
 from .. import _lib as L
 
 TYPES = L.TYPES
+_NEEDS_WORKSPACE = 4            # DPD_ERR_WORKSPACE
 
 
 def _type(t: torch.Tensor, what: str) -> int:
@@ -210,7 +211,8 @@ class Int8Inference:
         bc, self._bias_type = _check_bias(b, n, w.device)
         self.bias = None if bc is None else bc.detach().clone()
         self._w = (self.image.data_ptr(), self.scale.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
-        self._fn = L.lib().dpd_int8_linear
+        self._fn = L.entry("dpd_int8_linear")
+        self._index = self.device.index
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [..., K] -> [..., N] in the type of x.  `out` (optional: [..., N], contiguous, the type of x, apart from x in
@@ -232,10 +234,15 @@ class Int8Inference:
             raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {(*shape[:-1], n)} on {x.device} without gradient")
         elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise RuntimeError("out must not share memory with x")
-        nbytes = m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256                # dpd_int8_linear_workspace_bytes
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         qw, sw, b = self._w
         with L.device(x):
-            L.check(self._fn(x2.data_ptr(), t, m, k, ldx, qw, sw, b, self._bias_type, n, out.data_ptr(), n, ws.data_ptr(), nbytes,
-                             L.raw_stream(self.device.index)))
+            args = (x2.data_ptr(), t, m, k, ldx, qw, sw, b, self._bias_type, n, out.data_ptr(), n)
+            stream = L.raw_stream(self._index)
+            rc = self._fn(*args, 0, 0, stream) if m <= 16 else _NEEDS_WORKSPACE
+            if rc == _NEEDS_WORKSPACE:       # the tokens are quantised by a launch of their own
+                nbytes = m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256        # dpd_int8_linear_workspace_bytes
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+                rc = self._fn(*args, ws.data_ptr(), nbytes, stream)
+            if rc:
+                L.check(rc)
         return out
