@@ -152,19 +152,23 @@ struct PlainOut {
     DEV void put(int, int m, int n, float *v, Row, Col, Pre) const { store8(out + (int64_t)m * ldo + n, v, N - n, whole); }
 };
 
-// Few tokens: a workgroup owns 16 output channels and reads their weights once, straight into the fragments of the
-// matrix instruction (64 bytes of 16 rows a load; the waves take the 64-byte steps of the rows in turn and are joined in
-// LDS: integer sums, so the order does not matter).  TB blocks of 16 tokens share the weight fragments; a token row beyond
-// the last one repeats it.  VEC > 0: the tokens are quantised here, VEC elements a piece, by every workgroup for itself,
-// while its first weights are on their way; VEC == 0: they come quantised.  Bound by the read of the weights and by latency.
+// Few tokens (at most 16): a workgroup owns 16 output channels, quantises the tokens for itself, VEC elements a piece,
+// while its first weights are on their way, and reads those weights once, straight into the fragments of the matrix
+// instruction (64 bytes of 16 rows a load; the waves take the 64-byte steps of the rows in turn and are joined in LDS: integer
+// sums, so the order does not matter).  A token row beyond the last one repeats it.  One launch, bound by the read of the
+// weights and by latency: 1 token of 4096 x 4096 bf16 7.9 us (2.1 TB/s), of 16384 x 4096 17.0 us (3.9 TB/s).
 constexpr int FEW_HELD = 8;                             // pieces of the tokens that a thread quantises
 
-template <class T, int WAVES, int TB, int VEC>
-__global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T *__restrict__ x, int64_t ldx, int cols, const int8_t *__restrict__ qx, int64_t ld, int M,
-                                                           const int8_t *__restrict__ qw, ScaleOut<T> epi) {
+template <class T, int WAVES, int VEC>
+__global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T *__restrict__ x, int64_t ldx, int cols, int64_t ld, int M, const int8_t *__restrict__ qw,
+                                                           ScaleOut<T> epi) {
     constexpr int U = 8;                                // steps of a wave in flight
+    typedef T TV __attribute__((ext_vector_type(VEC)));
+    typedef int8_t QV __attribute__((ext_vector_type(VEC)));
     extern __shared__ __attribute__((aligned(16))) char few_lds[];
-    nt::i32x4 *part = (nt::i32x4 *)few_lds;             // [WAVES][TB][64]
+    nt::i32x4 *part = (nt::i32x4 *)few_lds;             // [WAVES][64]
+    unsigned *tops = (unsigned *)(few_lds + WAVES * 1024);              // [16]
+    int8_t *mine = (int8_t *)(tops + 16);                               // [M][ld]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16, steps = (int)(ld / 64);
     const int8_t *wr = qw + (int64_t)min(n0 + r, epi.N - 1) * ld + q * 16;
@@ -177,64 +181,50 @@ __global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T *__restrict__
         }
     };
     fetch(0);
-    float scale_of_mine = 0.f;
-    const int8_t *tok[TB];
-    if constexpr (VEC > 0) {
-        typedef T TV __attribute__((ext_vector_type(VEC > 0 ? VEC : 1)));
-        typedef int8_t QV __attribute__((ext_vector_type(VEC > 0 ? VEC : 1)));
-        unsigned *tops = (unsigned *)(few_lds + WAVES * TB * 1024);     // [16]
-        int8_t *mine = (int8_t *)(tops + 16);                           // [M][ld]
-        const int pieces = cols / VEC, total = M * pieces;
-        if (threadIdx.x < 16) tops[threadIdx.x] = 0;
-        for (int i = threadIdx.x; i < M * (int)(ld - cols); i += 64 * WAVES) {      // zeros behind the rows
-            const int m = i / (int)(ld - cols);
-            mine[m * ld + cols + i - m * (int)(ld - cols)] = 0;
-        }
-        TV v[FEW_HELD];
-        int row[FEW_HELD];
-#pragma unroll
-        for (int h = 0; h < FEW_HELD; ++h) {
-            const int e = min((int)threadIdx.x + h * 64 * WAVES, total - 1);        // behind the last piece: again, harmless
-            row[h] = e / pieces;
-            v[h] = *(const TV *)(x + row[h] * ldx + (int64_t)(e - row[h] * pieces) * VEC);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < FEW_HELD; ++h) {
-            if (h * 64 * WAVES >= total) break;
-            unsigned top = 0;
-#pragma unroll
-            for (int e = 0; e < (VEC > 0 ? VEC : 1); ++e) top = max(top, abs_bits(to_f32(v[h][e])));
-            const int first = __builtin_amdgcn_readfirstlane(row[h]);
-            if (__all(row[h] == first)) {
-                top = wave_umax(top);
-                if (lane == 0) atomicMax(tops + first, top);
-            } else {
-                atomicMax(tops + row[h], top);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < FEW_HELD; ++h) {
-            const int e = (int)threadIdx.x + h * 64 * WAVES;
-            if (e >= total) break;
-            const unsigned top = tops[row[h]];
-            const float s = row_scale(top), inv = 1.0f / s;
-            QV o;
-#pragma unroll
-            for (int k = 0; k < (VEC > 0 ? VEC : 1); ++k) o[k] = top < 0x7f800000u ? (int8_t)quantise(to_f32(v[h][k]), s, inv) : (int8_t)0;
-            *(QV *)(mine + row[h] * ld + (e - row[h] * pieces) * VEC) = o;
-        }
-        __syncthreads();
-        scale_of_mine = row_scale(tops[min(r, M - 1)]);
-        tok[0] = mine + min(r, M - 1) * ld + q * 16;
-    } else {
-#pragma unroll
-        for (int b = 0; b < TB; ++b) tok[b] = qx + (int64_t)min(b * 16 + r, M - 1) * ld + q * 16;
+    const int pieces = cols / VEC, total = M * pieces;
+    if (threadIdx.x < 16) tops[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < M * (int)(ld - cols); i += 64 * WAVES) {          // zeros behind the rows
+        const int m = i / (int)(ld - cols);
+        mine[m * ld + cols + i - m * (int)(ld - cols)] = 0;
     }
-    nt::i32x4 acc[TB];
+    TV v[FEW_HELD];
+    int row[FEW_HELD];
 #pragma unroll
-    for (int b = 0; b < TB; ++b) acc[b] = nt::i32x4{0, 0, 0, 0};
+    for (int h = 0; h < FEW_HELD; ++h) {
+        const int e = min((int)threadIdx.x + h * 64 * WAVES, total - 1);            // behind the last piece: again, harmless
+        row[h] = e / pieces;
+        v[h] = *(const TV *)(x + row[h] * ldx + (int64_t)(e - row[h] * pieces) * VEC);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < FEW_HELD; ++h) {
+        if (h * 64 * WAVES >= total) break;
+        unsigned top = 0;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(v[h][e])));
+        const int first = __builtin_amdgcn_readfirstlane(row[h]);
+        if (__all(row[h] == first)) {
+            top = wave_umax(top);
+            if (lane == 0) atomicMax(tops + first, top);
+        } else {
+            atomicMax(tops + row[h], top);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < FEW_HELD; ++h) {
+        const int e = (int)threadIdx.x + h * 64 * WAVES;
+        if (e >= total) break;
+        const unsigned top = tops[row[h]];
+        const float s = row_scale(top), inv = 1.0f / s;
+        QV o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o[k] = top < 0x7f800000u ? (int8_t)quantise(to_f32(v[h][k]), s, inv) : (int8_t)0;
+        *(QV *)(mine + row[h] * ld + (e - row[h] * pieces) * VEC) = o;
+    }
+    __syncthreads();
+    const int8_t *tok = mine + min(r, M - 1) * ld + q * 16;
+    nt::i32x4 acc = {0, 0, 0, 0};
     for (int i = 0; i * WAVES < steps; i += U) {
         nt::i32x4 now[U];
 #pragma unroll
@@ -242,43 +232,47 @@ __global__ __launch_bounds__(64 * WAVES) void k_few_tokens(const T *__restrict__
         if ((i + U) * WAVES < steps) fetch(i + U);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int s = min((i + u) * WAVES + wave, steps - 1);         // behind the last step the weights are zeros
-#pragma unroll
-            for (int b = 0; b < TB; ++b) acc[b] = nt::mfma<nt::I8>(now[u], *(const nt::i32x4 *)(tok[b] + (int64_t)s * 64), acc[b]);
+            const int s = min((i + u) * WAVES + wave, steps - 1);                   // behind the last step the weights are zeros
+            acc = nt::mfma<nt::I8>(now[u], *(const nt::i32x4 *)(tok + (int64_t)s * 64), acc);
         }
     }
-#pragma unroll
-    for (int b = 0; b < TB; ++b) part[(wave * TB + b) * 64 + lane] = acc[b];
+    part[wave * 64 + lane] = acc;
     __syncthreads();
-    if (wave >= TB) return;                             // wave b finishes token block b
-    nt::i32x4 sum = nt::i32x4{0, 0, 0, 0};
+    if (wave > 0) return;
 #pragma unroll
-    for (int k = 0; k < WAVES; ++k) sum += part[(k * TB + wave) * 64 + lane];
-    const int m = wave * 16 + r, n = n0 + q * 4;
-    if (m >= M || n >= epi.N) return;
-    const float s = VEC > 0 ? scale_of_mine : epi.sa[m];
+    for (int k = 1; k < WAVES; ++k) acc += part[k * 64 + lane];
+    const int n = n0 + q * 4;
+    if (r >= M || n >= epi.N) return;
+    const float s = row_scale(tops[r]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (n + e < epi.N) {
-            float v = (float)sum[e] * s * epi.sb[n + e];
-            if (epi.bias) v += load_any(epi.bias, epi.bias_type, n + e);
-            epi.out[(int64_t)m * epi.ldo + n + e] = from_f32<T>(v);
+            float y = (float)acc[e] * s * epi.sb[n + e];
+            if (epi.bias) y += load_any(epi.bias, epi.bias_type, n + e);
+            epi.out[(int64_t)r * epi.ldo + n + e] = from_f32<T>(y);
         }
 }
 
-// Pieces of the tokens for one workgroup: 0 if it should get them quantised.
+// Whether the tokens go through k_few_tokens, with how many waves and in what pieces.  Measured with 2 and more tokens, us,
+// one launch against the quantiser and a tiled product: 4096 x 4096, 2 tokens 8.2 against 9.6 and 4 tokens 9.7 against 9.7
+// (16 waves; 4 waves 10.4 and 13.6); 16384 x 4096, 2 tokens 16.7 against 17.5 and 4 tokens 21.3 against 16.9; 1024 x 8192,
+// 1 token 8.8 (16 waves) against 11.1.  4 waves are better for short rows: 2048 x 2048, 1 token 4.5 against 6.1 with 16.
+struct FewPlan {
+    int waves, vec;                                     // 0: no
+};
 template <class T>
-int fused_pieces(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, int threads) {
+FewPlan few_plan(const T *x, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ld) {
     constexpr int V = 16 / sizeof(T);
-    if (M > 16 || M * ld > 32768) return 0;
-    const bool vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && K % V == 0;
-    return M * (K / (vec ? V : 1)) <= (int64_t)FEW_HELD * threads ? (vec ? V : 1) : 0;
+    const int waves = ld >= 4096 && N <= 8192 ? 16 : 4;
+    if (M > 16 || M * ld > (waves == 16 ? 8192 : 4096)) return {0, 0};
+    const int vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && K % V == 0 ? V : 1;
+    return M * (K / vec) <= (int64_t)FEW_HELD * 64 * waves ? FewPlan{waves, vec} : FewPlan{0, 0};
 }
 
-template <class T, int WAVES, int TB, int VEC>
-int few_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, const int8_t *qx, int64_t ld, const int8_t *qw, const ScaleOut<T> &epi, hipStream_t st) {
-    const size_t lds = WAVES * TB * 1024 + (VEC ? 64 + M * ld : 0);
-    hipLaunchKernelGGL((k_few_tokens<T, WAVES, TB, VEC>), dim3((unsigned)((epi.N + 15) / 16)), dim3(64 * WAVES), lds, st, x, ldx, (int)K, qx, ld, (int)M, qw, epi);
+template <class T, int WAVES, int VEC>
+int few_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, const int8_t *qw, const ScaleOut<T> &epi, hipStream_t st) {
+    hipLaunchKernelGGL((k_few_tokens<T, WAVES, VEC>), dim3((unsigned)((epi.N + 15) / 16)), dim3(64 * WAVES), (size_t)(WAVES * 1024 + 64 + M * ld), st, x, ldx,
+                       (int)K, ld, (int)M, qw, epi);
     DPD_LAUNCH_CHECK();
     return DPD_OK;
 }
@@ -655,27 +649,22 @@ extern "C" int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, in
     DPD_REQUIRE(ldx >= K && ldo >= N, DPD_ERR_INVALID_ARG, "int8_linear: row stride");
     DPD_REQUIRE(((uintptr_t)qw & 15) == 0, DPD_ERR_INVALID_ARG, "int8_linear: the weight image is 16-byte aligned");
     const int64_t ld = nt::pad_to(K, 128);
-    // a workgroup of four waves: 16 channels each fill the chip from 4096 channels on; with fewer, and long rows, 16 waves
-    const bool tall = N < 2048 && ld >= 2048;
     hipStream_t st = as_stream(stream);
     return with_type(type, [&](auto t) {
         using T = decltype(t);
         const T *xt = (const T *)x;
         constexpr int V = 16 / sizeof(T);
-        const int vec = fused_pieces(xt, M, K, ldx, ld, tall ? 1024 : 256);
-        const bool enough = ws && ws_bytes >= dpd_int8_linear_workspace_bytes(M, N, K);
-        DPD_REQUIRE(vec || enough, DPD_ERR_WORKSPACE, "int8_linear: workspace");
+        const FewPlan few = few_plan(xt, M, N, K, ldx, ld);
+        if (few.waves) {
+            const ScaleOut<T> epi{nullptr, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
+            if (few.waves == 16) return few.vec == V ? few_tokens<T, 16, V>(xt, M, K, ldx, ld, qw, epi, st) : few_tokens<T, 16, 1>(xt, M, K, ldx, ld, qw, epi, st);
+            return few.vec == V ? few_tokens<T, 4, V>(xt, M, K, ldx, ld, qw, epi, st) : few_tokens<T, 4, 1>(xt, M, K, ldx, ld, qw, epi, st);
+        }
+        DPD_REQUIRE(ws && ws_bytes >= dpd_int8_linear_workspace_bytes(M, N, K), DPD_ERR_WORKSPACE, "int8_linear: workspace");
         float *sx = (float *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
         int8_t *qx = (int8_t *)sx + nt::pad_to(M * 4, 256);
-        const ScaleOut<T> epi{sx, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
-        if (vec == V) return tall ? few_tokens<T, 16, 1, V>(xt, M, K, ldx, nullptr, ld, qw, epi, st) : few_tokens<T, 4, 1, V>(xt, M, K, ldx, nullptr, ld, qw, epi, st);
-        if (vec == 1) return tall ? few_tokens<T, 16, 1, 1>(xt, M, K, ldx, nullptr, ld, qw, epi, st) : few_tokens<T, 4, 1, 1>(xt, M, K, ldx, nullptr, ld, qw, epi, st);
         const int rc = quantize_rows(xt, M, (int)K, ldx, qx, ld, sx, st);
-        if (rc) return rc;
-        if (M <= 16) return tall ? few_tokens<T, 16, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 1, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
-        if (M <= 32) return tall ? few_tokens<T, 16, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 2, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
-        if (M <= 64) return tall ? few_tokens<T, 16, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st) : few_tokens<T, 4, 4, 0>(xt, M, K, ldx, qx, ld, qw, epi, st);
-        return int8_product(qx, ld, sx, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
+        return rc ? rc : int8_product(qx, ld, sx, qw, ld, w_scale, bias, bias_type, M, N, ld, (T *)out, ldo, st);
     });
 }
 

@@ -383,8 +383,8 @@ int dpd_int8_matmul(const int8_t *a, int64_t lda, const float *a_scale, const in
 
 /* Tokens x [M, K] against a weight image: dpd_quantize_rows_int8 of x and dpd_int8_matmul in one call, out in the type of
  * x.  qw: [N, dpd_int8_row_bytes(K)] int8, 16-byte aligned, as dpd_quantize_rows_int8 writes it with that ldq.  Up to 16
- * tokens of together at most 2048 elements (16384 bytes where rows are 16-byte aligned) need no workspace: ws may be NULL
- * then, and DPD_ERR_WORKSPACE, before anything is launched, says that one is needed. */
+ * tokens that together have few elements need no workspace: ws may be NULL then, and DPD_ERR_WORKSPACE, before anything is
+ * launched, says that one is needed. */
 int64_t dpd_int8_row_bytes(int64_t K);
 size_t dpd_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, int64_t ldx, const int8_t *qw, const float *w_scale,
