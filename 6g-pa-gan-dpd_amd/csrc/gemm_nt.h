@@ -109,7 +109,7 @@ DEV void tile_of(const Args &g, int id, int n_tiles, int *tm, int *tn) {
         return;
     }
 }
-static inline int tiles_of(const Args &g) { return g.lower ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n; }
+static inline int64_t tiles_of(const Args &g) { return g.lower ? (int64_t)g.tiles_m * (g.tiles_m + 1) / 2 : (int64_t)g.tiles_m * g.tiles_n; }
 
 // Row of a tile that lane r (0..15) of block j of the B operand stands for: blocks 2q and 2q + 1 share 32 rows.
 DEV int b_row(int j, int r) { return (j >> 1) * 32 + (r >> 2) * 8 + (j & 1) * 4 + (r & 3); }
@@ -424,7 +424,9 @@ template <int KIND, int BM, int BN, int WAVES_M, int WAVES_N, int WAVES_K, int S
 static int launch(Args g, int batch, const Epilogue &epi, hipStream_t st) {
     g.tiles_m = (g.M + BM - 1) / BM;
     g.tiles_n = (g.N + BN - 1) / BN;
-    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, WAVES_K, STAGES, Epilogue>), dim3((unsigned)tiles_of(g), 1, (unsigned)batch),
+    const int64_t tiles = tiles_of(g);
+    DPD_REQUIRE(tiles * 64 * WAVES_M * WAVES_N * WAVES_K <= UINT32_MAX, DPD_ERR_SHAPE, "a product of %d x %d results is too large for one call", g.M, g.N);
+    hipLaunchKernelGGL((k_gemm<KIND, BM, BN, WAVES_M, WAVES_N, WAVES_K, STAGES, Epilogue>), dim3((unsigned)tiles, 1, (unsigned)batch),
                        dim3(64 * WAVES_M * WAVES_N * WAVES_K), 0, st, g, epi);
     DPD_LAUNCH_CHECK();
     return DPD_OK;
@@ -464,7 +466,7 @@ static inline int best_tile(const Args &g, int batch, bool split) {
         if ((g.lower && t.bm != t.bn) || one.per == 0.f) continue;
         Args a = g;
         a.tiles_m = (g.M + t.bm - 1) / t.bm, a.tiles_n = (g.N + t.bn - 1) / t.bn;
-        const int64_t tiles = (int64_t)tiles_of(a) * batch, size = two.per > 0.f ? 512 : 256, rest = tiles % size;
+        const int64_t tiles = tiles_of(a) * batch, size = two.per > 0.f ? 512 : 256, rest = tiles % size;
         const float c1 = (float)g.steps * one.per + one.fixed, c2 = (float)g.steps * two.per + two.fixed;
         const float cost = (float)(tiles / size) * (size == 512 ? c2 : c1) + (rest == 0 ? 0.f : rest > 256 ? c2 : c1);
         if (best < 0 || cost < least) best = i, least = cost;

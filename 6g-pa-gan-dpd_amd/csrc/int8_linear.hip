@@ -96,8 +96,13 @@ int quantize_rows(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *q, in
     constexpr int V = 16 / sizeof(T);
     const bool vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && cols % V == 0 && ((uintptr_t)q & 15) == 0 && ldq % V == 0;
     auto go = [&](auto kernel, int rows_per_block) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + rows_per_block - 1) / rows_per_block)), dim3(256), 0, st, x, rows, cols, ldx, q, ldq, scale);
-        DPD_LAUNCH_CHECK();
+        constexpr int64_t MOST = 1 << 22;              // rows a launch: a grid has fewer than 2^32 threads
+        for (int64_t r = 0; r < rows; r += MOST) {
+            const int64_t n = rows - r < MOST ? rows - r : MOST;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows_per_block - 1) / rows_per_block)), dim3(256), 0, st, x + r * ldx, n, cols, ldx, q + r * ldq,
+                               ldq, scale + r);
+            DPD_LAUNCH_CHECK();
+        }
         return DPD_OK;
     };
     if (vec) return cols <= 1024 ? go(k_quantize_rows<T, 64, V>, 4) : go(k_quantize_rows<T, 256, V>, 1);
@@ -518,7 +523,7 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
     const Turn tw = turn(gx, qw, N, ldqw, direct ? sw : nullptr, wt, p.n_pad), tx = turn(gw, qx, M, ldqx, nullptr, xt, p.m_pad);
     const int bx = gs || gt || part ? (int)(p.m_pad / 64) : 0, by = (int)(p.n_pad / 64);
     const int64_t blocks = (int64_t)bx * by + (int64_t)tw.bx * tw.by + (int64_t)tx.bx * tx.by;
-    DPD_REQUIRE(blocks <= INT32_MAX, DPD_ERR_SHAPE, "int8_linear_backward: %lld x %lld gradients are too many for one call", (long long)M, (long long)N);
+    DPD_REQUIRE(blocks * 256 <= UINT32_MAX, DPD_ERR_SHAPE, "int8_linear_backward: %lld x %lld gradients are too many for one call", (long long)M, (long long)N);
     hipLaunchKernelGGL((k_backward_images<T>), dim3((unsigned)blocks), dim3(256), 0, st, g, M, (int)N, ldg, whole8(g, ldg), sw, sx, gs, p.n_pad, gt,
                        p.m_pad, part, bx, by, tw, tx);
     DPD_LAUNCH_CHECK();

@@ -771,26 +771,22 @@ extern "C" int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t
     hipStream_t st = as_stream(stream);
     Coef coef{};
     for (int i = 0; i < 3 * steps; ++i) coef.v[i] = h_coef[i];
-    if (is_small(rows, cols))
+    const bool small = is_small(rows, cols);
+    if (small || fits(rows, cols, accurate != 0))
         return with_type(type, [&](auto t) {
             using T = decltype(t);
-            const FromTensor<T> from{(const T *)x, rows * cols, false, rows <= cols};
-            const ToTensor<T> to{(T *)out, rows * cols, false};
-            if (needs_16_waves(rows, cols))
-                hipLaunchKernelGGL((k_small<16, T>), dim3((unsigned)batch), dim3(1024), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
-            else
-                hipLaunchKernelGGL((k_small<4, T>), dim3((unsigned)batch), dim3(256), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
-            DPD_LAUNCH_CHECK();
-            return DPD_OK;
-        });
-    if (fits(rows, cols, accurate != 0))
-        return with_type(type, [&](auto t) {
-            using T = decltype(t);
-            const FromTensor<T> from{(const T *)x, rows * cols, false, rows <= cols};
-            const ToTensor<T> to{(T *)out, rows * cols, false};
-            if (accurate) hipLaunchKernelGGL((k_fit<true, T>), dim3((unsigned)batch), dim3(64 * FIT_WAVES), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
-            else hipLaunchKernelGGL((k_fit<false, T>), dim3((unsigned)batch), dim3(64 * FIT_WAVES), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps);
-            DPD_LAUNCH_CHECK();
+            constexpr int64_t MOST = 1 << 20;          // matrices a launch: a grid has fewer than 2^32 threads
+            for (int64_t z = 0; z < batch; z += MOST) {
+                const FromTensor<T> from{(const T *)x + z * rows * cols, rows * cols, false, rows <= cols};
+                const ToTensor<T> to{(T *)out + z * rows * cols, rows * cols, false};
+                const dim3 many((unsigned)(batch - z < MOST ? batch - z : MOST));
+                auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, many, dim3(threads), 0, st, from, to, (int)rows, (int)cols, coef, steps, eps); };
+                if (small && needs_16_waves(rows, cols)) go(k_small<16, T>, 1024);
+                else if (small) go(k_small<4, T>, 256);
+                else if (accurate) go(k_fit<true, T>, 64 * FIT_WAVES);
+                else go(k_fit<false, T>, 64 * FIT_WAVES);
+                DPD_LAUNCH_CHECK();
+            }
             return DPD_OK;
         });
     DPD_REQUIRE(batch <= 65535, DPD_ERR_SHAPE, "orthogonalize: %lld matrices of this size in one call (at most 65535)", (long long)batch);

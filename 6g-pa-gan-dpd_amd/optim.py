@@ -21,7 +21,7 @@ class Muon(torch.optim.Optimizer):
     Parameters that are not matrices (biases) are updated by torch's Adam with the options in `adam`; both kinds are groups
     of this optimiser, so schedulers and state_dict() cover them.  `params`: tensors, or groups with options of their own.
     The steps of all matrices of up to 64 x 128 take one launch (24 at a time); larger ones a handful each.  Every result is
-    the same in every run."""
+    the same in every run.  A step that is captured into a graph keeps the learning rate it was captured with."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients: Coefficients = COEFFICIENTS, eps: float = 1e-7, accurate: Optional[bool] = None, adam: Optional[Dict] = None):
@@ -34,18 +34,20 @@ class Muon(torch.optim.Optimizer):
                         coefficients=coefficients, eps=eps, accurate=accurate)
         params = list(params)
         given = params if params and isinstance(params[0], dict) else [{"params": params}]
-        groups, others = [], []
+        groups, others, seen = [], [], set()
         for g in given:
             ps = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            if len({id(p) for p in ps} | seen) != len(ps) + len(seen):
+                raise ValueError("a parameter is given twice: its update would run twice at once")
+            seen |= {id(p) for p in ps}
             rest = {k: v for k, v in g.items() if k != "params"}
             matrices = [p for p in ps if p.dim() == 2]
             if matrices:
                 groups.append({**rest, "params": matrices, "kind": "matrix"})
             others += [p for p in ps if p.dim() != 2]
-        self._adam = None
         if others:
-            self._adam = torch.optim.Adam(others, **(adam if adam is not None else dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True)))
-            groups += [{**g, "kind": "other"} for g in self._adam.param_groups]
+            options = torch.optim.Adam(others, **(adam if adam is not None else dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True)))
+            groups += [{**g, "kind": "other"} for g in options.param_groups]
         super().__init__(groups, defaults)
 
     def load_state_dict(self, state_dict):
@@ -70,8 +72,11 @@ class Muon(torch.optim.Optimizer):
             else:
                 others.append(group)
         if others:
-            self._adam.param_groups, self._adam.state = others, self.state     # the groups and the state are this optimiser's
-            self._adam.step()
+            adam = getattr(self, "_adam", None)
+            if adam is None:
+                adam = self._adam = torch.optim.Adam([p for g in others for p in g["params"]])
+            adam.param_groups, adam.state = others, self.state                 # the groups and the state are this optimiser's
+            adam.step()
         return loss
 
     def _matrices(self, group):
@@ -90,6 +95,8 @@ class Muon(torch.optim.Optimizer):
             own = state[p]
             m = own.get("momentum_buffer")
             if m is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the first step of a weight makes its momentum: take one before the capture, a replay would clear it each time")
                 m = own["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
             elif m.dtype != torch.float32 or m.shape != p.shape or not m.is_contiguous() or m.device != device:
                 raise RuntimeError(f"the momentum of a weight must be a contiguous float32 tensor of its shape on {device}, got {m.dtype} {tuple(m.shape)}")

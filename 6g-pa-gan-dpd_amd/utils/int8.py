@@ -156,7 +156,10 @@ class _Int8LinearFn(torch.autograd.Function):
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q(x) q(weight)^T + bias in the type of x, both factors quantised by rows in this call; differentiable in x, weight
-    and bias with the straight-through estimator (the quantisers count as the identity).  x [..., K], weight [N, K]."""
+    and bias with the straight-through estimator (the quantisers count as the identity).  x [..., K], weight [N, K].
+
+    What a graph captures: the pass may be captured together with its gradients; as with every torch module, an eager graph of
+    the same leaf tensors must not be alive then (let go of earlier losses first, or use torch.autograd.grad)."""
     L.need_gpu(x, weight, bias)
     _type(x, "x")
     _type(weight, "weight")
@@ -226,13 +229,15 @@ class Int8Inference:
             raise ValueError(f"expected {k} input features, got {tuple(shape)}")
         if x.device != self.device:
             raise RuntimeError(f"the weights are on {self.device}, the tokens on {x.device}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Int8Inference has no gradient: pass a detached tensor, or train with Int8Linear")
         x2, ldx = _rows(x)
         m = x2.shape[0]
         if out is None:
             out = torch.empty((*shape[:-1], n), dtype=x.dtype, device=self.device)
         elif out.shape != (*shape[:-1], n) or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device or out.requires_grad:
             raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {(*shape[:-1], n)} on {x.device} without gradient")
-        elif out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+        elif out.numel() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
             raise RuntimeError("out must not share memory with x")
         qw, sw, b = self._w
         with L.device(x):

@@ -299,6 +299,9 @@ def test_serving_refusals():
         Int8Inference({"weight": q, "scale": s[:4]})
     with pytest.raises(RuntimeError):
         eng(x.cpu())
+    assert eng(torch.empty(0, x.shape[1], device=DEV), out=torch.empty(0, eng.out_features, device=DEV)).shape == (0, eng.out_features)
+    with pytest.raises(RuntimeError, match="gradient"):
+        eng(x.clone().requires_grad_(True))
     q.zero_()                                                             # the engine keeps a copy
     assert eng(x).abs().max() > 0
 

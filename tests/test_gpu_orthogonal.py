@@ -60,8 +60,9 @@ def test_iterate(r, c, dtype):
 @pytest.mark.parametrize("accurate", [False, True])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_both_forms_of_the_factors(dtype, accurate):
-    x = update(150, 220, 3).to(dtype)
-    check(orthogonalize(x.to(DEV), accurate=accurate), x, dtype, accurate)
+    for r, c in ((150, 220), (70, 100), (40, 400), (300, 33)):
+        x = update(r, c, 3).to(dtype)
+        check(orthogonalize(x.to(DEV), accurate=accurate), x, dtype, accurate)
 
 
 def test_batches_and_layouts():
@@ -213,6 +214,22 @@ def test_muon_groups_biases_and_state():
     assert all(torch.equal(a, b) for a, b in zip(net.parameters(), twin.parameters()))
 
 
+def test_muon_copies():
+    """A deep copy of the optimiser goes on by itself, biases included."""
+    torch.manual_seed(1)
+    net = torch.nn.Linear(20, 30).to(DEV)
+    opt = Muon(net.parameters(), adam=dict(lr=1e-2))
+    net(torch.ones(4, 20, device=DEV)).square().mean().backward()
+    opt.step()
+    twin = copy.deepcopy(opt)
+    mine, other = [p for g in opt.param_groups for p in g["params"]], [p for g in twin.param_groups for p in g["params"]]
+    for p, q in zip(mine, other):
+        q.grad = p.grad.clone()
+    opt.step()
+    twin.step()
+    assert all(torch.equal(p, q) and p.data_ptr() != q.data_ptr() for p, q in zip(mine, other))
+
+
 def test_muon_many_matrices_and_refusals():
     shapes = [(1 + i % 7, 3 + i % 11) for i in range(60)]                 # more than one launch's table
     ps = [torch.nn.Parameter(update(r, c, i).to(DEV)) for i, (r, c) in enumerate(shapes)]
@@ -261,6 +278,9 @@ def test_muon_in_a_graph():
     ps = [torch.nn.Parameter(update(r, c, r).to(DEV)) for r, c in ((30, 32), (140, 90))]
     for p in ps:
         p.grad = torch.zeros_like(p)
+    with pytest.raises(RuntimeError, match="momentum"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            Muon(ps).step()
     opt, eager_ps = Muon(ps), [torch.nn.Parameter(p.detach().clone()) for p in ps]
     eager = Muon(eager_ps)
     for o, q in ((opt, ps), (eager, eager_ps)):

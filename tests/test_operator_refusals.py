@@ -130,6 +130,9 @@ def test_muon_refusals_and_groups():
     net.weight.grad = torch.zeros_like(net.weight)
     with pytest.raises(RuntimeError, match="MI355X"):
         opt.step()
+    for twice in ([net.weight, net.weight], [{"params": [net.weight]}, {"params": [net.weight]}]):
+        with pytest.raises(ValueError, match="twice"):
+            Muon(twice)
     opt = Muon([{"params": [net.weight], "lr": 0.7}, {"params": net.bias}])
     assert opt.param_groups[0]["lr"] == 0.7 and opt.param_groups[1]["kind"] == "other"
 
