@@ -36,77 +36,110 @@ DEV int quantise(float x, float s, float inv) {
     return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
-// One row per TEAM threads (a wave, or the whole workgroup), VEC elements a piece: 16 bytes where the rows allow it, single
-// elements where not.  A thread keeps its first HELD pieces in registers between the two passes and reads the others
-// again.  Bound by memory: 2 + 1 bytes an element (bf16).
-template <class T, int TEAM, int VEC>
-__global__ __launch_bounds__(256) void k_quantize_rows(const T *__restrict__ x, int64_t rows, int cols, int64_t ldx,
-                                                       int8_t *__restrict__ q, int64_t ldq, float *__restrict__ scale) {
-    constexpr int HELD = VEC == 1 ? 8 : 4;
+// A row in the hands of TEAM threads, VEC elements a piece: a thread keeps its first HELD pieces in registers between the
+// search for the largest value and the quantisation, and reads the others again.
+template <class T, int TEAM, int VEC, int HELD>
+struct HeldRow {
     typedef T TV __attribute__((ext_vector_type(VEC)));
     typedef int8_t QV __attribute__((ext_vector_type(VEC)));
+    TV held[HELD];
+    DEV void load(const T *x, int pieces, int t) {
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) held[h] = ((const TV *)x)[min(t + h * TEAM, pieces - 1)];       // behind the row its last piece again
+    }
+    DEV unsigned top(const T *x, int pieces, int t) const {            // of this thread's pieces
+        unsigned top = 0;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(held[h][e])));
+        for (int i = t + HELD * TEAM; i < pieces; i += TEAM) {
+            const TV v = ((const TV *)x)[i];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(v[e])));
+        }
+        return top;
+    }
+    DEV float put(const T *x, int pieces, int t, unsigned top, int8_t *q, int all) const {     // `all` pieces with the zeros behind the row
+        const float s = row_scale(top), inv = 1.0f / s;
+        const bool fine = top < 0x7f800000u;
+        auto one = [&](int i, TV v) {
+            QV o;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = fine ? (int8_t)quantise(to_f32(v[e]), s, inv) : (int8_t)0;
+            ((QV *)q)[i] = o;
+        };
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if (t + h * TEAM < all) one(t + h * TEAM, t + h * TEAM < pieces ? held[h] : TV{});
+        for (int i = t + HELD * TEAM; i < all; i += TEAM) one(i, i < pieces ? ((const TV *)x)[i] : TV{});
+        return s;
+    }
+};
+
+// One row per TEAM threads (a wave, or the whole workgroup): 16 bytes a piece where the rows allow it, single elements where
+// not; the rows of two matrices where both factors of a layer are quantised.  Bound by memory: 2 + 1 bytes an element (bf16);
+// 8192 x 8192 bf16 takes 44 us (4.6 TB/s).
+template <class T>
+struct Rows {
+    const T *x;
+    int64_t rows, ldx;
+    int8_t *q;
+    int64_t ldq;
+    float *scale;
+};
+
+template <class T, int TEAM, int VEC>
+__global__ __launch_bounds__(256) void k_quantize_rows(Rows<T> a, Rows<T> b, int cols) {
     __shared__ unsigned top4[4];
     const int t = threadIdx.x % TEAM;
-    const int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
-    if (TEAM == 64 && row >= rows) return;
-    const TV *xr = (const TV *)(x + row * ldx);
+    int64_t row = (int64_t)blockIdx.x * (256 / TEAM) + threadIdx.x / TEAM;
+    if (TEAM == 64 && row >= a.rows + b.rows) return;
+    const bool second = row >= a.rows;
+    if (second) row -= a.rows;
+    const Rows<T> &m = second ? b : a;
+    const T *xr = m.x + row * m.ldx;
     const int pieces = cols / VEC;
-    unsigned top = 0;
-    TV held[HELD];
-#pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        const int i = t + h * TEAM;
-        held[h] = i < pieces ? xr[i] : TV{};
-    }
-#pragma unroll
-    for (int h = 0; h < HELD; ++h)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(held[h][e])));
-    for (int i = t + HELD * TEAM; i < pieces; i += TEAM) {
-        const TV v = xr[i];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) top = max(top, abs_bits(to_f32(v[e])));
-    }
-    top = wave_umax(top);
+    HeldRow<T, TEAM, VEC, VEC == 1 ? 8 : 4> r;
+    r.load(xr, pieces, t);
+    unsigned top = wave_umax(r.top(xr, pieces, t));
     if (TEAM == 256) {
         if ((threadIdx.x & 63) == 0) top4[threadIdx.x >> 6] = top;
         __syncthreads();
         top = max(max(top4[0], top4[1]), max(top4[2], top4[3]));
     }
-    const float s = row_scale(top);
-    const bool fine = top < 0x7f800000u;
-    const float inv = 1.0f / s;
-    QV *qr = (QV *)(q + row * ldq);
-    auto put = [&](int i, TV v) {
-        QV o;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = fine ? (int8_t)quantise(to_f32(v[e]), s, inv) : (int8_t)0;
-        qr[i] = o;
-    };
-    const int all = (int)(ldq / VEC);                 // with the zeros behind the row
-#pragma unroll
-    for (int h = 0; h < HELD; ++h)
-        if (t + h * TEAM < all) put(t + h * TEAM, held[h]);
-    for (int i = t + HELD * TEAM; i < all; i += TEAM) put(i, i < pieces ? xr[i] : TV{});
-    if (t == 0) scale[row] = s;
+    const float s = r.put(xr, pieces, t, top, m.q + row * m.ldq, (int)(m.ldq / VEC));
+    if (t == 0) m.scale[row] = s;
 }
 
 template <class T>
-int quantize_rows(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *q, int64_t ldq, float *scale, hipStream_t st) {
+bool in_pieces(const Rows<T> &m, int cols) {
     constexpr int V = 16 / sizeof(T);
-    const bool vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && cols % V == 0 && ((uintptr_t)q & 15) == 0 && ldq % V == 0;
+    return ((uintptr_t)m.x & 15) == 0 && m.ldx % V == 0 && cols % V == 0 && ((uintptr_t)m.q & 15) == 0 && m.ldq % V == 0;
+}
+
+template <class T>
+int quantize_rows(const Rows<T> &a, const Rows<T> &b, int cols, hipStream_t st) {
+    constexpr int V = 16 / sizeof(T);
+    constexpr int64_t MOST = 1 << 22;                  // rows a launch: a grid has fewer than 2^32 threads
     auto go = [&](auto kernel, int rows_per_block) {
-        constexpr int64_t MOST = 1 << 22;              // rows a launch: a grid has fewer than 2^32 threads
-        for (int64_t r = 0; r < rows; r += MOST) {
-            const int64_t n = rows - r < MOST ? rows - r : MOST;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)((n + rows_per_block - 1) / rows_per_block)), dim3(256), 0, st, x + r * ldx, n, cols, ldx, q + r * ldq,
-                               ldq, scale + r);
+        for (Rows<T> c = a, d = b; c.rows + d.rows > 0;) {
+            Rows<T> now = c, then = d;
+            now.rows = c.rows < MOST ? c.rows : MOST;
+            then.rows = d.rows < MOST - now.rows ? d.rows : MOST - now.rows;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((now.rows + then.rows + rows_per_block - 1) / rows_per_block)), dim3(256), 0, st, now, then, cols);
             DPD_LAUNCH_CHECK();
+            c = Rows<T>{c.x + now.rows * c.ldx, c.rows - now.rows, c.ldx, c.q + now.rows * c.ldq, c.ldq, c.scale + now.rows};
+            d = Rows<T>{d.x + then.rows * d.ldx, d.rows - then.rows, d.ldx, d.q + then.rows * d.ldq, d.ldq, d.scale + then.rows};
         }
         return DPD_OK;
     };
-    if (vec) return cols <= 1024 ? go(k_quantize_rows<T, 64, V>, 4) : go(k_quantize_rows<T, 256, V>, 1);
+    if (in_pieces(a, cols) && (b.rows == 0 || in_pieces(b, cols))) return cols <= 1024 ? go(k_quantize_rows<T, 64, V>, 4) : go(k_quantize_rows<T, 256, V>, 1);
     return cols <= 1024 ? go(k_quantize_rows<T, 64, 1>, 4) : go(k_quantize_rows<T, 256, 1>, 1);
+}
+template <class T>
+int quantize_rows(const T *x, int64_t rows, int cols, int64_t ldx, int8_t *q, int64_t ldq, float *scale, hipStream_t st) {
+    return quantize_rows(Rows<T>{x, rows, ldx, q, ldq, scale}, Rows<T>{}, cols, st);
 }
 
 template <class T>
@@ -282,6 +315,95 @@ int few_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, const 
     return DPD_OK;
 }
 
+// More tokens, up to 16 MB of them: as above, but a wave quantises whole rows (the next one is on its way meanwhile), and each
+// weight fragment meets MB blocks of 16 tokens.  Rows of LDS are 16 bytes longer than the image's, so that 16 of them spread
+// over the banks; the waves' sums take their place at the end.  Bound by latency: 8 tokens of 1024 x 1024 bf16 5.4 us.
+constexpr int SOME_BYTES = 32 * 1024;                   // quantised tokens
+
+template <class T, int VEC, int MB>
+__global__ __launch_bounds__(1024) void k_some_tokens(const T *__restrict__ x, int64_t ldx, int cols, int ld, int M, const int8_t *__restrict__ qw,
+                                                      ScaleOut<T> epi) {
+    constexpr int WAVES = 16, U = 4;
+    __shared__ __attribute__((aligned(16))) char lds[SOME_BYTES + 16 * 16 * MB];
+    __shared__ float scale[16 * MB];
+    nt::i32x4 *part = (nt::i32x4 *)lds;                 // [WAVES][MB][64], once the tokens [M][ld + 16] have been read
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, steps = ld / 64, pitch = ld + 16;
+    const int8_t *wr = qw + (int64_t)min(n0 + r, epi.N - 1) * ld + q * 16;
+    nt::i32x4 w[U];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = (i + u) * WAVES + wave;
+            w[u] = s < steps ? *(const nt::i32x4 *)(wr + (int64_t)s * 64) : nt::i32x4{0, 0, 0, 0};
+        }
+    };
+    fetch(0);
+    const int pieces = cols / VEC;
+    HeldRow<T, 64, VEC, VEC == 1 ? 16 : 4> row, next;
+    if (wave < M) next.load(x + (int64_t)wave * ldx, pieces, lane);
+    for (int m = wave; m < M; m += WAVES) {
+        const T *xr = x + (int64_t)m * ldx;
+        row = next;
+        if (m + WAVES < M) next.load(xr + WAVES * ldx, pieces, lane);
+        const unsigned top = wave_umax(row.top(xr, pieces, lane));
+        const float s = row.put(xr, pieces, lane, top, (int8_t *)lds + m * pitch, ld / VEC);
+        if (lane == 0) scale[m] = s;
+    }
+    __syncthreads();
+    nt::i32x4 acc[MB] = {};
+    const int8_t *tok[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) tok[b] = (const int8_t *)lds + min(b * 16 + r, M - 1) * pitch + q * 16;
+    for (int i = 0; i * WAVES < steps; i += U) {
+        nt::i32x4 now[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = w[u];
+        if ((i + U) * WAVES < steps) fetch(i + U);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int s = min((i + u) * WAVES + wave, steps - 1);                   // behind the last step the weights are zeros
+#pragma unroll
+            for (int b = 0; b < MB; ++b) acc[b] = nt::mfma<nt::I8>(now[u], *(const nt::i32x4 *)(tok[b] + s * 64), acc[b]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < MB; ++b) part[(wave * MB + b) * 64 + lane] = acc[b];
+    __syncthreads();
+    if (wave >= MB) return;
+    nt::i32x4 sum = part[wave * 64 + lane];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) sum += part[(k * MB + wave) * 64 + lane];
+    const int m = wave * 16 + r, n = n0 + q * 4;
+    if (m >= M) return;
+    const float s = scale[m];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (n + e < epi.N) {
+            float y = (float)sum[e] * s * epi.sb[n + e];
+            if (epi.bias) y += load_any(epi.bias, epi.bias_type, n + e);
+            epi.out[(int64_t)m * epi.ldo + n + e] = from_f32<T>(y);
+        }
+}
+
+template <class T, int VEC>
+int some_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, const int8_t *qw, const ScaleOut<T> &epi, hipStream_t st) {
+    const dim3 grid((unsigned)((epi.N + 15) / 16));
+    if (M <= 16) hipLaunchKernelGGL((k_some_tokens<T, VEC, 1>), grid, dim3(1024), 0, st, x, ldx, (int)K, (int)ld, (int)M, qw, epi);
+    else hipLaunchKernelGGL((k_some_tokens<T, VEC, 2>), grid, dim3(1024), 0, st, x, ldx, (int)K, (int)ld, (int)M, qw, epi);
+    DPD_LAUNCH_CHECK();
+    return DPD_OK;
+}
+
+// Whether the tokens go through k_some_tokens.  On the device, one launch against the quantiser and a tiled product, bf16, us:
+// 1024 x 1024 with 4, 8, 16, 17, 32 tokens 5.2, 5.4, 6.1, 7.0, 8.7 against 6.9, 7.3, 7.3, 7.6, 7.8; 4096 x 2048 with 16 tokens
+// 8.4 against 7.6.  On the host the second launch and its workspace cost 4 us, which is more than any of these loses.  Not
+// for 64 tokens (1024 x 1024: 13.9 against 7.9), longer rows (2048 x 4096, 8 tokens: 10 against 8.9) or more than one
+// round of workgroups (16384 x 1024, 8 tokens: 14 against 8.0).  One and two tokens are faster in k_few_tokens (1024 x 1024,
+// 2 tokens: 4.7 against 5.1), where it takes them.
+bool takes_some(int64_t M, int64_t N, int64_t ld) { return M <= 32 && N <= 4096 && ld <= 2048 && M * ld <= SOME_BYTES; }
+
 // rows of an int8 matrix at a stride that the product can read (a multiple of 128 bytes, zeros behind the row)
 __global__ __launch_bounds__(256) void k_pad_rows(const int8_t *__restrict__ q, int64_t rows, int cols, int64_t ld,
                                                   int8_t *__restrict__ out, int64_t ldo) {
@@ -380,6 +502,7 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ par
     const int c = threadIdx.x & 31, k = threadIdx.x >> 5, n = blockIdx.x * 32 + c;
     double s = 0.0;
     if (n < N)
+#pragma unroll 4
         for (int64_t b = k; b < blocks; b += 8) s += (double)part[b * N + n];
     red[k][c] = s;
     __syncthreads();
@@ -660,6 +783,11 @@ extern "C" int dpd_int8_linear(const void *x, int type, int64_t M, int64_t K, in
         const T *xt = (const T *)x;
         constexpr int V = 16 / sizeof(T);
         const FewPlan few = few_plan(xt, M, N, K, ldx, ld);
+        if (takes_some(M, N, ld) && (M >= 3 || !few.waves)) {
+            const ScaleOut<T> epi{nullptr, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
+            return in_pieces(Rows<T>{xt, M, ldx, nullptr, ld, nullptr}, (int)K) ? some_tokens<T, V>(xt, M, K, ldx, ld, qw, epi, st)
+                                                                              : some_tokens<T, 1>(xt, M, K, ldx, ld, qw, epi, st);
+        }
         if (few.waves) {
             const ScaleOut<T> epi{nullptr, w_scale, bias, bias_type, (T *)out, ldo, (int)N, false};
             if (few.waves == 16) return few.vec == V ? few_tokens<T, 16, V>(xt, M, K, ldx, ld, qw, epi, st) : few_tokens<T, 16, 1>(xt, M, K, ldx, ld, qw, epi, st);
@@ -684,14 +812,20 @@ extern "C" int dpd_int8_linear_forward(const void *x, int type, int64_t M, int64
     DPD_REQUIRE((((uintptr_t)qx | (uintptr_t)qw) & 15) == 0, DPD_ERR_INVALID_ARG, "int8_linear_forward: the images are 16-byte aligned");
     const int64_t ld = nt::pad_to(K, 128);
     hipStream_t st = as_stream(stream);
-    auto quantize = [&](const void *p, int t, int64_t rows, int64_t stride, int8_t *q, float *scale) {
-        return rows == 0 ? DPD_OK : with_type(t, [&](auto e) {
+    auto quantize = [&](int t, bool tokens, bool weight) {
+        return with_type(t, [&](auto e) {
             using T = decltype(e);
-            return quantize_rows((const T *)p, rows, (int)K, stride, q, ld, scale, st);
+            const Rows<T> a{(const T *)x, tokens ? M : 0, ldx, qx, ld, x_scale}, b{(const T *)w, weight ? N : 0, ldw, qw, ld, w_scale};
+            // one launch for both, unless one of them can be read in wide pieces and the other cannot
+            if (a.rows && b.rows && in_pieces(a, (int)K) != in_pieces(b, (int)K)) {
+                const int rc = quantize_rows(a, Rows<T>{}, (int)K, st);
+                return rc ? rc : quantize_rows(b, Rows<T>{}, (int)K, st);
+            }
+            return a.rows ? quantize_rows(a, b, (int)K, st) : quantize_rows(b, a, (int)K, st);
         });
     };
-    int rc = quantize(x, type, M, ldx, qx, x_scale);
-    if (!rc) rc = quantize(w, w_type, N, ldw, qw, w_scale);
+    int rc = quantize(type, true, type == w_type);
+    if (!rc && type != w_type) rc = quantize(w_type, false, true);
     if (rc || M == 0 || N == 0) return rc;
     return with_type(type, [&](auto e) {
         using T = decltype(e);

@@ -243,7 +243,7 @@ class Int8Inference:
         with L.device(x):
             args = (x2.data_ptr(), t, m, k, ldx, qw, sw, b, self._bias_type, n, out.data_ptr(), n)
             stream = L.raw_stream(self._index)
-            rc = self._fn(*args, 0, 0, stream) if m <= 16 else _NEEDS_WORKSPACE
+            rc = self._fn(*args, 0, 0, stream) if m <= 32 else _NEEDS_WORKSPACE
             if rc == _NEEDS_WORKSPACE:       # the tokens are quantised by a launch of their own
                 nbytes = m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256        # dpd_int8_linear_workspace_bytes
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)

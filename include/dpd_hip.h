@@ -382,7 +382,7 @@ int dpd_int8_matmul(const int8_t *a, int64_t lda, const float *a_scale, const in
                     void *ws, size_t ws_bytes, void *stream);
 
 /* Tokens x [M, K] against a weight image: dpd_quantize_rows_int8 of x and dpd_int8_matmul in one call, out in the type of
- * x.  qw: [N, dpd_int8_row_bytes(K)] int8, 16-byte aligned, as dpd_quantize_rows_int8 writes it with that ldq.  Up to 16
+ * x.  qw: [N, dpd_int8_row_bytes(K)] int8, 16-byte aligned, as dpd_quantize_rows_int8 writes it with that ldq.  Up to 32
  * tokens that together have few elements need no workspace: ws may be NULL then, and DPD_ERR_WORKSPACE, before anything is
  * launched, says that one is needed. */
 int64_t dpd_int8_row_bytes(int64_t K);

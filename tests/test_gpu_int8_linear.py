@@ -249,7 +249,7 @@ def test_values_that_are_not_finite():
 # ------------------------------------------------------------------------------- serving
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 515, 1030), (1, 4096, 4096), (2, 64, 30), (3, 100, 12000), (7, 1000, 700), (16, 130, 4096),
-                                     (17, 515, 1030), (40, 2048, 1024), (128, 640, 130), (300, 333, 600)])
+                                     (17, 515, 1030), (2, 40, 2047), (3, 4096, 2048), (31, 4097, 60), (32, 33, 1000), (32, 20, 1030), (40, 2048, 1024), (128, 640, 130), (300, 333, 600)])
 def test_serving_is_the_quantiser_and_the_product(m, n, k, dtype):
     x, w, b = tokens(m, k, dtype, 15).to(DEV), tokens(n, k, dtype, 16).to(DEV), tokens(1, n, dtype, 17)[0].to(DEV)
     qw, sw = quantize_rows_int8(w)
