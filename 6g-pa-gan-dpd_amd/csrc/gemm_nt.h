@@ -21,6 +21,10 @@
 // Lane layout of the results: the B rows are the first operand of the instruction, so a lane of a 16 x 16 block holds
 // one row m = lane & 15 and four columns.  The B rows of a pair of blocks are interleaved in fours, so that the pair gives
 // a lane eight successive columns: n = 8 * (lane >> 4) + 0..7 of 32.
+//
+// Bound by the matrix cores, and on large products by the power that they may draw: with zeros for data 4096^3 in bf16 takes
+// 80 us, with random data 100 to 106 (1.3 PFLOP/s); int8 4096^3 62 to 66 us, 8192^3 430 to 470 us (2.3 to 2.5 POP/s).  The library's
+// products of these sizes take 96, 67 and 441 us.  Small ones are bound by the start of a kernel and the write-back at its end.
 #pragma once
 #include "common.h"
 

@@ -2,8 +2,9 @@
 //     X <- X / max(|X|_F, eps);   steps times:  A = X X^T,  X <- a X + (b A + c A A) X
 // on the short side of each matrix, and the optimiser step that uses it (momentum, iteration, update of the weights).
 //
-// Matrices of up to 64 x 128 run in one workgroup, in fp32 out of LDS.  Larger ones take three tiled products a step
-// (gemm_nt.h).  Their factors are fp16, scaled by powers of two so that the range is used: after the division by its
+// Matrices of up to 64 x 128 run in one workgroup, in fp32 out of LDS.  Larger ones that fit into the LDS of a compute unit as
+// fp16 factors run in one workgroup as well (one launch instead of 17 that wait for each other: 128 x 128 fp32 61 us
+// instead of 102).  The others take three tiled products a step (gemm_nt.h).  The factors of both are fp16, scaled by powers of two so that the range is used: after the division by its
 // norm a matrix has entries around 1 / sqrt(r c) and singular values that stay below 4, so X is held times
 // S = 2^floor(log2 sqrt(r c)) (at most 2^14) and A, B = b A + c A A times 2^12.  One fp16 term has a relative rounding of
 // 2^-11, an eighth of that of bf16 inputs; two terms (the split form of gemm_nt.h) hold 22 bits and match an fp32
@@ -119,7 +120,7 @@ DEV double block_sum_d(double v, double *red) {       // over the 256 threads of
 // to whole 16 x 16 blocks.  A wave forms a block with v_mfma_f32_16x16x4_f32 (32 cycles for 4 of the sum's terms: these, the
 // LDS reads in front of them and three barriers a step are the time): 16 terms from one 16-byte read of each factor, lane
 // q of a row taking terms 4 q .. 4 q + 3 of them, which for both factors is the same order.
-// Row strides are 4 modulo 64 words: 16 rows of 16 bytes touch every bank as often.
+// Row strides are 4 modulo 64 words: 16 rows of 16 bytes touch every bank as often.  32 x 30, 5 steps: 10.4 us.
 constexpr int SMALL_R = 64, SMALL_C = 128, XS = SMALL_C + 4, AS = SMALL_R + 4;
 constexpr int SMALL_LDS = SMALL_R * XS + 2 * SMALL_R * AS;
 
@@ -245,7 +246,8 @@ struct SmallTable {
 // such blocks on v_mfma_f32_16x16x32_f16 (four 16 x 16 tiles from two fragments of each factor; a tile's lane holds four
 // successive columns of one row).  The sums of A and A A run along rows of LDS; that of B X runs down the columns of X,
 // which the transposing read ds_read_b64_tr_b16 gives (4 rows of 16 columns each).  Rows are 16 bytes longer than their
-// padded length, so that 16 of them spread over the banks.  Five barriers a step instead of three launches.
+// padded length, so that 16 of them spread over the banks.  Five barriers a step instead of three launches.  Bound by the one
+// compute unit's LDS reads and by latency: 65 x 65 bf16 22 us (75 with tiled products), 128 x 128 fp32 61, 64 x 512 fp32 74.
 constexpr int FIT_LDS = 150 * 1024, FIT_WAVES = 16, FIT_BLOCKS = 3;     // blocks of X that a wave holds
 
 __host__ DEV int64_t fit_bytes(int64_t r, int64_t c, bool split) {
@@ -499,7 +501,9 @@ DEV void img_store8(const Image &im, int z, int64_t row, int col, const float *v
     *(nt::f16x8 *)p = h;
     if (SPLIT) *(nt::f16x8 *)(p + 64) = l;
 }
-// Sum of squares of each matrix (and, for the optimiser, the new momentum): NORM_BLOCKS fp64 partial sums each.
+
+// Sum of squares of each matrix (and, for the optimiser, the new momentum): NORM_BLOCKS fp64 partial sums each.  Bound by
+// memory: 4096 x 4096 bf16 9.8 us (3.4 TB/s).
 template <class From>
 __global__ __launch_bounds__(256) void k_norm(From from, int64_t n, double *__restrict__ part) {
     __shared__ double red[4];
@@ -528,7 +532,8 @@ DEV void zero_pads(const Image &im, int z, int row, int rows, int from) {
 }
 
 // X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.  The images
-// that the products fill first get the zeros behind their rows here too.
+// that the products fill first get the zeros behind their rows here too.  Bound by memory: 4096 x 4096 bf16 18 us (5.5 TB/s,
+// x out of the last-level cache).
 template <class From, bool SPLIT>
 __global__ __launch_bounds__(256) void k_prepare(From from, int r, int c, const double *__restrict__ part, int blocks, double eps, double scale,
                                                  Image P, Image Q, Image Q2, Image A, Image B) {
@@ -582,6 +587,9 @@ DEV void img_store_half(const Image &im, int z, int64_t row, int col, int half, 
     *(nt::f16x8 *)(im.base + img_row(im, z, row) + img_col<SPLIT>(col) + half * 64) = v;
 }
 // The two symmetric products compute their tiles on and below the diagonal; a tile below it is stored turned as well.
+// 4096 x 4096, fp16 factors: Gram and polynomial 71 to 76 us each (253 tiles of 192 x 192, 0.95 PFLOP/s of what is computed),
+// the update 113 to 120 us (1.2 PFLOP/s); 1024 x 4096: 14.8, 7.6 and 17.7 us; 3 of 777 x 1000 in the split form: 16.5, 15.3
+// and 27 us.
 template <bool SPLIT>
 struct GramOut : NoFactors {           // A = X X^T (times T_SCALE); zeros behind the rows
     static constexpr bool TURNED = true;

@@ -20,8 +20,8 @@ class Muon(torch.optim.Optimizer):
 
     Parameters that are not matrices (biases) are updated by torch's Adam with the options in `adam`; both kinds are groups
     of this optimiser, so schedulers and state_dict() cover them.  `params`: tensors, or groups with options of their own.
-    The steps of all matrices of up to 64 x 128 take one launch (24 at a time); larger ones a handful each.  Every result is
-    the same in every run.  A step that is captured into a graph keeps the learning rate it was captured with."""
+    The steps of all matrices of up to 64 x 128 take one launch (24 at a time), and so do those of larger ones that fit into a
+    compute unit; the others go through tiled products, up to 8 of one size together.  Every result is the same in every run.  A step that is captured into a graph keeps the learning rate it was captured with."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients: Coefficients = COEFFICIENTS, eps: float = 1e-7, accurate: Optional[bool] = None, adam: Optional[Dict] = None):
