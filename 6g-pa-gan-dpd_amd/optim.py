@@ -10,6 +10,7 @@ from .utils.orthogonal import COEFFICIENTS, Coefficients, coefficient_table, wan
 # autograd sees that the weights changed (the public form of the same call walks its argument as a tree first)
 _bump_versions = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
 _PTR, _I64 = ctypes.c_void_p, ctypes.c_int64
+_NO_WORKSPACE = 256              # what dpd_muon_workspace_bytes says when no matrix needs one
 
 
 class Muon(torch.optim.Optimizer):
@@ -81,15 +82,17 @@ class Muon(torch.optim.Optimizer):
 
     def _matrices(self, group):
         sets: Dict = {}
-        types, state = L.TYPES, self.state
+        types, state, fp32 = L.TYPES, self.state, torch.float32
+        seen = last = None
         for p in group["params"]:
             g = p.grad
             if g is None:
                 continue
-            if p.dim() != 2 or g.is_sparse:
-                raise ValueError(f"a weight matrix with a dense gradient is expected, got {tuple(p.shape)}, sparse = {g.is_sparse}")
-            dtype, device = p.dtype, p.device
-            L.need_gpu(p, g)
+            shape, dtype, device = p.shape, p.dtype, p.get_device()
+            if len(shape) != 2 or g.is_sparse:
+                raise ValueError(f"a weight matrix with a dense gradient is expected, got {tuple(shape)}, sparse = {g.is_sparse}")
+            if device < 0 or g.get_device() != device:
+                L.need_gpu(p, g)
             if dtype not in types or g.dtype != dtype or not p.is_contiguous():
                 raise RuntimeError(f"weights must be contiguous float32, bfloat16 or float16 with gradients of their type, got {dtype} / {g.dtype}")
             own = state[p]
@@ -97,26 +100,35 @@ class Muon(torch.optim.Optimizer):
             if m is None:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("the first step of a weight makes its momentum: take one before the capture, a replay would clear it each time")
-                m = own["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
-            elif m.dtype != torch.float32 or m.shape != p.shape or not m.is_contiguous() or m.device != device:
-                raise RuntimeError(f"the momentum of a weight must be a contiguous float32 tensor of its shape on {device}, got {m.dtype} {tuple(m.shape)}")
-            items = sets.get((dtype, device))
-            if items is None:
-                items = sets[(dtype, device)] = ([], [], [])
-            for column, t in zip(items, (p, g if g.is_contiguous() else g.contiguous(), m)):
-                column.append(t)
-        for (dtype, device), items in sets.items():
-            n = len(items[0])
+                m = own["momentum_buffer"] = torch.zeros_like(p, dtype=fp32)
+            elif m.dtype != fp32 or m.shape != shape or not m.is_contiguous() or m.get_device() != device:
+                raise RuntimeError(f"the momentum of a weight must be a contiguous float32 tensor of its shape on {p.device}, got {m.dtype} {tuple(m.shape)}")
+            if (dtype, device) != seen:
+                seen = (dtype, device)
+                last = sets.get(seen)
+                if last is None:
+                    last = sets[seen] = ([], [], [], [], [], [], [])
+            ps, gs, at_p, at_g, at_m, rows, cols = last
+            if not g.is_contiguous():
+                g = g.contiguous()
+            ps.append(p)
+            gs.append(g)                       # a copy has to live until the launch
+            at_p.append(p.data_ptr())
+            at_g.append(g.data_ptr())
+            at_m.append(m.data_ptr())
+            rows.append(shape[0])
+            cols.append(shape[1])
+        for (dtype, index), (ps, _, at_p, at_g, at_m, rows, cols) in sets.items():
+            n = len(ps)
             pointers, sizes = _PTR * n, _I64 * n
-            shapes = [p.shape for p in items[0]]
-            rows, cols = sizes(*[s[0] for s in shapes]), sizes(*[s[1] for s in shapes])
+            h_rows, h_cols = sizes(*rows), sizes(*cols)
             acc, steps = wants_accurate(group["accurate"], dtype), int(group["steps"])
             coef = coefficient_table(group["coefficients"], steps)
-            with L.device(items[0][0]):
-                nbytes = L.entry("dpd_muon_workspace_bytes")(n, rows, cols, acc)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            with L.device(ps[0]):
+                nbytes = L.entry("dpd_muon_workspace_bytes")(n, h_rows, h_cols, acc)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=ps[0].device) if nbytes > _NO_WORKSPACE else None
                 L.check(L.entry("dpd_muon_step")(
-                    n, *[pointers(*[t.data_ptr() for t in column]) for column in items], rows, cols, types[dtype], float(group["lr"]),
+                    n, pointers(*at_p), pointers(*at_g), pointers(*at_m), h_rows, h_cols, types[dtype], float(group["lr"]),
                     float(group["momentum"]), int(group["nesterov"]), float(group["weight_decay"]), steps, coef, float(group["eps"]), acc,
-                    ws.data_ptr(), nbytes, L.raw_stream(device.index)))
-            _bump_versions(items[0])
+                    0 if ws is None else ws.data_ptr(), nbytes, L.raw_stream(index)))
+            _bump_versions(ps)

@@ -50,8 +50,8 @@ def test_matmul_arguments(kw, code, text):
 
 
 def test_linear_and_backward_arguments():
-    ws = L.lib().dpd_int8_linear_workspace_bytes(17, 4, 16)
-    ok = [PTR, 0, 17, 16, 16, PTR, PTR, NULL, 0, 4, PTR, 4, PTR, ws, NULL]
+    ws = L.lib().dpd_int8_linear_workspace_bytes(40, 4, 16)          # few tokens need none
+    ok = [PTR, 0, 40, 16, 16, PTR, PTR, NULL, 0, 4, PTR, 4, PTR, ws, NULL]
     for at, value, code, text in ((1, 5, 1, "type"), (3, 0, 2, "input features"), (0, NULL, 1, "null"), (4, 15, 1, "stride"), (11, 3, 1, "stride"),
                                   (13, ws - 1, 4, "workspace"), (5, ctypes.c_void_p(PTR.value + 8), 1, "aligned")):
         args = list(ok)
