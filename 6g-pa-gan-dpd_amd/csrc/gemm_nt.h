@@ -221,6 +221,40 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     };
     auto next = [](int at) { return at == (STAGES - 1) * STAGE ? 0 : at + STAGE; };
 
+    // What the epilogue reads: AHEAD block rows together.  Where a wave has few results and its workgroup is alone on the
+    // compute unit, all of it in front of the loop, whose first wait it shares (1024 x 4096, update: 17.1 -> 16.3 us, last
+    // 14.5 -> 13.6); a wave with many has no registers for that, and a second workgroup hides the wait at the end (there it cost
+    // 42.4 -> 45.1 us).
+    constexpr int AHEAD = SPLIT ? 2 : TM % 4 == 0 ? 4 : TM;
+    constexpr bool EARLY = TM * TN <= 8 && AHEAD == TM && LDS > 80 * 1024;
+    static_assert(TM % AHEAD == 0, "whole groups of block rows");
+    typename Epilogue::Col col[TN / 2];
+    typename Epilogue::Row row[AHEAD];
+    typename Epilogue::Pre pre[AHEAD][TN / 2];
+    auto read_col = [&]() {
+#pragma unroll
+        for (int j = 0; j < TN / 2; ++j) col[j] = epi.col(blockIdx.z, n0 + wn * TN * 16 + j * 32 + q * 8);
+    };
+    auto read_rows = [&](int i0) {
+        if (WAVES_K > 1 && group > 0) return;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int m = m0 + (wm * TM + i0 + k) * 16 + r;
+            if (m >= g.M) continue;
+            row[k] = epi.row(blockIdx.z, m);
+#pragma unroll
+            for (int j = 0; j < TN / 2; ++j) {
+                const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
+                if (n < g.N) pre[k][j] = epi.pre(blockIdx.z, m, n);
+            }
+        }
+    };
+    if (EARLY) {
+        read_col(), read_rows(0);
+        // nothing of it may come behind the loads of the stages: the waits count those
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int s = 0; s < STAGES; ++s)
         if (s < steps) {
@@ -336,29 +370,11 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
                     for (int j = 0; j < TN; ++j) acc[i][j] += parts[((k * WAVES + wave) * TM * TN + i * TN + j) * 64 + lane];
         }
     }
-    typename Epilogue::Col col[TN / 2];
-#pragma unroll
-    for (int j = 0; j < TN / 2; ++j) col[j] = epi.col(blockIdx.z, n0 + wn * TN * 16 + j * 32 + q * 8);
+    if (!EARLY) read_col();
     const bool turn = Epilogue::TURNED && !(g.lower && tm == tn);
-    constexpr int AHEAD = SPLIT ? 2 : TM % 4 == 0 ? 4 : TM;    // block rows whose inputs are read together, in front of their use
-    static_assert(TM % AHEAD == 0, "whole groups of block rows");
 #pragma unroll
     for (int i0 = 0; i0 < TM; i0 += AHEAD) {
-        typename Epilogue::Row row[AHEAD];
-        typename Epilogue::Pre pre[AHEAD][TN / 2];
-        if (WAVES_K == 1 || group == 0) {
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const int m = m0 + (wm * TM + i0 + k) * 16 + r;
-                if (m >= g.M) continue;
-                row[k] = epi.row(blockIdx.z, m);
-#pragma unroll
-                for (int j = 0; j < TN / 2; ++j) {
-                    const int n = n0 + wn * TN * 16 + j * 32 + q * 8;
-                    if (n < g.N) pre[k][j] = epi.pre(blockIdx.z, m, n);
-                }
-            }
-        }
+        if (!EARLY) read_rows(i0);
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int i = i0 + k, m = m0 + (wm * TM + i) * 16 + r;

@@ -588,7 +588,7 @@ DEV void img_store_half(const Image &im, int z, int64_t row, int col, int half, 
 }
 // The two symmetric products compute their tiles on and below the diagonal; a tile below it is stored turned as well.
 // 4096 x 4096, fp16 factors: Gram and polynomial 71 to 76 us each (253 tiles of 192 x 192, 0.95 PFLOP/s of what is computed),
-// the update 113 to 120 us (1.2 PFLOP/s); 1024 x 4096: 14.8, 7.6 and 17.7 us; 3 of 777 x 1000 in the split form: 16.5, 15.3
+// the update 113 to 120 us (1.2 PFLOP/s); 1024 x 4096: 14.7, 7.2 and 16.6 us; 3 of 777 x 1000 in the split form: 16.5, 15.3
 // and 27 us.
 template <bool SPLIT>
 struct GramOut : NoFactors {           // A = X X^T (times T_SCALE); zeros behind the rows
