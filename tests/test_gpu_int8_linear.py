@@ -246,6 +246,32 @@ def test_values_that_are_not_finite():
     assert torch.isfinite(xg.grad[[0, 1, 3, 4]]).all() and not torch.isfinite(xg.grad[2]).any()
 
 
+def test_offsets_beyond_32_bits():
+    """The last rows of 70000 x 32768 (2.3e9 elements) come out as they do alone.  The product is exact; a gradient's sum may
+    be grouped otherwise, so that two results differ by twice what one may be off (head of this file; V is the same for both)."""
+    m, k, n, last = 70000, 32768, 24, 40
+    gen = torch.Generator(device=DEV).manual_seed(40)
+    x = torch.randn(m, k, generator=gen, device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    w = tokens(n, k, torch.float32, 41).to(DEV).requires_grad_(True)
+    tail = x.detach()[-last:].clone().requires_grad_(True)
+    g = torch.zeros(m, n, device=DEV, dtype=torch.bfloat16)
+    g[-last:] = tokens(last, n, torch.bfloat16, 42).to(DEV)
+    y = int8_linear(x, w)
+    want = int8_linear(tail, w)
+    assert torch.equal(y[-last:], want)
+    gx, gw = torch.autograd.grad(y, (x, w), g)
+    wx, ww = torch.autograd.grad(want, (tail, w), g[-last:])
+    assert not gx[:-last].any()
+    near = g[-last:].abs().float()
+    for a, b, size, terms, u in ((gx[-last:], wx, near @ w.detach().abs(), n, U[torch.bfloat16]), (gw, ww, near.t() @ tail.detach().abs().float(), last, U[torch.float32])):
+        assert ((a.double() - b.double()).abs() <= 2 * (u * b.double().abs() * 1.01 + (terms + 1) * 2.0 ** -23 * 1.02 * size.double())).all()
+    q, s = quantize_rows_int8(x)
+    qt, st = quantize_rows_int8(tail)
+    assert torch.equal(q[-last:], qt) and torch.equal(s[-last:], st)
+    eng = Int8Inference(dict(zip(("weight", "scale"), quantize_rows_int8(w))))
+    assert torch.equal(eng(x.detach())[-last:], want)
+
+
 # ------------------------------------------------------------------------------- serving
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 515, 1030), (1, 4096, 4096), (2, 64, 30), (3, 100, 12000), (7, 1000, 700), (16, 130, 4096),

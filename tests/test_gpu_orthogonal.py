@@ -256,6 +256,18 @@ def test_muon_many_matrices_and_refusals():
     assert torch.equal(q, r)
 
 
+def test_offsets_beyond_32_bits():
+    """The last of 5 matrices of 256 x 1700000 (2.2e9 elements) comes out as it does alone.  This looks for addresses, not for
+    roundings: sums may be grouped otherwise, which the factors' and the result's roundings (2^-11, 2^-8) turn into less
+    than 2^-6; a wrong address is off by the whole value."""
+    gen = torch.Generator(device=DEV).manual_seed(50)
+    x = torch.randn(5, 256, 1_700_000, generator=gen, device=DEV, dtype=torch.bfloat16)
+    y, want = orthogonalize(x)[4], orthogonalize(x[4])
+    assert torch.linalg.vector_norm(y.float() - want.float()) <= 2.0 ** -6 * torch.linalg.vector_norm(want.float())
+    tall = orthogonalize(x[3:].transpose(1, 2).contiguous())[1]
+    assert torch.linalg.vector_norm(tall.t().float() - want.float()) <= 2.0 ** -6 * torch.linalg.vector_norm(want.float())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_muon_matrices_of_one_size_go_together(dtype):
     """Wide and tall matrices of the same two sides share launches: each comes out as it does alone (the tile that is chosen
