@@ -96,3 +96,33 @@ def test_single_process_is_noop():
     assert not dp.enabled and dp.world == 1 and dp.shard_rows(10) == (0, 10)
     x = torch.ones(3, requires_grad=True)
     assert dp.global_sum(x) is x
+
+
+def test_gloo_never_gets_device_tensors(monkeypatch):
+    """gloo's device path can stall for good, so a device tensor is reduced through a host copy, whatever the environment says."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("dpd_parallel", os.path.join(ROOT, "6g-pa-gan-dpd_amd", "parallel.py"))
+    par = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(par)
+    host = torch.ones(3)
+
+    class OnDevice:
+        is_cuda = True
+
+        def detach(self):
+            return self
+
+        def cpu(self):
+            return host
+
+        def copy_(self, t):
+            self.got = t
+    seen = []
+    monkeypatch.setattr(par.dist, "get_backend", lambda group=None: "gloo")
+    monkeypatch.setattr(par.dist, "all_reduce", lambda t, op=None, group=None: seen.append(t))
+    monkeypatch.setattr(par.torch.cuda, "synchronize", lambda: None)
+    for mode in ("0", "1", "2"):
+        monkeypatch.setenv("DPD_GLOO_DEVICE_TENSORS", mode)
+        t = OnDevice()
+        par._all_reduce(t, dist.ReduceOp.SUM)
+        assert seen.pop() is host and t.got is host
