@@ -431,10 +431,12 @@ int int8_product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
 }
 
 // ---- gradients ---------------------------------------------------------------------------
-// bf16 planes of a value: 1 for bf16 gradients (one rounding of 2^-8, the type's own), 2 for fp16 (2^-16),
-// 3 for fp32 (the whole value): the planes of a row lie one behind the other along k, the smallest first.
+// bf16 planes of a gradient times a scale: 2 for bf16 and fp16 gradients (2^-16, so that the rounding of the result is
+// the only one that shows), 3 for fp32 (the whole value): the planes of a row lie one behind the other along k, the smallest
+// first.  One plane for bf16 would halve the two products (4096 tokens of 4096 x 4096: 364 instead of 574 us for the training
+// pass), but every term would be rounded by 2^-8 and the gradients be 2.3e-3 off in place of 1.7e-3.
 template <class T>
-constexpr int planes_of() { return std::is_same<T, float>::value ? 3 : std::is_same<T, __bf16>::value ? 1 : 2; }
+constexpr int planes_of() { return std::is_same<T, float>::value ? 3 : 2; }
 
 template <int P>
 DEV void put_planes8(__bf16 *p, int64_t plane, const float *v) {
@@ -456,7 +458,7 @@ DEV void put_planes8(__bf16 *p, int64_t plane, const float *v) {
 
 // One 64 x 64 tile of g [M, N]: gs[m, n] = g sw[n] (row-major, for gx), gt[n, m] = g sx[m] (transposed, for gw), each as
 // bf16 planes with zeros behind the rows, and this tile's column sums for gb.  Pieces of 8 elements on every access; bound
-// by memory (2 + 2 or 4 bytes an element in bf16).
+// by memory (2 + 8 bytes an element in bf16).
 template <class T>
 DEV void grad_images(int bx, int by, float (*t)[65], const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
                      const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad, __bf16 *__restrict__ gt, int64_t m_pad,
@@ -512,15 +514,13 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ par
     }
 }
 
-// q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves (exact), or, with the
-// scales of the rows, their values rounded to bf16.  A wave takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it
+// q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves, which are exact.  A wave takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it
 // turns in registers; the words meet in LDS (4 rows of a column a word) and leave as 16 bytes of 8 rows.  Bound by memory.
 struct Turn {
     const int8_t *q;
     int64_t rows, ld;
     int cols;
     bool whole;
-    const float *scale;
     __bf16 *out;
     int64_t rows_pad;
     int bx, by;                                       // workgroups along the rows and the columns; none: 0
@@ -531,7 +531,6 @@ DEV void transpose_i8(int bx, int by, unsigned (*t)[66], const Turn &a) {
     const int64_t rows = a.rows, ld = a.ld, rows_pad = a.rows_pad;
     const int cols = a.cols;
     const bool whole = a.whole;
-    const float *__restrict__ scale = a.scale;
     __bf16 *__restrict__ out = a.out;
     typedef __bf16 b8 __attribute__((ext_vector_type(8)));
     typedef unsigned u4 __attribute__((ext_vector_type(4)));
@@ -563,9 +562,6 @@ DEV void transpose_i8(int bx, int by, unsigned (*t)[66], const Turn &a) {
         }
     }
     const int i = (threadIdx.x & 31) * 8;             // this thread's rows
-    float f[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = r0 + i + k < rows ? (scale ? scale[r0 + i + k] : 1.f) : 0.f;
     __syncthreads();
     if (r0 + i >= rows_pad) return;
 #pragma unroll
@@ -574,7 +570,7 @@ DEV void transpose_i8(int bx, int by, unsigned (*t)[66], const Turn &a) {
         if (c0 + j >= cols) return;
         b8 o;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = (__bf16)((float)(int8_t)(t[j][(i + k) >> 2] >> (8 * (k & 3))) * f[k]);
+        for (int k = 0; k < 8; ++k) o[k] = (__bf16)(float)(int8_t)(t[j][(i + k) >> 2] >> (8 * (k & 3)));
         *(b8 *)(out + (int64_t)(c0 + j) * rows_pad + r0 + i) = o;
     }
 }
@@ -603,12 +599,11 @@ __global__ __launch_bounds__(256) void k_backward_images(const T *__restrict__ g
     transpose_i8(id % x.bx, id / x.bx, lds.u, x);
 }
 
-int planes_for(int type) { return type == DPD_F32 ? 3 : type == DPD_BF16 ? 1 : 2; }
+int planes_for(int type) { return type == DPD_F32 ? 3 : 2; }
 
 struct BackwardPlan {
     int64_t m_pad, n_pad, gs, gt, wt, xt, part, total;      // element counts and byte offsets into the workspace
-    BackwardPlan(int64_t M, int64_t N, int64_t K, int type, bool gx, bool gw, bool gb) {
-        const int p = planes_for(type);
+    BackwardPlan(int64_t M, int64_t N, int64_t K, int p, bool gx, bool gw, bool gb) {
         m_pad = nt::pad_to(M, 64), n_pad = nt::pad_to(N, 64);
         int64_t at = 0;
         auto take = [&](bool want, int64_t bytes) {
@@ -631,20 +626,16 @@ template <class T>
 int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const int8_t *qx, int64_t ldqx, const float *sx,
               const int8_t *qw, int64_t ldqw, const float *sw, T *gx, void *gw, int gw_type, void *gb, int gb_type, char *ws, hipStream_t st) {
     constexpr int P = planes_of<T>();
-    const BackwardPlan p(M, N, K, std::is_same<T, float>::value ? DPD_F32 : P == 1 ? DPD_BF16 : DPD_F16, gx, gw, gb);
+    const BackwardPlan p(M, N, K, P, gx, gw, gb);
     __bf16 *gs = gx ? (__bf16 *)(ws + p.gs) : nullptr, *wt = (__bf16 *)(ws + p.wt), *gt = gw ? (__bf16 *)(ws + p.gt) : nullptr,
            *xt = (__bf16 *)(ws + p.xt);
     float *part = gb ? (float *)(ws + p.part) : nullptr;
-    // bf16 gradients whose rows the product can read are its operand as they are; the weight's scales then go into the other
-    // one, rounded to bf16 there instead of in g times scale (one rounding of 2^-8 a term either way)
-    const bool direct = P == 1 && ((uintptr_t)g & 15) == 0 && ldg % 8 == 0 && N % 8 == 0 && ldg * 2 <= nt::MAX_ROW_BYTES;
-    if (direct) gs = nullptr;
-    auto turn = [&](bool want, const int8_t *q, int64_t rows, int64_t ld, const float *scale, __bf16 *out, int64_t rows_pad) {
-        Turn a{q, rows, ld, (int)K, whole16(q, ld, K), scale, out, rows_pad, 0, 0};
+    auto turn = [&](bool want, const int8_t *q, int64_t rows, int64_t ld, __bf16 *out, int64_t rows_pad) {
+        Turn a{q, rows, ld, (int)K, whole16(q, ld, K), out, rows_pad, 0, 0};
         if (want) a.bx = (int)((rows_pad + 255) / 256), a.by = (int)((K + 63) / 64);
         return a;
     };
-    const Turn tw = turn(gx, qw, N, ldqw, direct ? sw : nullptr, wt, p.n_pad), tx = turn(gw, qx, M, ldqx, nullptr, xt, p.m_pad);
+    const Turn tw = turn(gx, qw, N, ldqw, wt, p.n_pad), tx = turn(gw, qx, M, ldqx, xt, p.m_pad);
     const int bx = gs || gt || part ? (int)(p.m_pad / 64) : 0, by = (int)(p.n_pad / 64);
     const int64_t blocks = (int64_t)bx * by + (int64_t)tw.bx * tw.by + (int64_t)tx.bx * tx.by;
     DPD_REQUIRE(blocks * 256 <= UINT32_MAX, DPD_ERR_SHAPE, "int8_linear_backward: %lld x %lld gradients are too many for one call", (long long)M, (long long)N);
@@ -662,9 +653,8 @@ int gradients(const T *g, int64_t ldg, int64_t M, int64_t N, int64_t K, const in
     }
     if (gx) {
         nt::Args a{};
-        a.a = direct ? (const char *)g : (const char *)gs, a.lda = direct ? ldg * 2 : P * p.n_pad * 2;
-        a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
-        a.wrap = (int)(p.n_pad / 64), a.steps = P * a.wrap, a.tail = direct ? (int)(N * 2 - (int64_t)(a.steps - 1) * 128) : 128;
+        a.a = (const char *)gs, a.lda = P * p.n_pad * 2, a.b = (const char *)wt, a.ldb = p.n_pad * 2, a.M = (int)M, a.N = (int)K;
+        a.wrap = (int)(p.n_pad / 64), a.steps = P * a.wrap, a.tail = 128;
         const int rc = nt::product<nt::BF16>(a, 1, PlainOut<T>{gx, K, (int)K, whole8(gx, K)}, st);
         if (rc) return rc;
     }
@@ -836,7 +826,7 @@ extern "C" int dpd_int8_linear_forward(const void *x, int type, int64_t M, int64
 
 extern "C" size_t dpd_int8_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, int need_gx, int need_gw, int need_gb) {
     if (M < 0 || N < 0 || K < 0 || !is_type(type)) return 0;
-    return (size_t)BackwardPlan(M, N, K, type, need_gx, need_gw, need_gb).total + 256;
+    return (size_t)BackwardPlan(M, N, K, planes_for(type), need_gx, need_gw, need_gb).total + 256;
 }
 
 extern "C" int dpd_int8_linear_backward(const void *g, int type, int64_t M, int64_t N, int64_t K, int64_t ldg, const int8_t *qx, int64_t ldqx,

@@ -408,3 +408,16 @@ def test_a_layer_is_trained_and_then_served():
         want = net(x)
         got = torch.cat([second(torch.nn.functional.leaky_relu(first(x[i:i + 1]), 0.2)) for i in range(64)])
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m, n, k", [(1, 8, 16), (64, 64, 64), (96, 40, 72), (130, 65, 33), (520, 256, 128)])
+def test_gradients_are_rounded_to_their_type_once(m, n, k, dtype):
+    """A term g s q enters as two bf16 terms, off by 2^-16 (and g s by 2^-24): the type's own rounding of the result is
+    the only one of its size."""
+    x, w, g = tokens(m, k, dtype, 50), (tokens(n, k, dtype, 51).float() / k ** 0.5).to(dtype), tokens(m, n, dtype, 52) * 0.1
+    xd, wd = (t.to(DEV).requires_grad_(True) for t in (x, w))
+    int8_linear(xd, wd).backward(g.to(DEV))
+    (gx, gxs), (gw, gws), _ = oo.gradients(g, *oo.quantize_rows(x), *oo.quantize_rows(w))
+    close(xd.grad, gx, gxs, dtype, n, 2.0 ** -16 + 2.0 ** -24)
+    close(wd.grad, gw, gws, dtype, m, 2.0 ** -16 + 2.0 ** -24)
