@@ -5,11 +5,20 @@ from typing import Dict, Optional
 import torch
 
 from . import _lib as L
-from .utils.orthogonal import COEFFICIENTS, Coefficients, coefficient_table, wants_accurate
+from .utils.orthogonal import COEFFICIENTS, Coefficients, coefficient_table
 
 # autograd sees that the weights changed (the public form of the same call walks its argument as a tree first)
 _bump_versions = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
 _PTR, _I64 = ctypes.c_void_p, ctypes.c_int64
+
+
+def wants_accurate(accurate: Optional[bool], dtype: torch.dtype) -> int:
+    """Unless the caller says: fp16 factors for bf16 weights, factors in two terms for the others.  A step is a small part of
+    a weight, and the weight's own rounding (2^-8 of the whole) hides what fp16 factors do to it: after a step of lr 0.02, matrices
+    of 2048 and 4096 are 1.66e-3 off with either."""
+    return int(dtype != torch.bfloat16 if accurate is None else bool(accurate))
+
+
 _NO_WORKSPACE = 256              # what dpd_muon_workspace_bytes says when no matrix needs one
 
 
@@ -21,6 +30,7 @@ class Muon(torch.optim.Optimizer):
 
     Parameters that are not matrices (biases) are updated by torch's Adam with the options in `adam`; both kinds are groups
     of this optimiser, so schedulers and state_dict() cover them.  `params`: tensors, or groups with options of their own.
+    `accurate`: as for `orthogonalize`, but None means False for bf16 weights, whose own rounding hides the difference.
     The steps of all matrices of up to 64 x 128 take one launch (24 at a time), and so do those of larger ones that fit into a
     compute unit; the others go through tiled products, up to 8 of one size together.  Every result is the same in every run.  A step that is captured into a graph keeps the learning rate it was captured with."""
 

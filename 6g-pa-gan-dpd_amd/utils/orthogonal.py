@@ -31,11 +31,6 @@ def coefficient_table(coefficients: Coefficients, steps: int):
     return _table(coefficients, int(steps))
 
 
-def wants_accurate(accurate: Optional[bool], dtype: torch.dtype) -> int:
-    """bf16 input: factors in fp16 carry eight times its precision.  fp32 and fp16: factors in two terms."""
-    return int(dtype != torch.bfloat16 if accurate is None else bool(accurate))
-
-
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = COEFFICIENTS, eps: float = 1e-7,
                   accurate: Optional[bool] = None) -> torch.Tensor:
     """The Newton-Schulz iterate of each matrix of x [..., rows, cols] in the type of x:
@@ -43,9 +38,10 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
         X <- X / max(|X|_F, eps);   `steps` times:  A = X X^T,  X <- a X + (b A + c A A) X
 
     (on the transposed matrix where rows > cols).  `coefficients`: one triple (a, b, c), or one for each step; triples that
-    could take a singular value above 3.9 raise ValueError.  `accurate`: fp32 accuracy (the default for fp32 and fp16), or
-    factors rounded to fp16 with sums in fp32 (the default for bf16: an eighth of that type's own rounding; small
-    singular values next to large ones feel either, since the iteration amplifies them).  Matrices of up to 64 x 128 are
+    could take a singular value above 3.9 raise ValueError.  `accurate`: fp32 accuracy (the default), or, with False,
+    factors rounded to fp16 with sums in fp32, in a third of the time where the products are large (a bf16 4096 x 4096 matrix comes
+    out 1.9e-3 off, of which the rounding to its type is 1.7e-3; small singular values next to large ones feel the factors'
+    rounding more, since the iteration amplifies them).  Matrices of up to 64 x 128 are
     always computed in fp32.  A matrix that holds a NaN or an infinity comes out as NaN.  Not differentiable."""
     L.need_gpu(x)
     if x.dtype not in L.TYPES:
@@ -59,7 +55,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
     rows, cols = x.shape[-2:]
     batch = x.shape[:-2].numel()
     out = torch.empty_like(xc)
-    acc = wants_accurate(accurate, x.dtype)
+    acc = int(accurate is None or bool(accurate))
     with L.device(x):
         nbytes = L.entry("dpd_orthogonalize_workspace_bytes")(batch, rows, cols, acc)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)

@@ -320,3 +320,14 @@ def test_training_command_with_muon(tmp_path):
     main(args[:-2] + ["--epochs", "3", "--output-dir", str(tmp_path), "--resume", str(tmp_path / "latest.pth")])
     ck = torch.load(tmp_path / "latest.pth", weights_only=True)
     assert ck["epoch"] == 2 and ck["g_optimizer_state_dict"]["param_groups"][0]["kind"] == "matrix"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("r, c", [(65, 65), (70, 200), (300, 33), (130, 515), (600, 300)])
+def test_the_default_is_off_by_its_types_rounding_alone(r, c, dtype):
+    """An entry v that is computed with an error e comes out within e + U (|v| + e): what is left of an entry's distance behind
+    U |v| is at most (1 + U) e, and e is that of the accurate form whatever the type is."""
+    x = update(r, c, r + 2 * c).to(dtype)
+    want = oo.iterate(x)
+    left = ((orthogonalize(x.to(DEV)).double().cpu() - want).abs() - U[dtype] * want.abs()).clamp_min(0.0)
+    assert float(left.norm()) <= (1 + U[dtype]) * allowed(x, want, True), (float(left.norm()), float(want.norm()))
