@@ -33,6 +33,7 @@ extern int g_gen_deterministic;
 extern int g_critic_deterministic;
 extern int g_chain_carry;
 extern int g_gp_fused;
+extern int g_product_tile;
 static bool critic_use_mfma(int64_t N) { return g_critic_impl == 2 || (g_critic_impl == 0 && N >= 1024); }
 
 extern "C" int dpd_set_option(const char *name, int value) {
@@ -55,6 +56,10 @@ extern "C" int dpd_set_option(const char *name, int value) {
     }
     if (__builtin_strcmp(name, "gp_fused") == 0 && (value == 0 || value == 1)) {
         g_gp_fused = value;
+        return DPD_OK;
+    }
+    if (__builtin_strcmp(name, "product_tile") == 0 && value >= -1 && value <= 10) {
+        g_product_tile = value;
         return DPD_OK;
     }
     dpd_set_error("set_option: unknown option %s or bad value %d", name, value);

@@ -30,6 +30,8 @@
 
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
+extern int g_product_tile;       // dpd_set_option("product_tile", -1 by the rule / 0..10 that tile wherever it applies)
+
 namespace nt {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -134,7 +136,7 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     constexpr int WAVES = WAVES_M * WAVES_N, TM = BM / WAVES_M / 16, TN = BN / WAVES_N / 16;
     constexpr int LOADS_A = BM / 8 / WAVES, LOADS_B = BN / 8 / WAVES, LOADS = LOADS_A + LOADS_B, PART = (BM + BN) * STEP, STAGE = WAVES_K * PART;
     static_assert(LOADS_A >= 1 && LOADS_B >= 1 && LOADS_A * 8 * WAVES == BM && LOADS_B * 8 * WAVES == BN, "every wave loads whole groups of 8 rows");
-    static_assert(TN % 2 == 0 && (TM % 2 == 0 || KIND != F16_SPLIT) && STAGES >= 2 && (STAGES - 2) * LOADS < 64, "pairs of blocks; the wait counter has 6 bits");
+    static_assert(TN % 2 == 0 && (TM % 2 == 0 || KIND != F16_SPLIT) && STAGES >= 2 && (STAGES - 1) * LOADS < 64, "pairs of blocks; the wait counter has 6 bits");
     constexpr int PITCH = BM + 8, TURN_BYTES = Epilogue::TURNED ? BN * PITCH * 2 : 0, LDS = STAGES * STAGE > TURN_BYTES ? STAGES * STAGE : TURN_BYTES;
     static_assert(LDS <= 160 * 1024, "LDS of a compute unit");
     __shared__ __attribute__((aligned(256))) char smem[LDS];
@@ -481,6 +483,11 @@ constexpr Tile TILES[] = {
 static inline int best_tile(const Args &g, int batch, bool split) {
     int best = -1;
     float least = 0.f;
+    static_assert(sizeof(TILES) / sizeof(TILES[0]) == 11, "product_tile names every tile");
+    if (g_product_tile >= 0) {
+        const Tile &t = TILES[g_product_tile];
+        if (!(g.lower && t.bm != t.bn) && (split ? t.split_one : t.one).per > 0.f) return g_product_tile;
+    }
     for (int i = 0; i < (int)(sizeof(TILES) / sizeof(TILES[0])); ++i) {
         const Tile &t = TILES[i];
         const Round one = split ? t.split_one : t.one, two = split ? t.split_two : t.two;

@@ -7,6 +7,8 @@
 #include <type_traits>
 #include "gemm_nt.h"
 
+int g_product_tile = -1;
+
 namespace {
 
 constexpr float SCALE_FLOOR = 0x1p-100f;      // rows below it share its scale: a row of zeros has a finite one

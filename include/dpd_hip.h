@@ -62,7 +62,10 @@ int dpd_version(void);
  * enough rows to fill the waves evenly, else 0.  The results agree to fp32 rounding (same arithmetic per output).
  * "gp_fused": 1 (default) = dpd_critic_gp on rows of a multiple of 256 samples runs forward, input gradient and the
  * reverse chain in one pass over the samples and applies the row coefficients to per-unit partial sums afterwards;
- * 0 = the three-pass form for every shape.  Same results to fp32 summation order. */
+ * 0 = the three-pass form for every shape.  Same results to fp32 summation order.
+ * "product_tile": -1 (default) = the tiled products of the 8-bit layer and of the orthogonalised update choose their tile by
+ * the estimated time; 0..10 = that tile of the table in csrc/gemm_nt.h wherever it applies (square ones for symmetric
+ * products).  int8 products are the same with every tile, the others to fp32 summation order. */
 int dpd_set_option(const char *name, int value);
 
 /* Scratch size in bytes for the ws-taking entry points: dpd_workspace_bytes(0) suffices for every

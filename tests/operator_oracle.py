@@ -42,11 +42,11 @@ def _fp16_two(v, scale):
     return (h + (v - h).half().double()) / scale
 
 
-def iterate(x, steps=5, coef=COEF, eps=1e-7, form="exact"):
+def iterate(x, steps=5, coef=COEF, eps=1e-7, form="exact", device="cpu"):
     """The iterate of one matrix in 64 bits.  form "fp16" / "two": X, A and B rounded as the kernels' factors are (to one
     fp16 value or to two, scaled by S and by 4096), "fp32": to fp32; everything else exact.  The distance of such a result
     from the exact one is what those roundings do to this matrix."""
-    x = x.double().cpu()
+    x = x.double().to(device)
     flip = x.shape[0] > x.shape[1]
     if flip:
         x = x.t()

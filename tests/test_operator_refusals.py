@@ -168,3 +168,8 @@ def test_serving_workspace_formula():
     for m, n, k in ((0, 4, 1), (1, 4, 1), (7, 9, 128), (64, 3, 129), (1000, 5, 4096)):
         assert L.lib().dpd_int8_linear_workspace_bytes(m, n, k) == m * _row_bytes(k) + (m * 4 + 255) // 256 * 256 + 256
         assert L.lib().dpd_int8_row_bytes(k) == _row_bytes(k)
+
+
+def test_product_tile_option():
+    for value, code in ((10, 0), (0, 0), (11, 1), (-2, 1), (-1, 0)):
+        assert L.lib().dpd_set_option(b"product_tile", value) == code
