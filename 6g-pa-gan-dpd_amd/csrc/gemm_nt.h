@@ -15,8 +15,11 @@
 // hit 16 different 16-byte columns of the 256-byte bank row, for the row orders of both operands (measured: no conflicts).
 //
 // Operands of a product in a split form (SPLIT): a row holds blocks of 32 elements, first their leading halves (64
-// bytes), then their remainders (64 bytes).  A step then carries 32 elements, and the three products lead*lead,
-// lead*rest, rest*lead go into one accumulator: fp16 halves of a scaled fp32 value give 22 bits of it.
+// bytes), then their remainders (64 bytes), held times REST.  A step then carries 32 elements; the product lead*lead goes into
+// one accumulator, lead*rest and rest*lead into another, which joins the first divided by REST at the end.  The two halves
+// give 22 bits of every scaled value of at least 2^-14, the smallest normal fp16 number, and an absolute 2^-36 below; without
+// REST a remainder would be a subnormal below 2^-3 already, and an iterate's rows of a hundredth of the others' size would be 2.5e-6
+// off instead of 1.1e-7 (150 x 300; fp32 sums 0.7e-7).  The second accumulator leaves no registers for tiles above 256 x 128.
 //
 // Lane layout of the results: the B rows are the first operand of the instruction, so a lane of a 16 x 16 block holds
 // one row m = lane & 15 and four columns.  The B rows of a pair of blocks are interleaved in fours, so that the pair gives
@@ -82,6 +85,7 @@ struct Args {
 };
 
 constexpr int STEP = 128;                                   // bytes of a row per step
+constexpr float REST = 2048.f;                              // scale of the remainders of a split form: at most half a step of the leading half
 
 // Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, and
 // inside a run the tiles go down bands of 8 tile rows, so that the operands of neighbours meet in one L2.  `lower`: the
@@ -189,13 +193,20 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = typename Acc<KIND>::type{0, 0, 0, 0};
+    constexpr bool SPLIT = KIND == F16_SPLIT;
+    f32x4 cross[SPLIT ? TM : 1][SPLIT ? TN : 1];           // the products with remainders
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) cross[i][j] = f32x4{0, 0, 0, 0};
+    }
 
     // fragment c (0 or 1) of block i of A, of block j of B: the keys do not depend on i and j
     const int r = lane & 15, q = lane >> 4;
     const char *pa = mine + (wm * TM * 16 + r) * STEP, *pb = mine + (BM + wn * TN * 16) * STEP;
     const int ka[2] = {(q ^ key_a(r)) * 16, ((4 + q) ^ key_a(r)) * 16};
     const int kb[2] = {b_row(0, r) * STEP + (q ^ key_b(b_row(0, r))) * 16, b_row(0, r) * STEP + ((4 + q) ^ key_b(b_row(0, r))) * 16};
-    constexpr bool SPLIT = KIND == F16_SPLIT;
     i32x4 a0[SPLIT ? 2 : TM], b0[TN], a1[SPLIT ? 2 : TM], b1[TN];
     auto reada = [&](i32x4 *a, int k, int i, int at, int c) { a[k] = *(const i32x4 *)(pa + at + i * 16 * STEP + ka[c]); };
     auto readb = [&](i32x4 *b, int j, int at, int c) { b[j] = *(const i32x4 *)(pb + at + b_row(j, 0) * STEP + kb[c]); };
@@ -203,11 +214,11 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma<KIND>(b[j], a[i], acc[i][j]);
     };
-    auto mul3 = [&](int i, int j, int count) {             // small terms first; blocks j .. j + count - 1 in turn
+    auto mul3 = [&](int i, int j, int count) {             // blocks j .. j + count - 1 in turn
 #pragma unroll
-        for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b1[k], a0[i & 1], acc[i][k]);
+        for (int k = j; k < j + count; ++k) cross[i][k] = mfma<F16_SPLIT>(b1[k], a0[i & 1], cross[i][k]);
 #pragma unroll
-        for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b0[k], a1[i & 1], acc[i][k]);
+        for (int k = j; k < j + count; ++k) cross[i][k] = mfma<F16_SPLIT>(b0[k], a1[i & 1], cross[i][k]);
 #pragma unroll
         for (int k = j; k < j + count; ++k) acc[i][k] = mfma<KIND>(b0[k], a0[i & 1], acc[i][k]);
     };
@@ -346,6 +357,10 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
     if constexpr (SPLIT) {
         for (; s + STAGES < steps; ++s) step_split(s, Yes{});
         for (; s < steps; ++s) step_split(s, No{});
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] += cross[i][j] * (1.f / REST);
     } else {
         for (; s + STAGES < steps; ++s) step(s, Yes{});
         for (; s < steps; ++s) step(s, No{});
@@ -420,7 +435,7 @@ DEV void gemm_tile(const Args &g, const Epilogue &epi) {
                             float v = acc[i][j][e];
                             if (SPLIT) {
                                 asm volatile("" : "+v"(v));    // nothing of one pass is kept for the other: registers
-                                v -= half ? (float)(_Float16)v : 0.f;
+                                if (half) v = (v - (float)(_Float16)v) * REST;
                             }
                             mine_t[((j >> 1) * 32 + (j & 1) * 4 + e) * PITCH + i * 16] = (_Float16)v;
                         }
@@ -457,7 +472,10 @@ static int launch(Args g, int batch, const Epilogue &epi, hipStream_t st) {
 // Which tile: the one whose rounds over the 256 compute units are estimated to take least.  A round has one workgroup on
 // every compute unit, or two where 80 KB of LDS hold one; it takes steps * per + fixed.  Measured with full rounds of 1024 to
 // 4096 rows, fp16 operands (int8 and bf16 take the same time a step) and the split form, us; the fixed part of the fourth one's
-// split form with an epilogue that stores both orientations (3 x 777 x 1000: 30.4 us, 27.6 with the fifth).
+// split form with an epilogue that stores both orientations (3 x 777 x 1000: 30.4 us, 27.6 with the fifth).  The lines were
+// fitted at 12 steps and more and say too little for fewer.  Iterations in the split form with every tile forced in turn, us,
+// the rule's against the best: 3 of 777 x 1000 325, 303; 1024 x 4096 408, 405; 2048 x 2048 754, 749; 4096 x 4096 4258, 4086; 8 of
+// 500 x 700 286, 275; 300 x 400 122, 102.
 struct Round {
     float per, fixed;
 };
@@ -467,9 +485,9 @@ struct Tile {
     Round split_one, split_two;
 };
 constexpr Tile TILES[] = {
-    {256, 256, {1.35f, 10.f}, {}, {2.2f, 7.f}, {}},
+    {256, 256, {1.35f, 10.f}, {}, {}, {}},                                    // no registers for two accumulators: not split
     {256, 128, {0.885f, 6.4f}, {}, {1.28f, 4.8f}, {}},
-    {192, 192, {0.94f, 7.f}, {}, {1.28f, 8.f}, {}},
+    {192, 192, {0.94f, 7.f}, {}, {}, {}},                                     // nor this one
     {128, 128, {0.48f, 4.4f}, {}, {0.615f, 7.5f}, {}},
     {128, 128, {0.685f, 1.2f}, {0.904f, 5.6f}, {0.7f, 4.f}, {1.33f, 2.2f}},
     {128, 64, {0.32f, 3.1f}, {0.565f, 3.8f}, {0.4175f, 2.8f}, {0.7075f, 4.1f}},
@@ -505,16 +523,17 @@ static inline int best_tile(const Args &g, int batch, bool split) {
 template <int KIND, class Epilogue>
 static int product(const Args &g, int batch, const Epilogue &epi, hipStream_t st) {
     constexpr bool SPLIT = KIND == F16_SPLIT;
-    switch (best_tile(g, batch, SPLIT)) {
-    case 0: return launch<KIND, 256, 256, 2, 4, 1, 2>(g, batch, epi, st);
+    const int tile = best_tile(g, batch, SPLIT);
+    if constexpr (!SPLIT) {
+        if (tile == 0) return launch<KIND, 256, 256, 2, 4, 1, 2>(g, batch, epi, st);
+        if (tile == 2) return launch<KIND, 192, 192, 4, 2, 1, 3>(g, batch, epi, st);
+        if (tile == 6) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
+    }
+    switch (tile) {
     case 1: return launch<KIND, 256, 128, 4, 2, 1, 3>(g, batch, epi, st);
-    case 2: return launch<KIND, 192, 192, SPLIT ? 2 : 4, 2, 1, 3>(g, batch, epi, st);
     case 3: return launch<KIND, 128, 128, 2, SPLIT ? 2 : 4, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
     case 4: return launch<KIND, 128, 128, 2, 4, 1, 2>(g, batch, epi, st);
     case 5: return launch<KIND, 128, 64, 2, 2, 1, 3>(g, batch, epi, st);
-    case 6:
-        if constexpr (!SPLIT) return launch<KIND, 96, 96, 2, 3, 2, 3>(g, batch, epi, st);
-        [[fallthrough]];
     case 7: return launch<KIND, 64, 64, 2, 2, 2, 4>(g, batch, epi, st);
     case 8: return launch<KIND, 64, 64, 2, 2, SPLIT ? 2 : 1, SPLIT ? 2 : 4>(g, batch, epi, st);
     case 9: return launch<KIND, 64, 32, 2, 1, 4, 3>(g, batch, epi, st);

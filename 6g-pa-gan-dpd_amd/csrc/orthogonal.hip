@@ -4,18 +4,20 @@
 //
 // Matrices of up to 64 x 128 run in one workgroup, in fp32 out of LDS.  Larger ones that fit into the LDS of a compute unit as
 // fp16 factors run in one workgroup as well (one launch instead of 17 that wait for each other: 128 x 128 fp32 61 us
-// instead of 102).  The others take three tiled products a step (gemm_nt.h).  The factors of both are fp16, scaled by powers of two so that the range is used: after the division by its
-// norm a matrix has entries around 1 / sqrt(r c) and singular values that stay below 4, so X is held times
-// S = 2^floor(log2 sqrt(r c)) (at most 2^14) and A, B = b A + c A A times 2^12.  One fp16 term has a relative rounding of
-// 2^-11, an eighth of that of bf16 inputs; two terms (the split form of gemm_nt.h) hold 22 bits and match an fp32
-// evaluation.  Sums are fp32 in the matrix cores, the norm is a sum of fp64.
+// instead of 102).  The others take three tiled products a step (gemm_nt.h).  The factors of both are fp16, scaled by powers of
+// two so that the range is used: the iterates' singular values, and with them the entries, stay below 3.9, so X is held times
+// S = 2^14 and A, B = b A + c A A (below 15.3) times 2^12.  One fp16 term has a relative rounding of 2^-11, an eighth of that of
+// bf16 inputs.  Two terms (the split form of gemm_nt.h) hold 22 bits of every entry of X above 2^-28 of the matrix's norm and an
+// absolute 2^-50 of the norm below, so that rows and columns far smaller than the others come out as accurate as an fp32
+// evaluation has them (1000 x 1000, half of the rows times 1e-2, 1e-4, 1e-6, 1e-8: 1.4e-7, 1.4e-7, 4.3e-7, 4.4e-5 off;
+// fp32 0.9e-7).  Sums are fp32 in the matrix cores, the norm is a sum of fp64.
 #include <cmath>
 #include <utility>
 #include "gemm_nt.h"
 
 namespace {
 
-constexpr float T_SCALE = 4096.f;
+constexpr float S_SCALE = 16384.f, T_SCALE = 4096.f;
 constexpr int MAX_STEPS = 32, NORM_BLOCKS = 512;
 
 struct Coef {
@@ -275,21 +277,21 @@ struct Plane {                          // a factor in LDS
         if (SPLIT) {
             const nt::f16x4 b = *(const nt::f16x4 *)(l + row * pitch + col);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += (float)b[e];
+            for (int e = 0; e < 4; ++e) v[e] += (float)b[e] * (1.f / nt::REST);
         }
         return v;
     }
     DEV void put4(int row, int col, f32x4_t v) const {
         nt::f16x4 a, b;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = (_Float16)v[e], b[e] = (_Float16)(v[e] - (float)a[e]);
+        for (int e = 0; e < 4; ++e) a[e] = (_Float16)v[e], b[e] = (_Float16)((v[e] - (float)a[e]) * nt::REST);
         *(nt::f16x4 *)(h + row * pitch + col) = a;
         if (SPLIT) *(nt::f16x4 *)(l + row * pitch + col) = b;
     }
     DEV void put(int row, int col, float v) const {
         const _Float16 a = (_Float16)v;
         h[row * pitch + col] = a;
-        if (SPLIT) l[row * pitch + col] = (_Float16)(v - (float)a);
+        if (SPLIT) l[row * pitch + col] = (_Float16)((v - (float)a) * nt::REST);
     }
 };
 
@@ -302,11 +304,11 @@ struct Block {                          // N x N tiles of a product: tile (ti, t
 template <bool SPLIT, bool DOWN, int N>
 DEV Block<N> block_product(const Plane<SPLIT> &U, int u0, const Plane<SPLIT> &V, int v0, int n, int lane) {
     const int r = lane & 15, q = lane >> 4;
-    Block<N> b;
+    Block<N> b, cross;                  // cross: the products with remainders
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < N; ++j) b.t[i][j] = f32x4_t{0, 0, 0, 0};
+        for (int j = 0; j < N; ++j) b.t[i][j] = cross.t[i][j] = f32x4_t{0, 0, 0, 0};
     const int u_at = (u0 + r) * U.pitch + q * 8, v_at = DOWN ? (q * 8 + (r >> 2)) * V.pitch + v0 + (r & 3) * 4 : (v0 + r) * V.pitch + q * 8;
 #pragma unroll 2
     for (int k = 0; k < n; k += 32) {
@@ -326,21 +328,27 @@ DEV Block<N> block_product(const Plane<SPLIT> &U, int u0, const Plane<SPLIT> &V,
                 if (SPLIT) vl[i] = *(const nt::f16x8 *)(V.l + to);
             }
         }
-        auto add = [&](const nt::f16x8 *v, const nt::f16x8 *u) {
+        auto add = [&](const nt::f16x8 *v, const nt::f16x8 *u, Block<N> &to) {
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < N; ++j) b.t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j], u[i], b.t[i][j], 0, 0, 0);
+                for (int j = 0; j < N; ++j) to.t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[j], u[i], to.t[i][j], 0, 0, 0);
         };
-        if (SPLIT) add(vl, uh), add(vh, ul);
-        add(vh, uh);
+        if (SPLIT) add(vl, uh, cross), add(vh, ul, cross);
+        add(vh, uh, b);
+    }
+    if (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) b.t[i][j] += cross.t[i][j] * (1.f / nt::REST);
     }
     return b;
 }
 
 // A = X X^T (times T_SCALE), then B = b A + c A A in its place, by blocks of N x N tiles: at most one a wave.
 template <bool SPLIT, int N>
-DEV void fit_poly(const Plane<SPLIT> &X, const Plane<SPLIT> &A, int r32, int c32, float S, float cb3, float cc, int wave, int lane) {
+DEV void fit_poly(const Plane<SPLIT> &X, const Plane<SPLIT> &A, int r32, int c32, float cb3, float cc, int wave, int lane) {
     const int i16 = lane & 15, q = lane >> 4, side = r32 / (16 * N), ba = wave / side, bj = wave - ba * side;
     const bool has = wave < side * side;
     auto each = [&](auto f) {
@@ -355,7 +363,7 @@ DEV void fit_poly(const Plane<SPLIT> &X, const Plane<SPLIT> &A, int r32, int c32
         each([&](int i, int j, int row, int col) {
             f32x4_t v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = b.t[i][j][e] * (T_SCALE / (S * S));
+            for (int e = 0; e < 4; ++e) v[e] = b.t[i][j][e] * (T_SCALE / (S_SCALE * S_SCALE));
             A.put4(row, col, v);
         });
     }
@@ -382,16 +390,13 @@ DEV void fit_iterate(const From &from, const To &to, int z, int rows, int cols, 
     const int wave0 = __builtin_amdgcn_readfirstlane(t >> 6);
     Plane<SPLIT> X{lds, lds + r32 * (c32 + 8), c32 + 8}, A;
     A.h = lds + r32 * (c32 + 8) * (SPLIT ? 2 : 1), A.l = A.h + r32 * (r32 + 8), A.pitch = r32 + 8;
-    int log_s = 0;
-    while (log_s < 14 && (int64_t)1 << (2 * log_s + 2) <= (int64_t)r * c) ++log_s;
-    const float S = (float)(1 << log_s);
     for (int e = t; e < r32 * (c32 + 8) * (SPLIT ? 2 : 1) / 8; e += 64 * FIT_WAVES) ((f32x4_t *)lds)[e] = f32x4_t{0, 0, 0, 0};
     double s = 0.0;
     for (int e = t; e < n; e += 64 * FIT_WAVES) {
         const float v = from.first(z, e);
         s += (double)v * (double)v;
     }
-    const double norm = sqrt(group_sum_d<FIT_WAVES>(s, red)), inv = (double)S / (norm > eps ? norm : (norm == norm ? eps : norm));
+    const double norm = sqrt(group_sum_d<FIT_WAVES>(s, red)), inv = (double)S_SCALE / (norm > eps ? norm : (norm == norm ? eps : norm));
     for (int e = t; e < n; e += 64 * FIT_WAVES) {      // the same thread saw the same elements: no barrier for the momentum
         const int i = e / cols, j = e - i * cols;
         const float v = (float)((double)from.again(z, e) * inv);
@@ -404,8 +409,8 @@ DEV void fit_iterate(const From &from, const To &to, int z, int rows, int cols, 
         asm volatile("" : "+s"(wave), "+v"(lane));
         const int i16 = lane & 15, q = lane >> 4;
         const float ca = coef.v[3 * k], cb3 = coef.v[3 * k + 1], cc = coef.v[3 * k + 2];
-        if (r32 <= 64) fit_poly<SPLIT, 1>(X, A, r32, c32, S, cb3, cc, wave, lane);       // 16 tiles for 16 waves
-        else fit_poly<SPLIT, 2>(X, A, r32, c32, S, cb3, cc, wave, lane);
+        if (r32 <= 64) fit_poly<SPLIT, 1>(X, A, r32, c32, cb3, cc, wave, lane);       // 16 tiles for 16 waves
+        else fit_poly<SPLIT, 2>(X, A, r32, c32, cb3, cc, wave, lane);
         const bool last = k + 1 == steps;
         Block<2> x[FIT_BLOCKS];                           // X <- a X + B X, written once every wave has read X
 #pragma unroll
@@ -438,7 +443,7 @@ DEV void fit_iterate(const From &from, const To &to, int z, int rows, int cols, 
                         } else if (row < r) {          // in fp32, where it belongs
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                if (col + e < c) to.put(z, wide ? (int64_t)row * cols + col + e : (int64_t)(col + e) * cols + row, x[h].t[i][j][e] * (1.f / S));
+                                if (col + e < c) to.put(z, wide ? (int64_t)row * cols + col + e : (int64_t)(col + e) * cols + row, x[h].t[i][j][e] * (1.f / S_SCALE));
                         }
                     }
             }
@@ -482,7 +487,7 @@ DEV int64_t img_col(int col) { return SPLIT ? (int64_t)(col >> 5) * 128 + (col &
 template <bool SPLIT>
 struct Eight {                         // eight values of an image as they lie there
     nt::f16x8 h[SPLIT ? 2 : 1];
-    DEV float operator[](int i) const { return SPLIT ? (float)h[0][i] + (float)h[SPLIT ? 1 : 0][i] : (float)h[0][i]; }
+    DEV float operator[](int i) const { return SPLIT ? (float)h[0][i] + (float)h[SPLIT ? 1 : 0][i] * (1.f / nt::REST) : (float)h[0][i]; }
 };
 template <bool SPLIT>
 DEV Eight<SPLIT> img_load8(const Image &im, int z, int64_t row, int col) {
@@ -497,7 +502,7 @@ DEV void img_store8(const Image &im, int z, int64_t row, int col, const float *v
     char *p = im.base + img_row(im, z, row) + img_col<SPLIT>(col);
     nt::f16x8 h, l;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i], l[i] = (_Float16)(v[i] - (float)h[i]);
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i], l[i] = (_Float16)((v[i] - (float)h[i]) * nt::REST);
     *(nt::f16x8 *)p = h;
     if (SPLIT) *(nt::f16x8 *)(p + 64) = l;
 }
@@ -531,7 +536,7 @@ DEV void zero_pads(const Image &im, int z, int row, int rows, int from) {
     }
 }
 
-// X0 = x S / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.  The images
+// X0 = x S_SCALE / max(norm, eps) into both images, P [r, c] and Q = P^T [c, r], zeros behind the rows.  64 x 64 tiles.  The images
 // that the products fill first get the zeros behind their rows here too.  Bound by memory: 4096 x 4096 bf16 18 us (5.5 TB/s,
 // x out of the last-level cache).
 template <class From, bool SPLIT>
@@ -636,7 +641,7 @@ struct NextOut : NoFactors {           // X <- a X + B X into P (in place: a til
 template <bool SPLIT, class To>
 struct LastOut : NoFactors {           // the last step: X in the orientation of the result (P, or Q for tall matrices)
     Image X;
-    float a, scale;                    // scale = 1 / S
+    float a, scale;                    // scale = 1 / S_SCALE
     To to;
     int N;
     typedef Eight<SPLIT> Pre;
@@ -693,15 +698,12 @@ int large(const From &from, const To &to_wide, const To &to_tall, int batch, int
     double *part = (double *)(ws + pl.part);
     const Image P{ws + pl.p, pl.ld_c, r * pl.ld_c}, A{ws + pl.a, pl.ld_r, r * pl.ld_r}, B{ws + pl.b, pl.ld_r, r * pl.ld_r};
     Image Q{ws + pl.q0, pl.ld_r, c * pl.ld_r}, Q2{ws + pl.q1, pl.ld_r, c * pl.ld_r};
-    int log_s = 0;
-    while (log_s < 14 && (int64_t)1 << (2 * log_s + 2) <= (int64_t)r * c) ++log_s;
-    const float S = (float)(1 << log_s);
     const int64_t n = (int64_t)r * c;
     const int blocks = grid_for(n, 256 * 8, NORM_BLOCKS);
     hipLaunchKernelGGL((k_norm<From>), dim3(blocks, 1, batch), dim3(256), 0, st, from, n, part);
     DPD_LAUNCH_CHECK();
     hipLaunchKernelGGL((k_prepare<From, SPLIT>), dim3((unsigned)((c + 63) / 64), (unsigned)((r + 63) / 64), batch), dim3(256), 0, st, from, r, c, part, blocks,
-                       eps, (double)S, P, Q, Q2, A, B);
+                       eps, (double)S_SCALE, P, Q, Q2, A, B);
     DPD_LAUNCH_CHECK();
     auto product = [&](const Image &x, int M, const Image &y, int N, bool symmetric, int many, const auto &epi) {
         nt::Args g{};
@@ -715,16 +717,16 @@ int large(const From &from, const To &to_wide, const To &to_tall, int batch, int
     };
     for (int k = 0; k < steps; ++k) {
         const float *f = coef + 3 * k;
-        int rc = product(P, r, P, r, true, batch, GramOut<SPLIT>{{}, A, T_SCALE / (S * S), r});
+        int rc = product(P, r, P, r, true, batch, GramOut<SPLIT>{{}, A, T_SCALE / (S_SCALE * S_SCALE), r});
         if (!rc) rc = product(A, r, A, r, true, batch, PolyOut<SPLIT>{{}, A, B, f[1], f[2], r});
         if (!rc && k + 1 < steps) {
             rc = product(B, r, Q, c, false, batch, NextOut<SPLIT>{{}, P, Q2, f[0], c});
             std::swap(Q, Q2);
         } else if (!rc) {
-            if (wides) rc = product(B, r, Q, c, false, wides, LastOut<SPLIT, To>{{}, P, f[0], 1.f / S, to_wide, c});
+            if (wides) rc = product(B, r, Q, c, false, wides, LastOut<SPLIT, To>{{}, P, f[0], 1.f / S_SCALE, to_wide, c});
             if (!rc && batch > wides) {
                 const Image q = from_z(Q, wides);
-                rc = product(q, c, from_z(B, wides), r, false, batch - wides, LastOut<SPLIT, To>{{}, q, f[0], 1.f / S, to_tall, r});
+                rc = product(q, c, from_z(B, wides), r, false, batch - wides, LastOut<SPLIT, To>{{}, q, f[0], 1.f / S_SCALE, to_tall, r});
             }
         }
         if (rc) return rc;

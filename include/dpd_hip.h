@@ -416,7 +416,7 @@ int dpd_int8_linear_backward(const void *g, int type, int64_t M, int64_t N, int6
  * on the transposed matrix where rows > cols.  h_coef: steps triples (a, b, c), host memory.  The iterate's singular
  * values are at most 1 at the start; coefficients that could take them above 3.9, or b A + c A A above 15, are refused
  * (DPD_ERR_SHAPE), as are more than 32 steps.  accurate != 0: fp32 accuracy (each factor as two fp16 halves, three
- * products); accurate == 0: factors rounded to fp16 (2^-11), sums in fp32. */
+ * products: 22 bits of every entry above 2^-28 of the matrix's norm, 2^-50 of the norm below); accurate == 0: factors rounded to fp16 (2^-11), sums in fp32. */
 size_t dpd_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int accurate);
 int dpd_orthogonalize(const void *x, int type, int64_t batch, int64_t rows, int64_t cols, int steps, const float *h_coef,
                       double eps, int accurate, void *out, void *ws, size_t ws_bytes, void *stream);

@@ -42,9 +42,18 @@ def _fp16_two(v, scale):
     return (h + (v - h).half().double()) / scale
 
 
+def _bits22(v, scale):
+    """Two values of 11 bits, without a smallest exponent."""
+    def eleven(u):
+        m, e = torch.frexp(u)
+        return torch.ldexp(torch.round(m * 2048) / 2048, e)
+    h = eleven(v)
+    return h + eleven(v - h)
+
+
 def iterate(x, steps=5, coef=COEF, eps=1e-7, form="exact", device="cpu"):
     """The iterate of one matrix in 64 bits.  form "fp16" / "two": X, A and B rounded as the kernels' factors are (to one
-    fp16 value or to two, scaled by S and by 4096), "fp32": to fp32; everything else exact.  The distance of such a result
+    fp16 value or to two, scaled by S and by 4096), "22 bits": to two values of 11 bits each, "fp32": to fp32; everything else exact.  The distance of such a result
     from the exact one is what those roundings do to this matrix."""
     x = x.double().to(device)
     flip = x.shape[0] > x.shape[1]
@@ -55,7 +64,7 @@ def iterate(x, steps=5, coef=COEF, eps=1e-7, form="exact", device="cpu"):
     while log_s < 14 and 1 << (2 * log_s + 2) <= r * c:
         log_s += 1
     S = float(1 << log_s)
-    rnd = {"exact": lambda v, s: v, "fp16": _fp16, "two": _fp16_two, "fp32": lambda v, s: v.float().double()}[form]
+    rnd = {"exact": lambda v, s: v, "fp16": _fp16, "two": _fp16_two, "22 bits": _bits22, "fp32": lambda v, s: v.float().double()}[form]
     triples = coef if isinstance(coef[0], (tuple, list)) else [coef] * steps
     x = rnd(x / max(float(x.norm()), eps), S)
     for k, (a, b, c5) in enumerate(triples):

@@ -331,3 +331,21 @@ def test_the_default_is_off_by_its_types_rounding_alone(r, c, dtype):
     want = oo.iterate(x)
     left = ((orthogonalize(x.to(DEV)).double().cpu() - want).abs() - U[dtype] * want.abs()).clamp_min(0.0)
     assert float(left.norm()) <= (1 + U[dtype]) * allowed(x, want, True), (float(left.norm()), float(want.norm()))
+
+
+@pytest.mark.parametrize("small_part", [1e-2, 1e-3, 1e-4, 1e-6])
+@pytest.mark.parametrize("along", ["rows", "columns"])
+@pytest.mark.parametrize("r, c", [(40, 60), (100, 120), (150, 300), (410, 260)])
+def test_rows_and_columns_far_smaller_than_the_others(r, c, along, small_part):
+    """Every second row or column scaled down: each of them comes out as accurate as the others, relative to itself.  Allowed,
+    as for the whole matrix: three times what rounding X, A and B to fp32 and to 22 bits does to the worst of these rows, and the
+    sums' roundings (max(r, c)^(1/2) 2^-22)."""
+    x = update(r, c, 7)
+    dim = 1 if along == "rows" else 0
+    (x[::2] if dim else x[:, ::2]).mul_(small_part)
+    want = oo.iterate(x)
+    norm = want.norm(dim=dim)
+    worst = lambda y: float(((y - want).norm(dim=dim) / norm).max())
+    tol = 3 * worst(oo.iterate(x, form="fp32")) + 3 * worst(oo.iterate(x, form="22 bits")) + max(r, c) ** 0.5 * 2.0 ** -22 + U[torch.float32]
+    err = worst(orthogonalize(x.to(DEV)).double().cpu())
+    assert err <= tol, (err, tol)
