@@ -208,14 +208,20 @@ class Int8Inference:
         if k < 1 or k > 131071:
             raise ValueError(f"{k} input features; 1 to 131071 keep the 32-bit sum exact")
         self.out_features, self.in_features, self.device = n, k, w.device
-        self.image = torch.zeros(n, _row_bytes(k), dtype=torch.int8, device=w.device)
-        self.image[:, :k] = w
-        self.scale = _check_scale(s, n, w.device, "scale").clone()
+        # held where nobody rebinds them: the calls pass their addresses
+        self._image = torch.zeros(n, _row_bytes(k), dtype=torch.int8, device=w.device)
+        self._image[:, :k] = w
+        self._scale = _check_scale(s, n, w.device, "scale").detach().clone()
         bc, self._bias_type = _check_bias(b, n, w.device)
-        self.bias = None if bc is None else bc.detach().clone()
-        self._w = (self.image.data_ptr(), self.scale.data_ptr(), 0 if self.bias is None else self.bias.data_ptr())
+        self._bias = None if bc is None else bc.detach().clone()
+        self._w = (self._image.data_ptr(), self._scale.data_ptr(), 0 if self._bias is None else self._bias.data_ptr())
         self._fn = L.entry("dpd_int8_linear")
         self._index = self.device.index
+
+    # what is served, to look at; other weights are another engine
+    image = property(lambda self: self._image)
+    scale = property(lambda self: self._scale)
+    bias = property(lambda self: self._bias)
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [..., K] -> [..., N] in the type of x.  `out` (optional: [..., N], contiguous, the type of x, apart from x in

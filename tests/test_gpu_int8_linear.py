@@ -421,3 +421,14 @@ def test_gradients_are_rounded_to_their_type_once(m, n, k, dtype):
     (gx, gxs), (gw, gws), _ = oo.gradients(g, *oo.quantize_rows(x), *oo.quantize_rows(w))
     close(xd.grad, gx, gxs, dtype, n, 2.0 ** -16 + 2.0 ** -24)
     close(wd.grad, gw, gws, dtype, m, 2.0 ** -16 + 2.0 ** -24)
+
+
+def test_the_weights_of_an_engine_are_not_rebound():
+    """The calls use the addresses of what the engine holds, so nothing else can take its place (and free it)."""
+    eng = Int8Inference({**dict(zip(("weight", "scale"), quantize_rows_int8(tokens(8, 32, torch.float32, 20).to(DEV)))), "bias": torch.ones(8, device=DEV)})
+    x = tokens(4, 32, torch.float32, 21).to(DEV)
+    want = eng(x)
+    for name in ("scale", "image", "bias"):
+        with pytest.raises(AttributeError):
+            setattr(eng, name, torch.zeros_like(getattr(eng, name)))
+    assert torch.equal(eng(x), want) and eng.scale.shape == (8,) and eng.image.shape == (8, 128) and torch.equal(eng.bias, torch.ones(8, device=DEV))

@@ -173,3 +173,10 @@ def test_serving_workspace_formula():
 def test_product_tile_option():
     for value, code in ((10, 0), (0, 0), (11, 1), (-2, 1), (-1, 0)):
         assert L.lib().dpd_set_option(b"product_tile", value) == code
+
+
+def test_the_weights_of_an_engine_have_no_setter():
+    eng = object.__new__(Int8Inference)
+    for name in ("scale", "image", "bias"):
+        with pytest.raises(AttributeError):
+            setattr(eng, name, torch.zeros(3))
