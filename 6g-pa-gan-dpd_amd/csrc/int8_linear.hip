@@ -845,9 +845,11 @@ extern "C" int dpd_int8_linear_backward(const void *g, int type, int64_t M, int6
     if (!gx && !gw && !gb) return DPD_OK;
     DPD_REQUIRE(g && (!gx || (qw && w_scale)) && (!gw || (qx && x_scale)), DPD_ERR_INVALID_ARG, "int8_linear_backward: null pointer");
     DPD_REQUIRE(ldg >= N && (!gw || ldqx >= K) && (!gx || ldqw >= K), DPD_ERR_INVALID_ARG, "int8_linear_backward: row stride");
-    const int64_t row = planes_for(type) * 2 * nt::pad_to(M > N ? M : N, 64);
-    DPD_REQUIRE(row <= nt::MAX_ROW_BYTES, DPD_ERR_SHAPE, "int8_linear_backward: %lld tokens or %lld output features are too many for one call",
-                (long long)M, (long long)N);
+    // gx sums along the output features, gw along the tokens: so long are the rows of g's images
+    const int64_t row_x = gx ? planes_for(type) * 2 * nt::pad_to(N, 64) : 0, row_w = gw ? planes_for(type) * 2 * nt::pad_to(M, 64) : 0;
+    DPD_REQUIRE(row_x <= nt::MAX_ROW_BYTES, DPD_ERR_SHAPE, "int8_linear_backward: %lld output features are too many for the gradient of x", (long long)N);
+    DPD_REQUIRE(row_w <= nt::MAX_ROW_BYTES, DPD_ERR_SHAPE, "int8_linear_backward: %lld tokens are too many for the weight's gradient in one call",
+                (long long)M);
     DPD_REQUIRE(ws && ws_bytes >= dpd_int8_linear_backward_workspace_bytes(M, N, K, type, gx != nullptr, gw != nullptr, gb != nullptr),
                 DPD_ERR_WORKSPACE, "int8_linear_backward: workspace");
     char *w = (char *)(((uintptr_t)ws + 255) & ~(uintptr_t)255);

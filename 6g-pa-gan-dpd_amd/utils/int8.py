@@ -14,6 +14,8 @@ from .. import _lib as L
 
 TYPES = L.TYPES
 _NEEDS_WORKSPACE = 4            # DPD_ERR_WORKSPACE
+_MOST_OUTS = {torch.float32: 1398080, torch.bfloat16: 2097088, torch.float16: 2097088}      # with a gradient of x
+_MOST_TOKENS = 1 << 20          # of one backward call: bounds its workspace, and below what the weight's gradient can sum over
 
 
 def _type(t: torch.Tensor, what: str) -> int:
@@ -141,22 +143,35 @@ class _Int8LinearFn(torch.autograd.Function):
         dev = kept.device
         g2, ldg = _rows(gy)
         gx = torch.empty((*ctx.lead, k), dtype=tx, device=dev) if need_x else None
-        gw = torch.empty(n, k, dtype=tw, device=dev) if need_w else None
-        gb = torch.empty(n, dtype=tb, device=dev) if need_b else None
         ptr = lambda t: t.data_ptr() if t is not None else 0
         t, (qx, qw, sx, sw) = TYPES[tx], _addresses(kept, m, n, ld)
+        # more tokens than one call takes: in parts, whose weight and bias gradients are added in fp32, in their order
+        part = max(64, min(_MOST_TOKENS, (1 << 35) // max(n, 64) // 64 * 64))
+        whole = m <= part
         with L.device(kept):
-            nbytes = L.entry("dpd_int8_linear_backward_workspace_bytes")(m, n, k, t, need_x, need_w, need_b)
+            gw = torch.empty(n, k, dtype=tw if whole else torch.float32, device=dev) if need_w else None
+            gb = torch.empty(n, dtype=tb if whole else torch.float32, device=dev) if need_b else None
+            nbytes = L.entry("dpd_int8_linear_backward_workspace_bytes")(min(m, part), n, k, t, need_x, need_w, need_b)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            L.check(L.entry("dpd_int8_linear_backward")(
-                g2.data_ptr(), t, m, n, k, ldg, qx, ld, sx, qw, ld, sw, ptr(gx), ptr(gw), TYPES[tw], ptr(gb), TYPES[tb] if need_b else 0,
-                ws.data_ptr(), nbytes, L.raw_stream(dev.index)))
-        return gx, gw, gb
+            type_w, type_b = TYPES[tw if whole else torch.float32], (TYPES[tb if whole else torch.float32] if need_b else 0)
+            size_g, size_x = g2.element_size(), tx.itemsize
+            for at in range(0, max(m, 1), part):
+                w, b = (gw, gb) if at == 0 else (torch.empty_like(gw) if need_w else None, torch.empty_like(gb) if need_b else None)
+                L.check(L.entry("dpd_int8_linear_backward")(
+                    g2.data_ptr() + at * ldg * size_g, t, min(m - at, part), n, k, ldg, qx + at * ld, ld, sx + at * 4, qw, ld, sw,
+                    gx.data_ptr() + at * k * size_x if need_x else 0, ptr(w), type_w, ptr(b), type_b, ws.data_ptr(), nbytes, L.raw_stream(dev.index)))
+                if at:
+                    if need_w:
+                        gw += w
+                    if need_b:
+                        gb += b
+        return gx, gw if whole or not need_w else gw.to(tw), gb if whole or not need_b else gb.to(tb)
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q(x) q(weight)^T + bias in the type of x, both factors quantised by rows in this call; differentiable in x, weight
     and bias with the straight-through estimator (the quantisers count as the identity).  x [..., K], weight [N, K].
+    Any number of tokens; where x has a gradient, up to 1,398,080 (fp32) or 2,097,088 (bf16, fp16) output features.
 
     What a graph captures: the pass may be captured together with its gradients; as with every torch module, an eager graph of
     the same leaf tensors must not be alive then (let go of earlier losses first, or use torch.autograd.grad)."""
@@ -166,6 +181,8 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.device != weight.device:
         raise ValueError(f"cannot apply a weight of shape {tuple(weight.shape)} on {weight.device} to {tuple(x.shape)} on {x.device}")
     _check_bias(bias, weight.shape[0], x.device)
+    if weight.shape[0] > _MOST_OUTS[x.dtype] and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{weight.shape[0]} output features are too many for the gradient of a {x.dtype} x (at most {_MOST_OUTS[x.dtype]})")
     return _Int8LinearFn.apply(x, weight, bias)
 
 

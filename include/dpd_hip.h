@@ -403,7 +403,9 @@ int dpd_int8_linear_forward(const void *x, int type, int64_t M, int64_t K, int64
 /* Its straight-through gradients (the quantisers count as the identity): gx [M, K] = g (qw w_scale) in the type of g,
  * gw [N, K] = g^T (qx x_scale), gb [N] = column sums of g; each may be NULL.  Products on the bf16 matrix cores: the
  * 8-bit factor is exact there, g times a scale is held in two bf16 terms (types bf16 and fp16: 2^-16) or in three (fp32:
- * the whole value); sums in fp32, in a fixed order. */
+ * the whole value); sums in fp32, in a fixed order.  One call takes up to 1,398,080 (fp32) or 2,097,088 (bf16, fp16) output
+ * features where gx is wanted and as many tokens where gw is (DPD_ERR_SHAPE above); the weight's gradient of more tokens is
+ * the sum of the gradients of their parts. */
 size_t dpd_int8_linear_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int type, int need_gx, int need_gw, int need_gb);
 int dpd_int8_linear_backward(const void *g, int type, int64_t M, int64_t N, int64_t K, int64_t ldg, const int8_t *qx, int64_t ldqx,
                              const float *x_scale, const int8_t *qw, int64_t ldqw, const float *w_scale, void *gx, void *gw,

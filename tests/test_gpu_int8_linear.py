@@ -432,3 +432,33 @@ def test_the_weights_of_an_engine_are_not_rebound():
         with pytest.raises(AttributeError):
             setattr(eng, name, torch.zeros_like(getattr(eng, name)))
     assert torch.equal(eng(x), want) and eng.scale.shape == (8,) and eng.image.shape == (8, 128) and torch.equal(eng.bias, torch.ones(8, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m", [(1 << 20) + 777, 2_200_001])
+def test_more_tokens_than_one_backward_call_takes(m, dtype):
+    """Rows of whole numbers with a largest of 127 have the scale 1, and every partial sum below is a whole number of fewer than
+    24 bits: the gradients are exact whatever the order.  (|gw| <= |sum of m terms of at most 127|: a walk of m steps of
+    127 would reach 2^24 only at 114 times its deviation.)"""
+    n, k = 20, 16
+    gen = torch.Generator().manual_seed(60)
+    x, w = torch.randint(-3, 4, (m, k), generator=gen), torch.randint(-3, 4, (n, k), generator=gen)
+    x[:, 0], w[:, 0] = 127, 127
+    g = torch.randint(-1, 2, (m, n), generator=gen)
+    xd, wd, bd = (t.to(dtype).to(DEV).requires_grad_(True) for t in (x, w, torch.zeros(n)))
+    y = int8_linear(xd, wd, bd)
+    for leaves in ((xd, wd, bd), (xd,), (wd,), (bd,)):
+        for t, got in zip(leaves, torch.autograd.grad(y, leaves, g.to(dtype).to(DEV), retain_graph=True)):
+            want = (g.double() @ w.double() if t is xd else g.double().t() @ x.double() if t is wd else g.double().sum(0)).to(dtype)
+            assert got.dtype == dtype and torch.equal(got.cpu(), want)
+
+
+def test_output_features_that_have_no_gradient_of_x_are_refused_before_the_forward():
+    w = torch.ones(1398081, 1, device=DEV, requires_grad=True)
+    x = torch.ones(2, 1, device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="output features"):
+        int8_linear(x, w)
+    with torch.no_grad():
+        assert int8_linear(x, w).shape == (2, 1398081)
+    gw, = torch.autograd.grad(int8_linear(x.detach(), w).sum(), w)
+    assert torch.equal(gw, torch.full_like(w, 2.0))

@@ -180,3 +180,17 @@ def test_the_weights_of_an_engine_have_no_setter():
     for name in ("scale", "image", "bias"):
         with pytest.raises(AttributeError):
             setattr(eng, name, torch.zeros(3))
+
+
+@pytest.mark.parametrize("kind, most", [(0, 1398080), (1, 2097088), (2, 2097088)])
+def test_backward_limits_are_those_of_the_gradients_that_are_wanted(kind, most):
+    """Without a workspace: code 4 says that the sizes are taken, code 2 that they are not."""
+    from dpd_amd.utils.int8 import _MOST_OUTS, _MOST_TOKENS
+    assert most in _MOST_OUTS.values() and _MOST_TOKENS <= most
+
+    def call(m, n, gx=NULL, gw=NULL, gb=NULL):
+        return rc("dpd_int8_linear_backward", PTR, kind, m, n, 16, n, PTR, 128, PTR, PTR, 128, PTR, gx, gw, 0, gb, 0, NULL, 0, NULL)[0]
+    assert call(1 << 24, 4, gx=PTR) == 4 and call(1 << 24, 4, gb=PTR) == 4        # nothing is summed over the tokens; gb by tiles
+    assert call(most, 4, gw=PTR) == 4 and call(most + 1, 4, gw=PTR) == 2
+    assert call(4, most, gx=PTR) == 4 and call(4, most + 1, gx=PTR) == 2
+    assert call(4, 1 << 24, gw=PTR) == 4 and call(4, 1 << 24, gb=PTR) == 4
