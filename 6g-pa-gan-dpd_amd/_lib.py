@@ -152,6 +152,14 @@ def device(t):
     return _HERE_ALREADY if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def refuse_gradient(what, *tensors):
+    """For calls without a gradient: a tensor that asks for one, or carries a forward-mode tangent, is not let pass in silence."""
+    dual = torch.autograd.forward_ad
+    for t in tensors:
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled()) or (getattr(dual, "_current_level", 0) >= 0 and dual.unpack_dual(t).tangent is not None)):
+            raise RuntimeError(f"{what} has no gradient: pass detached tensors")
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

@@ -63,8 +63,11 @@ def _row_bytes(k: int) -> int:
 
 def quantize_rows_int8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) of the rows of x [..., K]: scale = max(max|row|, 2^-100) times fl32(1 / 127) in fp32, q = round-half-even(row / scale)
-    as int8.  A row that holds a NaN or an infinity gets the scale NaN and zeros, so every product with it is NaN."""
+    as int8.  A row that holds a NaN or an infinity gets the scale NaN and zeros, so every product with it is NaN.  The results
+    have no history (`int8_linear` is what has a gradient)."""
     L.need_gpu(x)
+    with torch.no_grad():                # a tangent only: a leaf that is trained may be looked at
+        L.refuse_gradient("quantize_rows_int8", x)
     x = x.detach()
     x2, ldx = _rows(x)
     with L.device(x):
@@ -88,7 +91,8 @@ def _matmul(a, lda, sa, b, ldb, sb, bias, bias_type, m, n, k, dtype):
 def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """a [..., K] int8 with one scale a row, b [N, K] int8 with one scale a row: (a b^T) a_scale b_scale + bias as [..., N].
-    The sum is exact (K <= 131071); scales and bias enter in fp32, and the result is rounded once."""
+    The sum is exact (K <= 131071); scales and bias enter in fp32, and the result is rounded once.  Not differentiable: scales or a
+    bias that require a gradient are refused."""
     L.need_gpu(a, a_scale, b, b_scale, bias)
     if a.dtype != torch.int8 or b.dtype != torch.int8:
         raise RuntimeError(f"int8_matmul takes int8 matrices, got {a.dtype} and {b.dtype}")
@@ -101,6 +105,7 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
     m, n, k = a2.shape[0], b2.shape[0], b2.shape[1]
     sa, sb = _check_scale(a_scale, m, a.device, "a_scale"), _check_scale(b_scale, n, a.device, "b_scale")
     bc, bt = _check_bias(bias, n, a.device)
+    L.refuse_gradient("int8_matmul (training: int8_linear)", sa, sb, bc)
     with L.device(a):
         return _matmul(a2, lda, sa, b2, ldb, sb, bc, bt, m, n, k, out_dtype).view(*a.shape[:-1], n)
 
@@ -252,8 +257,7 @@ class Int8Inference:
             raise ValueError(f"expected {k} input features, got {tuple(shape)}")
         if x.device != self.device:
             raise RuntimeError(f"the weights are on {self.device}, the tokens on {x.device}")
-        if x.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("Int8Inference has no gradient: pass a detached tensor, or train with Int8Linear")
+        L.refuse_gradient("Int8Inference (training: Int8Linear)", x)
         x2, ldx = _rows(x)
         m = x2.shape[0]
         if out is None:

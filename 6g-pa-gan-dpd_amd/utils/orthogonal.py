@@ -49,8 +49,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
         raise RuntimeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
     if x.dim() < 2:
         raise ValueError(f"expected matrices [..., rows, cols], got {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("orthogonalize has no gradient: pass a detached tensor")
+    L.refuse_gradient("orthogonalize", x)
     coef = coefficient_table(coefficients, steps)
     xc = x.detach().contiguous()
     rows, cols = x.shape[-2:]

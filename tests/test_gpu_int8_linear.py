@@ -462,3 +462,26 @@ def test_output_features_that_have_no_gradient_of_x_are_refused_before_the_forwa
         assert int8_linear(x, w).shape == (2, 1398081)
     gw, = torch.autograd.grad(int8_linear(x.detach(), w).sum(), w)
     assert torch.equal(gw, torch.full_like(w, 2.0))
+
+
+def test_gradients_are_not_dropped_in_silence():
+    import torch.autograd.forward_ad as fwd
+    from dpd_amd.utils import orthogonalize
+    x = tokens(4, 32, torch.float32, 21).to(DEV)
+    q, s = quantize_rows_int8(x)
+    eng, leaf = Int8Inference({"weight": q, "scale": s}), lambda t: t.clone().requires_grad_(True)
+    for call in (lambda: int8_matmul(q, leaf(s), q, s), lambda: int8_matmul(q, s, q, leaf(s)), lambda: int8_matmul(q, s, q, s, bias=leaf(s)),
+                 lambda: eng(leaf(x)), lambda: orthogonalize(leaf(x))):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: int8_matmul(q, dual(s), q, s), lambda: int8_matmul(q, s, q, s, bias=dual(s)), lambda: eng(dual(x)), lambda: orthogonalize(dual(x)),
+                     lambda: quantize_rows_int8(dual(x))):
+            with pytest.raises(RuntimeError, match="gradient"):
+                call()
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            int8_linear(dual(x), x)
+        assert torch.equal(eng(x), int8_matmul(q, s, q, s))               # tensors without a tangent pass
