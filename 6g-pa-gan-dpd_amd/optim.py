@@ -22,6 +22,18 @@ def wants_accurate(accurate: Optional[bool], dtype: torch.dtype) -> int:
 _NO_WORKSPACE = 256              # what dpd_muon_workspace_bytes says when no matrix needs one
 
 
+_ADAM_KEYS = frozenset(torch.optim.Adam([torch.zeros(1)]).defaults)
+
+
+def _check_options(o):
+    """The options of a group of matrices."""
+    if not 0.0 <= o["momentum"] < 1.0:
+        raise ValueError(f"momentum must lie in [0, 1), got {o['momentum']}")
+    if o["lr"] < 0.0 or o["weight_decay"] < 0.0 or not o["eps"] > 0.0:
+        raise ValueError(f"lr and weight_decay must not be negative and eps must be positive, got {o['lr']}, {o['weight_decay']}, {o['eps']}")
+    coefficient_table(o["coefficients"], o["steps"])
+
+
 class Muon(torch.optim.Optimizer):
     """For every weight matrix W with gradient G and momentum M (fp32):
 
@@ -29,37 +41,49 @@ class Muon(torch.optim.Optimizer):
         W <- W (1 - lr weight_decay) - lr sqrt(max(1, rows / cols)) O(U),   O = `dpd_amd.utils.orthogonalize`
 
     Parameters that are not matrices (biases) are updated by torch's Adam with the options in `adam`; both kinds are groups
-    of this optimiser, so schedulers and state_dict() cover them.  `params`: tensors, or groups with options of their own.
+    of this optimiser, so schedulers and state_dict() cover them.  `params`: tensors, or groups with options of their own, which
+    hold for the matrices of the group and, where Adam has them (lr, betas, eps, weight_decay, ...), for its other parameters too.
     `accurate`: as for `orthogonalize`, but None means False for bf16 weights, whose own rounding hides the difference.
     The steps of all matrices of up to 64 x 128 take one launch (24 at a time), and so do those of larger ones that fit into a
     compute unit; the others go through tiled products, up to 8 of one size together.  Every result is the same in every run.  A step that is captured into a graph keeps the learning rate it was captured with."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients: Coefficients = COEFFICIENTS, eps: float = 1e-7, accurate: Optional[bool] = None, adam: Optional[Dict] = None):
-        if not 0.0 <= momentum < 1.0:
-            raise ValueError(f"momentum must lie in [0, 1), got {momentum}")
-        if lr < 0.0 or weight_decay < 0.0 or not eps > 0.0:
-            raise ValueError(f"lr and weight_decay must not be negative and eps must be positive, got {lr}, {weight_decay}, {eps}")
-        coefficient_table(coefficients, steps)
         defaults = dict(kind="matrix", lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                         coefficients=coefficients, eps=eps, accurate=accurate)
+        _check_options(defaults)
+        self._adam_options = dict(adam if adam is not None else dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True))
         params = list(params)
-        given = params if params and isinstance(params[0], dict) else [{"params": params}]
-        groups, others, seen = [], [], set()
-        for g in given:
+        groups, others = [], []
+        for g in params if params and isinstance(params[0], dict) else [{"params": params}]:
             ps = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
-            if len({id(p) for p in ps} | seen) != len(ps) + len(seen):
-                raise ValueError("a parameter is given twice: its update would run twice at once")
-            seen |= {id(p) for p in ps}
-            rest = {k: v for k, v in g.items() if k != "params"}
-            matrices = [p for p in ps if p.dim() == 2]
-            if matrices:
-                groups.append({**rest, "params": matrices, "kind": "matrix"})
-            others += [p for p in ps if p.dim() != 2]
+            for to, part in ((groups, [p for p in ps if p.dim() == 2]), (others, [p for p in ps if p.dim() != 2])):
+                if part:
+                    to.append({**g, "params": part})
+        super().__init__(groups + others, defaults)
+
+    def add_param_group(self, param_group):
+        """One group for the matrices in it, with its options over the constructor's, and one for the rest, with those of its
+        options that Adam knows over the constructor's `adam`."""
+        ps = param_group["params"]
+        ps = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+        known = {id(p) for g in self.param_groups for p in g["params"]}
+        if len({id(p) for p in ps} | known) != len(ps) + len(known):
+            raise ValueError("a parameter is given twice: its update would run twice at once")
+        rest = {k: v for k, v in param_group.items() if k != "params"}
+        matrices, others = [p for p in ps if p.dim() == 2], [p for p in ps if p.dim() != 2]
+        if matrices:
+            _check_options({**self.defaults, **rest})
         if others:
-            options = torch.optim.Adam(others, **(adam if adam is not None else dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True)))
-            groups += [{**g, "kind": "other"} for g in options.param_groups]
-        super().__init__(groups, defaults)
+            options = {**self._adam_options, **{k: v for k, v in rest.items() if k in _ADAM_KEYS}}
+            adam = {**rest, **torch.optim.Adam(others, **options).param_groups[0], "kind": "other"}
+        if matrices:
+            super().add_param_group({**rest, "params": matrices, "kind": "matrix"})
+        if others:
+            super().add_param_group(adam)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "_adam_options": self._adam_options}      # a copy takes groups too
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)

@@ -194,3 +194,43 @@ def test_backward_limits_are_those_of_the_gradients_that_are_wanted(kind, most):
     assert call(most, 4, gw=PTR) == 4 and call(most + 1, 4, gw=PTR) == 2
     assert call(4, most, gx=PTR) == 4 and call(4, most + 1, gx=PTR) == 2
     assert call(4, 1 << 24, gw=PTR) == 4 and call(4, 1 << 24, gb=PTR) == 4
+
+
+def test_muon_options_of_a_group_hold_for_its_biases():
+    a, b = torch.nn.Linear(6, 5), torch.nn.Linear(5, 4)
+    opt = Muon([{"params": a.parameters(), "lr": 0.7, "weight_decay": 0.0, "steps": 3}, {"params": b.parameters(), "name": "b"}], adam=dict(lr=0.3, weight_decay=0.2))
+    kinds = [(g["kind"], g["lr"], g["weight_decay"], len(g["params"])) for g in opt.param_groups]
+    assert kinds == [("matrix", 0.7, 0.0, 1), ("matrix", 0.02, 0.0, 1), ("other", 0.7, 0.0, 1), ("other", 0.3, 0.2, 1)]
+    assert opt.param_groups[0]["steps"] == 3 and opt.param_groups[1]["name"] == opt.param_groups[3]["name"] == "b"
+    # the biases move as Adam with these options moves them, on the CPU too
+    twin, before = torch.nn.Linear(6, 5), a.bias.detach().clone()
+    twin.bias.data.copy_(before)
+    adam = torch.optim.Adam([twin.bias], lr=0.7, weight_decay=0.0)
+    a.bias.grad = twin.bias.grad = torch.linspace(-1, 1, 5)
+    opt.step()
+    adam.step()
+    assert torch.equal(a.bias, twin.bias) and not torch.equal(a.bias, before)
+
+
+@pytest.mark.parametrize("bad", [dict(momentum=2.0), dict(lr=-1.0), dict(weight_decay=-0.1), dict(eps=0.0), dict(steps=99), dict(coefficients=(1.0, 2.0))])
+def test_muon_checks_the_options_of_groups(bad):
+    net, more = torch.nn.Linear(6, 5), torch.nn.Linear(5, 4)
+    with pytest.raises(ValueError):
+        Muon([{"params": [net.weight], **bad}])
+    opt = Muon(net.parameters())
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": list(more.parameters()), **bad})
+    assert len(opt.param_groups) == 2
+
+
+def test_muon_takes_groups_later():
+    import copy
+    net, more = torch.nn.Linear(6, 5), torch.nn.Linear(5, 4)
+    first = Muon(net.parameters(), adam=dict(lr=0.3))
+    for opt in (first, copy.deepcopy(first)):
+        opt.add_param_group({"params": list(more.parameters()), "lr": 0.5})
+        assert [(g["kind"], g["lr"]) for g in opt.param_groups] == [("matrix", 0.02), ("other", 0.3), ("matrix", 0.5), ("other", 0.5)]
+        with pytest.raises(ValueError, match="twice"):
+            opt.add_param_group({"params": [more.weight, more.weight]})
+    with pytest.raises(ValueError, match="twice"):
+        first.add_param_group({"params": [net.bias]})
