@@ -100,12 +100,20 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        others = []
+        # everything is looked at before the first weight changes
+        calls, others = [], []
         for group in self.param_groups:
             if group["kind"] == "matrix":
-                self._matrices(group)
+                calls += self._calls(group)
             else:
                 others.append(group)
+                if any(p.grad is not None and p.grad.is_sparse for p in group["params"]):
+                    raise ValueError("a dense gradient is expected")
+        if len(calls) > 1:
+            for call in calls:
+                self._launch(call, check_only=True)
+        for call in calls:
+            self._launch(call)
         if others:
             adam = getattr(self, "_adam", None)
             if adam is None:
@@ -114,7 +122,8 @@ class Muon(torch.optim.Optimizer):
             adam.step()
         return loss
 
-    def _matrices(self, group):
+    def _calls(self, group):
+        """What the library is called with for this group's matrices: one call for each type and device."""
         sets: Dict = {}
         types, state, fp32 = L.TYPES, self.state, torch.float32
         seen = last = None
@@ -152,17 +161,29 @@ class Muon(torch.optim.Optimizer):
             at_m.append(m.data_ptr())
             rows.append(shape[0])
             cols.append(shape[1])
-        for (dtype, index), (ps, _, at_p, at_g, at_m, rows, cols) in sets.items():
-            n = len(ps)
-            pointers, sizes = _PTR * n, _I64 * n
-            h_rows, h_cols = sizes(*rows), sizes(*cols)
-            acc, steps = wants_accurate(group["accurate"], dtype), int(group["steps"])
-            coef = coefficient_table(group["coefficients"], steps)
-            with L.device(ps[0]):
-                nbytes = L.entry("dpd_muon_workspace_bytes")(n, h_rows, h_cols, acc)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=ps[0].device) if nbytes > _NO_WORKSPACE else None
-                L.check(L.entry("dpd_muon_step")(
-                    n, pointers(*at_p), pointers(*at_g), pointers(*at_m), h_rows, h_cols, types[dtype], float(group["lr"]),
-                    float(group["momentum"]), int(group["nesterov"]), float(group["weight_decay"]), steps, coef, float(group["eps"]), acc,
-                    0 if ws is None else ws.data_ptr(), nbytes, L.raw_stream(index)))
+        for ps, _, at_p, *_ in sets.values():
+            if len(set(at_p)) != len(ps):
+                raise ValueError("two weights share their memory: their updates would run at once")
+        if not sets:
+            return []
+        steps = int(group["steps"])
+        return [(key, lists, group, steps, coefficient_table(group["coefficients"], steps)) for key, lists in sets.items()]
+
+    def _launch(self, call, check_only=False):
+        """The call; or, with no matrices, what it says to the options."""
+        (dtype, index), (ps, _, at_p, at_g, at_m, rows, cols), group, steps, coef = call
+        n = 0 if check_only else len(ps)
+        pointers, sizes = _PTR * n, _I64 * n
+        if check_only:
+            at_p = at_g = at_m = rows = cols = ()
+        h_rows, h_cols = sizes(*rows), sizes(*cols)
+        acc = wants_accurate(group["accurate"], dtype)
+        with L.device(ps[0]):
+            nbytes = L.entry("dpd_muon_workspace_bytes")(n, h_rows, h_cols, acc)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=ps[0].device) if nbytes > _NO_WORKSPACE else None
+            L.check(L.entry("dpd_muon_step")(
+                n, pointers(*at_p), pointers(*at_g), pointers(*at_m), h_rows, h_cols, L.TYPES[dtype], float(group["lr"]),
+                float(group["momentum"]), int(group["nesterov"]), float(group["weight_decay"]), steps, coef, float(group["eps"]), acc,
+                0 if ws is None else ws.data_ptr(), nbytes, L.raw_stream(index)))
+        if not check_only:
             _bump_versions(ps)

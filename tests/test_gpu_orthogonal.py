@@ -349,3 +349,32 @@ def test_rows_and_columns_far_smaller_than_the_others(r, c, along, small_part):
     tol = 3 * worst(oo.iterate(x, form="fp32")) + 3 * worst(oo.iterate(x, form="22 bits")) + max(r, c) ** 0.5 * 2.0 ** -22 + U[torch.float32]
     err = worst(orthogonalize(x.to(DEV)).double().cpu())
     assert err <= tol, (err, tol)
+
+
+def test_muon_refuses_before_the_first_weight_changes():
+    def fresh():
+        ps = [torch.nn.Parameter(update(r, c, r).to(DEV)) for r, c in ((30, 32), (20, 12))] + [torch.nn.Parameter(torch.ones(5, device=DEV))]
+        for p in ps:
+            p.grad = torch.ones_like(p)
+        return ps, [p.detach().clone() for p in ps]
+
+    wild = [(3.4, -4.7, 2.0), (30.0, 0.0, 0.0)]                           # in range only as two triples; refused by the library
+    for groups, spoil in ((lambda ps: [{"params": ps[:1]}, {"params": ps[1:2], "steps": 2, "coefficients": wild}], lambda ps, o: None),
+                          (lambda ps: [{"params": ps[:1]}, {"params": ps[1:2]}], lambda ps, o: o.param_groups[1].update(steps=50)),
+                          (lambda ps: [{"params": ps[:1]}, {"params": ps[1:2]}], lambda ps, o: o.param_groups[1].update(eps=-1.0)),
+                          (lambda ps: [{"params": ps[:1]}, {"params": ps[1:2]}], lambda ps, o: setattr(ps[1], "data", ps[1].data.double())),
+                          (lambda ps: ps, lambda ps, o: setattr(ps[2], "grad", torch.ones(5, device=DEV).to_sparse()))):
+        ps, before = fresh()
+        opt = Muon(groups(ps))
+        spoil(ps, opt)
+        with pytest.raises((ValueError, RuntimeError)):
+            opt.step()
+        torch.cuda.synchronize()
+        assert torch.equal(ps[0], before[0]) and not any(s["momentum_buffer"].any() for s in opt.state.values() if "momentum_buffer" in s)
+    # the same memory under two names would be updated by two workgroups at once
+    ps, before = fresh()
+    other = torch.nn.Parameter(ps[0].data)
+    other.grad = ps[0].grad
+    with pytest.raises(ValueError, match="memory"):
+        Muon([ps[0], other]).step()
+    assert torch.equal(ps[0], before[0])
