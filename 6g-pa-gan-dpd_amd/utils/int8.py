@@ -247,7 +247,7 @@ class Int8Inference:
 
     def __call__(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [..., K] -> [..., N] in the type of x.  `out` (optional: [..., N], contiguous, the type of x, apart from x in
-        memory) receives the result in place of a new tensor."""
+        memory, from its first element to its last) receives the result in place of a new tensor."""
         k, n = self.in_features, self.out_features
         t = TYPES.get(x.dtype)
         if t is None:
@@ -264,8 +264,10 @@ class Int8Inference:
             out = torch.empty((*shape[:-1], n), dtype=x.dtype, device=self.device)
         elif out.shape != (*shape[:-1], n) or out.dtype != x.dtype or not out.is_contiguous() or out.device != x.device or out.requires_grad:
             raise RuntimeError(f"out must be a contiguous {x.dtype} tensor of shape {(*shape[:-1], n)} on {x.device} without gradient")
-        elif out.numel() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
-            raise RuntimeError("out must not share memory with x")
+        elif m:
+            at, to, size = x2.data_ptr(), out.data_ptr(), x.element_size()
+            if at < to + m * n * size and to < at + ((m - 1) * ldx + k) * size:
+                raise RuntimeError("out must not share memory with x")
         qw, sw, b = self._w
         with L.device(x):
             args = (x2.data_ptr(), t, m, k, ldx, qw, sw, b, self._bias_type, n, out.data_ptr(), n)

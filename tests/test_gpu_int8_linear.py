@@ -485,3 +485,27 @@ def test_gradients_are_not_dropped_in_silence():
         with pytest.raises((RuntimeError, NotImplementedError)):
             int8_linear(dual(x), x)
         assert torch.equal(eng(x), int8_matmul(q, s, q, s))               # tensors without a tangent pass
+
+
+def test_serving_into_a_part_of_one_buffer():
+    """x and out may be parts of one allocation, and may not overlap in whatever way they came to."""
+    w = tokens(8, 32, torch.float32, 20).to(DEV)
+    eng = Int8Inference(dict(zip(("weight", "scale"), quantize_rows_int8(w))))
+    x = tokens(4, 32, torch.float32, 21).to(DEV)
+    want = eng(x)
+    buf = torch.empty(32 + 128 + 32, device=DEV)
+    for lo in (0, 160):
+        part, out = buf[32:160].view(4, 32), buf[lo:lo + 32].view(4, 8)
+        part.copy_(x)
+        assert eng(part, out=out) is out and torch.equal(out, want) and torch.equal(part, x)
+    for lo in (1, 32, 100, 159):
+        with pytest.raises(RuntimeError, match="share"):
+            eng(part, out=buf[lo:lo + 32].view(4, 8))
+    rows = buf[:160].view(4, 40)[:, :32]                                  # rows with gaps, the last one without
+    rows.copy_(x)
+    assert torch.equal(eng(rows, out=buf[152:184].view(4, 8)), want)
+    with pytest.raises(RuntimeError, match="share"):
+        eng(rows, out=buf[151:183].view(4, 8))
+    turned = buf[:128].view(32, 4)
+    turned.copy_(x.t())
+    assert torch.equal(eng(turned.t(), out=buf[:32].view(4, 8)), want)    # copied before anything is written
