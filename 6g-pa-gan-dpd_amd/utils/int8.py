@@ -14,6 +14,7 @@ from .. import _lib as L
 
 TYPES = L.TYPES
 _NEEDS_WORKSPACE = 4            # DPD_ERR_WORKSPACE
+_MOST_STRIDE = (1 << 23) - 128  # bytes from row to row of an int8 factor
 _MOST_OUTS = {torch.float32: 1398080, torch.bfloat16: 2097088, torch.float16: 2097088}      # with a gradient of x
 _MOST_TOKENS = 1 << 20          # of one backward call: bounds its workspace, and below what the weight's gradient can sum over
 
@@ -33,6 +34,12 @@ def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= k:
         return x, x.stride(0)
     return x.contiguous().view(-1, k) if x.numel() else x.new_empty(x.shape[:-1].numel(), k), k
+
+
+def _near_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """The same for the product, whose offsets inside a tile of 256 rows have 32 bits: rows further apart are copied."""
+    x2, ld = _rows(x)
+    return (x2, ld) if ld <= _MOST_STRIDE else (x2.contiguous(), x2.shape[1])
 
 
 def _check_scale(s: torch.Tensor, rows: int, device, what: str) -> torch.Tensor:
@@ -100,8 +107,8 @@ def int8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale
         raise RuntimeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     if b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1] or a.device != b.device:
         raise ValueError(f"cannot multiply rows of {tuple(a.shape)} on {a.device} with rows of {tuple(b.shape)} on {b.device}")
-    a2, lda = _rows(a)
-    b2, ldb = _rows(b)
+    a2, lda = _near_rows(a)
+    b2, ldb = _near_rows(b)
     m, n, k = a2.shape[0], b2.shape[0], b2.shape[1]
     sa, sb = _check_scale(a_scale, m, a.device, "a_scale"), _check_scale(b_scale, n, a.device, "b_scale")
     bc, bt = _check_bias(bias, n, a.device)

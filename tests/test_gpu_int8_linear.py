@@ -509,3 +509,13 @@ def test_serving_into_a_part_of_one_buffer():
     turned = buf[:128].view(32, 4)
     turned.copy_(x.t())
     assert torch.equal(eng(turned.t(), out=buf[:32].view(4, 8)), want)    # copied before anything is written
+
+
+def test_matmul_rows_far_apart():
+    (a, sa), (b, sb) = ints(3, 64, 70), ints(5, 64, 71)
+    want, size = oo.matmul(a, sa, b, sb)
+    far = torch.zeros(5, 9_000_000, dtype=torch.int8, device=DEV)
+    far[:3, 16:80], far[:, 100:164] = a.to(DEV), b.to(DEV)
+    x, y = far[:3, 16:80], far[:, 100:164]
+    close(int8_matmul(x, sa.to(DEV), y, sb.to(DEV)), want, size, torch.float32)
+    close(int8_matmul(x[1:2], sa[1:2].to(DEV), y, sb.to(DEV)), want[1:2], size[1:2], torch.float32)

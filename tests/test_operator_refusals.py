@@ -234,3 +234,9 @@ def test_muon_takes_groups_later():
             opt.add_param_group({"params": [more.weight, more.weight]})
     with pytest.raises(ValueError, match="twice"):
         first.add_param_group({"params": [net.bias]})
+
+
+def test_longest_stride_of_the_product():
+    from dpd_amd.utils.int8 import _MOST_STRIDE
+    assert rc("dpd_int8_matmul", *matmul_args(lda=_MOST_STRIDE, K=15))[0] == 4                # a workspace is all that is missing
+    assert rc("dpd_int8_matmul", *matmul_args(lda=_MOST_STRIDE + 1, K=15))[0] == 1
