@@ -304,7 +304,7 @@ template <class T>
 FewPlan few_plan(const T *x, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ld) {
     constexpr int V = 16 / sizeof(T);
     const int waves = ld >= 4096 && N <= 8192 ? 16 : 4;
-    if (M > 16 || M * ld > (waves == 16 ? 8192 : 4096)) return {0, 0};
+    if (M > 16 || M * ld > (waves == 16 ? 8192 : 4096) || (N + 15) / 16 * 64 * waves > UINT32_MAX) return {0, 0};      // a grid has fewer than 2^32 threads
     const int vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && K % V == 0 ? V : 1;
     return M * (K / vec) <= (int64_t)FEW_HELD * 64 * waves ? FewPlan{waves, vec} : FewPlan{0, 0};
 }

@@ -240,3 +240,9 @@ def test_longest_stride_of_the_product():
     from dpd_amd.utils.int8 import _MOST_STRIDE
     assert rc("dpd_int8_matmul", *matmul_args(lda=_MOST_STRIDE, K=15))[0] == 4                # a workspace is all that is missing
     assert rc("dpd_int8_matmul", *matmul_args(lda=_MOST_STRIDE + 1, K=15))[0] == 1
+
+
+def test_one_token_against_more_channels_than_one_grid_covers():
+    """16 channels a workgroup of 256 threads: from 2^28 channels on the tiled product takes the token, with a workspace."""
+    got, msg = rc("dpd_int8_linear", PTR, 0, 1, 16, 16, PTR, PTR, NULL, 0, (1 << 28) + 16, PTR, (1 << 28) + 16, NULL, 0, NULL)
+    assert got == 4 and "workspace" in msg
