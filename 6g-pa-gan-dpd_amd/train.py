@@ -147,7 +147,7 @@ def create_models(config: dict, qat: bool, device):
 def create_optimizers(gen, disc, config: dict):
     o = config["training"]["optimizer"]
     kw = dict(betas=tuple(o.get("betas", [0.0, 0.9])), weight_decay=float(o.get("weight_decay", 1e-5)), fused=True)
-    kind = str(o.get("type", "adam")).lower()
+    kind = str(o.get("type") or "adam").lower()
     if kind == "muon":           # the weight matrices by orthogonalised momentum, the biases by Adam as below
         from .optim import Muon
         mk = lambda net, lr: Muon(net.parameters(), lr=float(o.get("lr_matrix", 2e-3)), momentum=float(o.get("momentum", 0.95)),

@@ -246,3 +246,11 @@ def test_one_token_against_more_channels_than_one_grid_covers():
     """16 channels a workgroup of 256 threads: from 2^28 channels on the tiled product takes the token, with a workspace."""
     got, msg = rc("dpd_int8_linear", PTR, 0, 1, 16, 16, PTR, PTR, NULL, 0, (1 << 28) + 16, PTR, (1 << 28) + 16, NULL, 0, NULL)
     assert got == 4 and "workspace" in msg
+
+
+def test_an_empty_optimizer_type_is_adam():
+    from dpd_amd.train import create_optimizers, load_config
+    config = load_config("")
+    for kind in (None, "", "Adam"):
+        config["training"]["optimizer"] = dict(config["training"]["optimizer"], type=kind)
+        assert all(type(o) is torch.optim.Adam for o in create_optimizers(torch.nn.Linear(3, 2), torch.nn.Linear(3, 2), config))
