@@ -317,7 +317,7 @@ int few_tokens(const T *x, int64_t M, int64_t K, int64_t ldx, int64_t ld, const 
     return DPD_OK;
 }
 
-// More tokens, up to 16 MB of them: as above, but a wave quantises whole rows (the next one is on its way meanwhile), and each
+// More tokens, up to MB blocks of 16: as above, but a wave quantises whole rows (the next one is on its way meanwhile), and each
 // weight fragment meets MB blocks of 16 tokens.  Rows of LDS are 16 bytes longer than the image's, so that 16 of them spread
 // over the banks; the waves' sums take their place at the end.  Bound by latency: 8 tokens of 1024 x 1024 bf16 5.4 us.
 constexpr int SOME_BYTES = 32 * 1024;                   // quantised tokens

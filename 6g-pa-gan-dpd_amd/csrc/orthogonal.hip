@@ -120,7 +120,7 @@ DEV double block_sum_d(double v, double *red) {       // over the 256 threads of
 // ---- small matrices --------------------------------------------------------------------------
 // One workgroup, one matrix, in fp32: r <= c after the transposition, X [r][c], A and B [r][r] in LDS, padded with zeros
 // to whole 16 x 16 blocks.  A wave forms a block with v_mfma_f32_16x16x4_f32 (32 cycles for 4 of the sum's terms: these, the
-// LDS reads in front of them and three barriers a step are the time): 16 terms from one 16-byte read of each factor, lane
+// LDS reads in front of them and four barriers a step are the time): 16 terms from one 16-byte read of each factor, lane
 // q of a row taking terms 4 q .. 4 q + 3 of them, which for both factors is the same order.
 // Row strides are 4 modulo 64 words: 16 rows of 16 bytes touch every bank as often.  32 x 30, 5 steps: 10.4 us.
 constexpr int SMALL_R = 64, SMALL_C = 128, XS = SMALL_C + 4, AS = SMALL_R + 4;
@@ -681,14 +681,14 @@ bool is_small(int64_t rows, int64_t cols) {
     return r <= SMALL_R && c <= SMALL_C;
 }
 
-// `batch` matrices of short side r and long side c, the first `wides` of them with rows <= cols.  `to_wide`, `to_tall`: where
-// the two kinds go, counted from the first of each.
 // One compute unit holds the matrix (it needs no workspace then, like a small one).
 bool fits(int64_t rows, int64_t cols, bool split) {
     const int64_t r = rows < cols ? rows : cols, c = rows < cols ? cols : rows;
     return r <= 128 && c <= 65536 && fit_bytes(r, c, split) <= FIT_LDS && ((r + 31) / 32) * ((c + 31) / 32) <= FIT_WAVES * FIT_BLOCKS;
 }
 
+// `batch` matrices of short side r and long side c, the first `wides` of them with rows <= cols.  `to_wide`, `to_tall`: where
+// the two kinds go, counted from the first of each.
 template <bool SPLIT, class From, class To>
 int large(const From &from, const To &to_wide, const To &to_tall, int batch, int wides, int64_t r64, int64_t c64, int steps, const float *coef, double eps,
           char *ws, hipStream_t st) {
