@@ -435,7 +435,7 @@ int int8_product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
 // ---- gradients ---------------------------------------------------------------------------
 // bf16 planes of a gradient times a scale: 2 for bf16 and fp16 gradients (2^-16, so that the rounding of the result is
 // the only one that shows), 3 for fp32 (the whole value): the planes of a row lie one behind the other along k, the smallest
-// first.  One plane for bf16 would halve the two products (4096 tokens of 4096 x 4096: 364 instead of 574 us for the training
+// first.  One plane for bf16 would halve the two products (4096 tokens of 4096 x 4096: 364 instead of 517 to 574 us for the training
 // pass), but every term would be rounded by 2^-8 and the gradients be 2.3e-3 off in place of 1.7e-3.
 template <class T>
 constexpr int planes_of() { return std::is_same<T, float>::value ? 3 : 2; }
@@ -578,7 +578,7 @@ DEV void transpose_i8(int bx, int by, unsigned (*t)[66], const Turn &a) {
 }
 
 // Everything that the two products of the backward read, in one launch: the images of g, and both 8-bit factors turned.  Bound
-// by memory: 4096 tokens of 4096 x 4096 bf16 move 168 MB in 45 to 49 us (3.4 to 3.7 TB/s).
+// by memory: 4096 tokens of 4096 x 4096 bf16 move 269 MB in 63 to 78 us (3.5 to 4.3 TB/s).
 template <class T>
 __global__ __launch_bounds__(256) void k_backward_images(const T *__restrict__ g, int64_t M, int N, int64_t ldg, bool whole, const float *__restrict__ sw,
                                                          const float *__restrict__ sx, __bf16 *__restrict__ gs, int64_t n_pad, __bf16 *__restrict__ gt,

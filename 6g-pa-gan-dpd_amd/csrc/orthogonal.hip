@@ -3,14 +3,14 @@
 // on the short side of each matrix, and the optimiser step that uses it (momentum, iteration, update of the weights).
 //
 // Matrices of up to 64 x 128 run in one workgroup, in fp32 out of LDS.  Larger ones that fit into the LDS of a compute unit as
-// fp16 factors run in one workgroup as well (one launch instead of 17 that wait for each other: 128 x 128 fp32 61 us
+// fp16 factors run in one workgroup as well (one launch instead of 17 that wait for each other: 128 x 128 fp32 64 us
 // instead of 102).  The others take three tiled products a step (gemm_nt.h).  The factors of both are fp16, scaled by powers of
 // two so that the range is used: the iterates' singular values, and with them the entries, stay below 3.9, so X is held times
 // S = 2^14 and A, B = b A + c A A (below 15.3) times 2^12.  One fp16 term has a relative rounding of 2^-11, an eighth of that of
 // bf16 inputs.  Two terms (the split form of gemm_nt.h) hold 22 bits of every entry of X above 2^-28 of the matrix's norm and an
 // absolute 2^-50 of the norm below, so that rows and columns far smaller than the others come out as accurate as an fp32
-// evaluation has them (1000 x 1000, half of the rows times 1e-2, 1e-4, 1e-6, 1e-8: 1.4e-7, 1.4e-7, 4.3e-7, 4.4e-5 off;
-// fp32 0.9e-7).  Sums are fp32 in the matrix cores, the norm is a sum of fp64.
+// evaluation has them (1000 x 1000, half of the rows times 1e-2, 1e-4, 1e-6: the worst row 3.6e-6, 3.8e-6, 3.1e-6 off, nearly all
+// of it from the sums; times 1e-8: 4.3e-5).  Sums are fp32 in the matrix cores, the norm is a sum of fp64.
 #include <cmath>
 #include <utility>
 #include "gemm_nt.h"
@@ -249,7 +249,7 @@ struct SmallTable {
 // successive columns of one row).  The sums of A and A A run along rows of LDS; that of B X runs down the columns of X,
 // which the transposing read ds_read_b64_tr_b16 gives (4 rows of 16 columns each).  Rows are 16 bytes longer than their
 // padded length, so that 16 of them spread over the banks.  Five barriers a step instead of three launches.  Bound by the one
-// compute unit's LDS reads and by latency: 65 x 65 bf16 22 us (75 with tiled products), 128 x 128 fp32 61, 64 x 512 fp32 74.
+// compute unit's LDS reads and by latency: 65 x 65 with one term 22 us (75 with tiled products), 38 with two; 128 x 128 40 and 64, 64 x 512 52 and 78.
 constexpr int FIT_LDS = 150 * 1024, FIT_WAVES = 16, FIT_BLOCKS = 3;     // blocks of X that a wave holds
 
 __host__ DEV int64_t fit_bytes(int64_t r, int64_t c, bool split) {
@@ -592,9 +592,10 @@ DEV void img_store_half(const Image &im, int z, int64_t row, int col, int half, 
     *(nt::f16x8 *)(im.base + img_row(im, z, row) + img_col<SPLIT>(col) + half * 64) = v;
 }
 // The two symmetric products compute their tiles on and below the diagonal; a tile below it is stored turned as well.
-// 4096 x 4096, fp16 factors: Gram and polynomial 71 to 76 us each (253 tiles of 192 x 192, 0.95 PFLOP/s of what is computed),
-// the update 113 to 120 us (1.2 PFLOP/s); 1024 x 4096: 14.7, 7.2 and 16.6 us; 3 of 777 x 1000 in the split form: 16.5, 15.3
-// and 27 us.
+// 4096 x 4096, one term: Gram and polynomial 71 to 76 us each (253 tiles of 192 x 192, 0.95 PFLOP/s of what is computed),
+// the update 113 to 120 us (1.2 PFLOP/s); 1024 x 4096: 14.7, 7.2 and 16.6 us.  Split form: 245, 255 and 348 us (528 tiles of
+// 128 x 128, 16 of them in a third round; 1.2 PFLOP/s in the update's three products); 33.7, 12.8 and 35.7 us; 3 of 777 x 1000
+// 16.9, 15.9 and 28.0 us.
 template <bool SPLIT>
 struct GramOut : NoFactors {           // A = X X^T (times T_SCALE); zeros behind the rows
     static constexpr bool TURNED = true;
