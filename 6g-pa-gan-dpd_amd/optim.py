@@ -34,6 +34,12 @@ def _check_options(o):
     coefficient_table(o["coefficients"], o["steps"])
 
 
+def _listed(params):
+    if isinstance(params, set):
+        raise TypeError("parameters have to come in an order that is the same in every run; a set has none")
+    return [params] if isinstance(params, torch.Tensor) else list(params)
+
+
 class Muon(torch.optim.Optimizer):
     """For every weight matrix W with gradient G and momentum M (fp32):
 
@@ -53,10 +59,10 @@ class Muon(torch.optim.Optimizer):
                         coefficients=coefficients, eps=eps, accurate=accurate)
         _check_options(defaults)
         self._adam_options = dict(adam if adam is not None else dict(lr=1e-4, betas=(0.0, 0.9), weight_decay=1e-5, fused=True))
-        params = list(params)
+        params = _listed(params)
         groups, others = [], []
         for g in params if params and isinstance(params[0], dict) else [{"params": params}]:
-            ps = [g["params"]] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            ps = _listed(g["params"])
             for to, part in ((groups, [p for p in ps if p.dim() == 2]), (others, [p for p in ps if p.dim() != 2])):
                 if part:
                     to.append({**g, "params": part})
@@ -65,8 +71,7 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, param_group):
         """One group for the matrices in it, with its options over the constructor's, and one for the rest, with those of its
         options that Adam knows over the constructor's `adam`."""
-        ps = param_group["params"]
-        ps = [ps] if isinstance(ps, torch.Tensor) else list(ps)
+        ps = _listed(param_group["params"])
         known = {id(p) for g in self.param_groups for p in g["params"]}
         if len({id(p) for p in ps} | known) != len(ps) + len(known):
             raise ValueError("a parameter is given twice: its update would run twice at once")

@@ -254,3 +254,15 @@ def test_an_empty_optimizer_type_is_adam():
     for kind in (None, "", "Adam"):
         config["training"]["optimizer"] = dict(config["training"]["optimizer"], type=kind)
         assert all(type(o) is torch.optim.Adam for o in create_optimizers(torch.nn.Linear(3, 2), torch.nn.Linear(3, 2), config))
+
+
+def test_muon_takes_no_sets():
+    """Their order changes from run to run, and with it what a saved state belongs to."""
+    net = torch.nn.Linear(6, 5)
+    for params in (set(net.parameters()), [{"params": set(net.parameters())}]):
+        with pytest.raises(TypeError, match="order"):
+            Muon(params)
+    opt = Muon([net.weight])
+    with pytest.raises(TypeError, match="order"):
+        opt.add_param_group({"params": {net.bias}})
+    assert Muon(net.weight).param_groups[0]["params"] == [net.weight]     # one tensor alone
