@@ -19,7 +19,8 @@
 // one accumulator, lead*rest and rest*lead into another, which joins the first divided by REST at the end.  The two halves
 // give 22 bits of every scaled value of at least 2^-14, the smallest normal fp16 number, and an absolute 2^-36 below; without
 // REST a remainder would be a subnormal below 2^-3 already: in an iteration of 150 x 300, X at unit size, the factors' roundings
-// would put rows of a hundredth of the others' size 2.5e-6 off instead of 1.1e-7, rows of a ten-thousandth 2.4e-4.  The second accumulator leaves no registers for tiles above 256 x 128.
+// would put rows of a hundredth of the others' size 2.5e-6 off instead of 1.1e-7, rows of a ten-thousandth 2.4e-4.  The second
+// accumulator leaves no registers for tiles above 256 x 128.
 //
 // Lane layout of the results: the B rows are the first operand of the instruction, so a lane of a 16 x 16 block holds
 // one row m = lane & 15 and four columns.  The B rows of a pair of blocks are interleaved in fours, so that the pair gives

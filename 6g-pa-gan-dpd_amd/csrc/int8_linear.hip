@@ -304,7 +304,8 @@ template <class T>
 FewPlan few_plan(const T *x, int64_t M, int64_t N, int64_t K, int64_t ldx, int64_t ld) {
     constexpr int V = 16 / sizeof(T);
     const int waves = ld >= 4096 && N <= 8192 ? 16 : 4;
-    if (M > 16 || M * ld > (waves == 16 ? 8192 : 4096) || (N + 15) / 16 * 64 * waves > UINT32_MAX) return {0, 0};      // a grid has fewer than 2^32 threads
+    if (M > 16 || M * ld > (waves == 16 ? 8192 : 4096)) return {0, 0};
+    if ((N + 15) / 16 * 64 * waves > UINT32_MAX) return {0, 0};                // a grid has fewer than 2^32 threads
     const int vec = ((uintptr_t)x & 15) == 0 && ldx % V == 0 && K % V == 0 ? V : 1;
     return M * (K / vec) <= (int64_t)FEW_HELD * 64 * waves ? FewPlan{waves, vec} : FewPlan{0, 0};
 }
@@ -435,8 +436,8 @@ int int8_product(const int8_t *a, int64_t lda, const float *sa, const int8_t *b,
 // ---- gradients ---------------------------------------------------------------------------
 // bf16 planes of a gradient times a scale: 2 for bf16 and fp16 gradients (2^-16, so that the rounding of the result is
 // the only one that shows), 3 for fp32 (the whole value): the planes of a row lie one behind the other along k, the smallest
-// first.  One plane for bf16 would halve the two products (4096 tokens of 4096 x 4096: 364 instead of 517 to 574 us for the training
-// pass), but every term would be rounded by 2^-8 and the gradients be 2.3e-3 off in place of 1.7e-3.
+// first.  One plane for bf16 would halve the two products (4096 tokens of 4096 x 4096: 364 instead of 517 to 574 us for the
+// training pass), but every term would be rounded by 2^-8 and the gradients be 2.3e-3 off in place of 1.7e-3.
 template <class T>
 constexpr int planes_of() { return std::is_same<T, float>::value ? 3 : 2; }
 
@@ -516,8 +517,8 @@ __global__ __launch_bounds__(256) void k_bias_grad(const float *__restrict__ par
     }
 }
 
-// q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves, which are exact.  A wave takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it
-// turns in registers; the words meet in LDS (4 rows of a column a word) and leave as 16 bytes of 8 rows.  Bound by memory.
+// q [rows, cols] int8 -> out [cols, rows_pad] bf16, zeros behind the rows: the integers themselves, which are exact.  A wave
+// takes 64 x 64, a thread 4 rows of 16 columns, whose bytes it turns in registers; the words meet in LDS (4 rows of a column a word) and leave as 16 bytes of 8 rows.  Bound by memory.
 struct Turn {
     const int8_t *q;
     int64_t rows, ld;

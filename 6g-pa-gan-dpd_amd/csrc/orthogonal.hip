@@ -249,7 +249,8 @@ struct SmallTable {
 // successive columns of one row).  The sums of A and A A run along rows of LDS; that of B X runs down the columns of X,
 // which the transposing read ds_read_b64_tr_b16 gives (4 rows of 16 columns each).  Rows are 16 bytes longer than their
 // padded length, so that 16 of them spread over the banks.  Five barriers a step instead of three launches.  Bound by the one
-// compute unit's LDS reads and by latency: 65 x 65 with one term 22 us (75 with tiled products), 38 with two; 128 x 128 40 and 64, 64 x 512 52 and 78.
+// compute unit's LDS reads and by latency: 65 x 65 with one term 22 us (75 with tiled products), 38 with two;
+// 128 x 128 40 and 64, 64 x 512 52 and 78.
 constexpr int FIT_LDS = 150 * 1024, FIT_WAVES = 16, FIT_BLOCKS = 3;     // blocks of X that a wave holds
 
 __host__ DEV int64_t fit_bytes(int64_t r, int64_t c, bool split) {

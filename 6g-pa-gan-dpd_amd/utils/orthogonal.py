@@ -41,8 +41,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Coefficients = 
     could take a singular value above 3.9 raise ValueError.  `accurate`: fp32 accuracy (the default: 22 bits
     of every entry above 2^-28 of its matrix's norm, an absolute 2^-50 of the norm below), or, with False,
     factors rounded to fp16 with sums in fp32, in a third of the time where the products are large (4096 x 4096: 1.3 instead of
-    4.2 ms; a bf16 matrix comes out 1.9e-3 off, of which the rounding to its type is 1.7e-3; small singular values next to large ones feel the factors'
-    rounding more, since the iteration amplifies them).  Matrices of up to 64 x 128 are
+    4.2 ms; a bf16 matrix comes out 1.9e-3 off, of which the rounding to its type is 1.7e-3; small singular values next to large
+    ones feel the factors' rounding more, since the iteration amplifies them).  Matrices of up to 64 x 128 are
     always computed in fp32.  A matrix that holds a NaN or an infinity comes out as NaN.  Not differentiable."""
     L.need_gpu(x)
     if x.dtype not in L.TYPES:
